@@ -315,6 +315,96 @@ int qe_latent_compose(const void *base, const void *crop, void *out, int64_t h, 
 int qe_latent_crop(const void *src, void *out, int64_t h, int64_t w, int64_t row_bytes, int64_t x0, int64_t y0,
                    int64_t x1, int64_t y1, void *stream);
 
+/* ---- decoding over the paged caches of a batch, and making a cache smaller (device) ----------------
+ *
+ * No counterpart in the reference, which evicts whole prefixes by time of use and leaves text generation to other
+ * processes. dtype codes as below: 1 = bf16, 2 = fp16. head_dim: 64 or 128. heads_q a multiple of heads_kv.
+ *
+ * A draft batch: `batch` requests, request b with lengths[b] cached tokens in pool pages (token t is pool row
+ * tables[b * table_width + t / page_size] * page_size + t % page_size; any page_size >= 1) and the drafted tokens
+ * ("nodes") starts[b] .. starts[b + 1] - 1 of the batch's `total`. What a drafted node sees: every cached token of
+ * its request, and of the request's drafted nodes, by `mode`: 0 the chain up to itself, 1 those whose bit is set in
+ * its row of `masks` ([total][mask_words] 32-bit words, bit j % 32 of word j / 32 = node j of the same request),
+ * 2 all. starts, lengths, tables and masks are device memory and are read when the kernel runs, so a captured graph
+ * replays with their current values; `total` and max_nodes bound the nodes of the batch and of one request,
+ * max_length and sum_length the cached tokens of one request and of all (they size the grid and the split, nothing
+ * past tables' room is read whatever they say: cached tokens past max_length are not attended to). A page outside
+ * the pool reads as zeros and sets bit 1 of *err_flag. */
+typedef struct qe_draft_batch {
+  const int32_t *starts;   /* [batch + 1] */
+  const int32_t *lengths;  /* [batch] */
+  const int32_t *tables;   /* [batch][table_width] page ids; may be null when table_width is 0 */
+  const int32_t *masks;    /* mode 1, else null */
+  int32_t batch, table_width, page_size, mask_words;
+  int32_t mode, total, max_nodes, max_length;
+  int64_t sum_length;
+} qe_draft_batch;
+
+/* masks of mode 1 from the nodes' parents: parents [total] int32, the parent's index within the request or -1 (the
+ * node follows the cache); each parent before its children. A node sees itself and its ancestors. A parent outside
+ * [-1, node) counts as -1 and sets bit 8 of *err_flag. Writes every word of the rows of the batch's nodes. */
+int qe_tree_masks(const int32_t *parents, const int32_t *starts, int32_t batch, int32_t total, int32_t max_nodes,
+                  int32_t mask_words, int32_t *masks, int32_t *err_flag, void *stream);
+
+/* Bytes of device workspace that qe_tree_attention needs for this batch on the current device (0: none); 16-byte
+ * aligned. It is scratch of one call: calls that may overlap need one each. */
+int qe_tree_attention_workspace(qe_draft_batch batch, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+                                int64_t *bytes);
+
+/* Attention of a batch's drafted tokens over [the request's cached tokens; the drafted ones they see]:
+ *   out[i][h] = sum_j softmax_j(scale q[i][h] . K[j][h / G]) V[j][h / G],   G = heads_q / heads_kv
+ * and, optionally, lse[h][i] (fp32, [heads_q][total]), the natural log of the softmax's denominator.
+ *   q    [total][heads_q][head_dim]: element (i, h, d) at q + i * q_token_stride + h * q_head_stride (bytes)
+ *   k_pool / v_pool  one layer's planes, rows of heads_kv x head_dim elements, pool_rows of them
+ *   k_draft / v_draft [total][heads_kv][head_dim] with the given strides, or both null: the nodes see the cache only
+ *   out  strides in bytes. Nodes that see no key get zeros (lse -inf). Rows of q outside the requests' nodes are
+ *        not read and their rows of out and lse are left as they were.
+ * Everything 16-byte aligned with strides that are multiples of 16 bytes. A hidden key contributes nothing, whatever
+ * its K and V hold (NaN and infinities too). Results do not depend on the run. */
+int qe_tree_attention(qe_draft_batch batch, const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                      int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t dtype, const void *k_pool,
+                      const void *v_pool, int64_t pool_rows, const void *k_draft, const void *v_draft,
+                      int64_t draft_token_stride, int64_t draft_head_stride, float scale, void *out,
+                      int64_t out_token_stride, int64_t out_head_stride, float *lse, void *workspace,
+                      int64_t workspace_bytes, int32_t *err_flag, void *stream);
+
+/* The attention weight of every key, from the queries' lse (what qe_tree_attention and qe_paged_attention return):
+ *   w[b][g][j] (+)= sum over request b's nodes i that see j and the G query heads h of K/V head g of
+ *                   exp(scale q[i][h] . K[j][g] - lse[h][i])
+ * j counts the request's cached tokens, then (k_draft not null) its drafted ones. weights: fp32, element (b, g, j) at
+ * weights + b * weights_batch_stride + g * weights_head_stride + j (elements), j < width; with accumulate != 0 the
+ * sums are added to what is there, else positions past the request's keys get 0. width must hold max_length +
+ * (k_draft ? max_nodes : 0). lse [heads_q] rows, lse_head_stride elements apart. A query whose lse is -inf (it saw
+ * nothing) or +inf (taken out by the caller) counts nothing. Sums are fp32, in an order that does not depend on the
+ * run. Other arguments as qe_tree_attention's. */
+int qe_attention_weights(qe_draft_batch batch, const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                         int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t dtype, const void *k_pool,
+                         int64_t pool_rows, const void *k_draft, int64_t draft_token_stride, int64_t draft_head_stride,
+                         const float *lse, int64_t lse_head_stride, float scale, int32_t accumulate, float *weights,
+                         int64_t weights_batch_stride, int64_t weights_head_stride, int64_t width, int32_t *err_flag,
+                         void *stream);
+
+/* Per row the positions a cache of `budget` tokens keeps, in rising order: the first `sinks`, the last `recent`, and
+ * of the others the heaviest (of equal weights the lowest position first; a NaN counts as -inf).
+ *   weights  fp32, row r at weights + (r / (n1 * n2)) * s0 + (r / n2 % n1) * s1 + (r % n2) * s2 (elements), `width`
+ *            values a row; rows = n0 * n1 * n2
+ *   lengths  int32 [rows] positions that row holds (device; clamped to [0, width]), or null: width
+ *   keep     int32 [rows][budget]; where a row holds fewer positions than the budget, the rest is -1
+ *   kept     fp32 [rows][budget] the kept positions' weights (0 beside a -1); may be null
+ * sinks + recent <= budget. */
+int qe_heaviest(const float *weights, int64_t n0, int64_t n1, int64_t n2, int64_t s0, int64_t s1, int64_t s2,
+                int64_t width, const int32_t *lengths, int64_t budget, int64_t sinks, int64_t recent, int32_t *keep,
+                float *kept, void *stream);
+
+/* Moves kept tokens inside a pool, each K/V head its own: for every layer l, K and V, head h and i < n_keep with
+ * p = keep[l][h][i] >= 0:  row dst_slots[i] of the plane, head h = row src_slots[p], head h. keep: int32
+ * [layers][heads][n_keep], contiguous; a negative entry leaves its place as it was; one past n_src, or a slot
+ * outside the pool, is skipped and sets bit 1 of *err_flag. The source and destination slots must not overlap.
+ * pool: plane 2 l + c is layer l's K (c = 0) or V plane; rows of heads x head_bytes; everything 16-byte aligned. */
+int qe_retain(qe_planes pool, int64_t pool_rows, int32_t layers, int32_t heads, int64_t head_bytes,
+              const int64_t *src_slots, int64_t n_src, const int32_t *keep, int64_t n_keep, const int64_t *dst_slots,
+              int32_t *err_flag, void *stream);
+
 /* ---- prefix index: radix tree + slot allocator + LRU eviction (host) -------------------------
  *
  * Restates the behaviour of SGLang's RadixCache (page_size 1 and paged) and TokenToKVPoolAllocator

@@ -31,6 +31,15 @@ class Planes(ctypes.Structure):
                 ("planes_inner", c_int32), ("_pad", c_int32)]
 
 
+class DraftBatch(ctypes.Structure):
+    """``qe_draft_batch``: the cached and drafted tokens of a batch of requests."""
+
+    _fields_ = [("starts", c_void_p), ("lengths", c_void_p), ("tables", c_void_p), ("masks", c_void_p),
+                ("batch", c_int32), ("table_width", c_int32), ("page_size", c_int32), ("mask_words", c_int32),
+                ("mode", c_int32), ("total", c_int32), ("max_nodes", c_int32), ("max_length", c_int32),
+                ("sum_length", c_int64)]
+
+
 _P64 = POINTER(c_int64)
 _P32 = POINTER(c_int32)
 _PU64 = POINTER(c_uint64)
@@ -74,6 +83,18 @@ SIGNATURES: dict[str, list] = {
                                   c_int32, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_int64, c_int64, c_int32,
                                   c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                   c_void_p],
+    "qe_tree_masks": [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p],
+    "qe_tree_attention_workspace": [DraftBatch, c_int32, c_int32, c_int32, _P64],
+    "qe_tree_attention": [DraftBatch, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p,
+                          c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_float, c_void_p, c_int64,
+                          c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
+    "qe_attention_weights": [DraftBatch, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p,
+                             c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_float, c_int32, c_void_p,
+                             c_int64, c_int64, c_int64, c_void_p, c_void_p],
+    "qe_heaviest": [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                    c_int64, c_int64, c_void_p, c_void_p, c_void_p],
+    "qe_retain": [Planes, c_int64, c_int32, c_int32, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                  c_void_p, c_void_p],
     "qe_norm_scale_amax": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                            c_int64, c_int64, c_int64, c_int64, c_float, c_void_p, c_void_p],
     "qe_silu_mul_amax": [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
@@ -181,5 +202,5 @@ def ptr64(array) -> "ctypes._Pointer":
     return array.ctypes.data_as(_P64)
 
 
-__all__ = ["LIB_PATH", "QEError", "Planes", "SIGNATURES", "call", "lib", "on_device", "planes", "ptr64",
+__all__ = ["LIB_PATH", "QEError", "DraftBatch", "Planes", "SIGNATURES", "call", "lib", "on_device", "planes", "ptr64",
            "stream_of", "version", "c_uint8"]

@@ -1,0 +1,686 @@
+// Attention of drafted tokens (one token, a chain or a tree for each request of a batch) over the requests' paged
+// caches.
+//
+// Per request b, drafted node i and query head h (K/V head g = h / G): the scores s_j = scale q . K_j over the cached
+// tokens and the drafted ones the node sees, out = sum_j e^{s_j - m} V_j / sum_j e^{s_j - m}, lse = m + log sum.
+// The G n rows (node, head of the group) of a K/V head share every K and V row, so they are one matrix product with
+// the keys; the keys are split over CTAs and warps, each with its own running maximum and sum, and joined at the end
+// by out = sum_w e^{m_w - m} O_w / sum_w e^{m_w - m} l_w.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstring>
+
+#include "qe_decode.cuh"
+
+namespace qe {
+
+int decode_batch(const char *who, const qe_draft_batch &in, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+                 int32_t dtype, int64_t pool_rows, bool has_pool, int32_t *err, DecodeBatch *out) {
+  QE_CHECK_ARG(in.batch >= 0 && in.batch <= 65535 && in.total >= 0 && in.max_nodes >= 0 && in.max_length >= 0 &&
+                   in.sum_length >= 0 && in.table_width >= 0,
+               "%s: negative size, or more than 65535 requests", who);
+  QE_CHECK_ARG(heads_q >= 1 && heads_kv >= 1 && heads_q % heads_kv == 0 && heads_q <= 65535,
+               "%s: heads_q must be a positive multiple of heads_kv (at most 65535)", who);
+  QE_CHECK_ARG(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128", who);
+  QE_CHECK_ARG(dtype == 1 || dtype == 2, "%s: dtype must be bf16 (1) or fp16 (2)", who);
+  QE_CHECK_ARG(in.mode >= 0 && in.mode <= 2, "%s: mode must be 0, 1 or 2", who);
+  QE_CHECK_ARG(int64_t(in.total) * heads_q < (int64_t(1) << 31), "%s: total x heads_q passes 2^31", who);
+  QE_CHECK_ARG(in.page_size >= 1, "%s: page_size must be at least 1", who);
+  if (in.batch > 0) QE_CHECK_ARG(in.starts && in.lengths, "%s: null starts or lengths", who);
+  if (in.mode == 1 && in.total > 0)
+    QE_CHECK_ARG(in.masks && in.mask_words >= 1 && int64_t(in.mask_words) * 32 >= in.max_nodes,
+                 "%s: mode 1 needs masks of at least max_nodes bits a row", who);
+  if (in.table_width > 0 && in.max_length > 0) {
+    QE_CHECK_ARG(in.tables && has_pool, "%s: null tables or pool plane", who);
+    QE_CHECK_ARG(pool_rows >= in.page_size && pool_rows % in.page_size == 0 && pool_rows < (int64_t(1) << 31),
+                 "%s: pool_rows must be a positive multiple of page_size below 2^31", who);
+  }
+  DecodeBatch d{};
+  d.starts = in.starts;
+  d.lengths = in.lengths;
+  d.tables = in.tables;
+  d.masks = in.masks;
+  d.batch = in.batch;
+  d.table_width = has_pool ? in.table_width : 0;
+  d.page_size = in.page_size;
+  d.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (in.page_size == (1 << s)) d.page_shift = s;
+  d.mask_words = in.mask_words;
+  d.mode = in.mode;
+  d.total = in.total;
+  d.max_nodes = in.max_nodes;
+  d.max_length = in.max_length;
+  d.pool_pages = has_pool && pool_rows > 0 ? int32_t(pool_rows / in.page_size) : 0;
+  d.err = err;
+  *out = d;
+  return QE_OK;
+}
+
+namespace {
+
+// ---- masks of a tree --------------------------------------------------------------------------------------------
+
+// One thread per node: its ancestors have falling indices, so its words are written from the last to the first.
+__global__ void tree_masks_kernel(const int32_t *parents, const int32_t *starts, int total, int max_nodes, int words,
+                                  int32_t *masks, int32_t *err) {
+  const int b = blockIdx.y;
+  const int lo = min(max(starts[b], 0), total);
+  const int hi = min(max(starts[b + 1], lo), total);
+  const int n = min(hi - lo, max_nodes);
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  int32_t *row = masks + int64_t(lo + i) * words;
+  int w = words - 1;
+  uint32_t cur = 0;
+  for (int j = i; j >= 0;) {
+    const int at = j >> 5;
+    if (at < words) {  // words of at least max_nodes bits: always so
+      while (w > at) {
+        row[w--] = int32_t(cur);
+        cur = 0;
+      }
+      cur |= 1u << (j & 31);
+    }
+    int parent = parents[lo + j];
+    if (parent < -1 || parent >= j) {
+      if (err) atomicOr(err, 8);
+      parent = -1;
+    }
+    j = parent;
+  }
+  while (w >= 0) {
+    row[w--] = int32_t(cur);
+    cur = 0;
+  }
+}
+
+// ---- few rows: every warp on its own keys ---------------------------------------------------------------------
+
+constexpr int kWarps = 4;    // per CTA; two CTAs an SM
+constexpr int kStages = 3;   // 16-key tiles (K and V) in flight per warp
+constexpr int kKeys = 16;    // keys per tile
+constexpr float kGrowLog2 = 8.0f;  // a row's reference maximum moves when a score passes it by more than this
+
+struct TreeParams {
+  DecodeBatch batch;
+  const char *q, *k_pool, *v_pool, *k_draft, *v_draft;
+  int64_t q_token, q_head;                    // bytes
+  int64_t pool_row, draft_token, draft_head;  // bytes
+  char *out;
+  int64_t out_token, out_head;  // bytes
+  float *lse;
+  int heads_q, heads_kv, group;
+  int tiles_per_cta;  // 16-key tiles
+  int splits;         // splits of the longest request (the workspace's)
+  float scale_log2;
+  float *part_o;   // [splits][total * heads_q][D]
+  float2 *part_ml;  // [splits][total * heads_q]: (m in log2 units, l)
+};
+
+template <int D>
+__host__ __device__ constexpr int row_bytes() {
+  return D * 2;
+}
+// byte offset of 16-byte chunk c of row r: chunks rotate with the row so that 8 rows' same chunk hit 8 banks
+template <int D>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return uint32_t(r * row_bytes<D>() + ((c ^ (r & 7)) << 4));
+}
+
+__host__ __device__ inline int tiles_of(int len, int drafted) {
+  return (len + kKeys - 1) / kKeys + (drafted + kKeys - 1) / kKeys;
+}
+
+template <int D, int MT>
+__host__ __device__ constexpr int tree_smem_bytes() {
+  return MT * 16 * row_bytes<D>() + kWarps * kStages * 2 * kKeys * row_bytes<D>();
+}
+
+// joins (m, l) pairs: the factor that brings sums at reference m to reference m_all
+__device__ __forceinline__ float join_factor(float m, float m_all) { return m == m_all ? 1.0f : exp2_approx(m - m_all); }
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeParams p) {
+  constexpr int kRow = row_bytes<D>();
+  constexpr int kChunks = D / 8;         // 16-byte chunks of a row
+  constexpr int kSteps = D / 16;         // k-steps of Q K^T
+  constexpr int kTileBytes = kKeys * kRow;
+  constexpr int kCopies = kKeys * kChunks / 32;  // per lane and tile, K or V
+  static_assert(kWarps * MT * 16 * (D + 2) * 4 <= kWarps * kStages * 2 * kTileBytes, "the join fits the ring");
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z, kvh = blockIdx.y % p.heads_kv, row0 = int(blockIdx.y / p.heads_kv) * (MT * 16);
+  grid_dep_wait();
+  grid_dep_launch();
+  const Request rq = request_of(p.batch, b);
+  const int rows = min(rq.n * p.group - row0, MT * 16);
+  if (rows <= 0) return;
+  const int drafted = p.k_draft ? rq.n : 0;
+  const int cached_tiles = (rq.len + kKeys - 1) / kKeys;
+  const int tiles = tiles_of(rq.len, drafted);
+  const int first = int(blockIdx.x) * p.tiles_per_cta;
+  if (first >= tiles && blockIdx.x > 0) return;  // split 0 writes the rows of a request without keys
+  const int last = min(tiles, first + p.tiles_per_cta);
+  const bool whole = tiles <= p.tiles_per_cta;
+
+  const uint32_t q_smem = smem_u32(smem);
+  const uint32_t ring = q_smem + MT * 16 * kRow + warp * (kStages * 2 * kTileBytes);
+
+  // ---- K/V tiles: lanes 0-15 look up a key's row each, every lane copies 16-byte chunks ----
+  const int64_t head_off = int64_t(kvh) * kRow;
+  auto lookup = [&](int t) -> int {  // pool row or drafted token of key `lane` of tile t; -1: nothing there
+    if (t >= last || lane >= kKeys) return -1;
+    if (t < cached_tiles) {
+      const int key = t * kKeys + lane;
+      return key < rq.len ? pool_row(p.batch, b, key) : -1;
+    }
+    const int j = (t - cached_tiles) * kKeys + lane;
+    return j < drafted ? rq.lo + j : -1;
+  };
+  auto copy_tile = [&](int t, int stage, int row) {
+    if (t < last) {
+      const bool cached = t < cached_tiles;
+      const char *kb = cached ? p.k_pool + head_off : p.k_draft + int64_t(kvh) * p.draft_head;
+      const char *vb = cached ? p.v_pool + head_off : p.v_draft + int64_t(kvh) * p.draft_head;
+      const int64_t stride = cached ? p.pool_row : p.draft_token;
+      const uint32_t dst = ring + stage * (2 * kTileBytes);
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int r = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
+        const int at = __shfl_sync(0xffffffffu, row, r);
+        const int64_t off = at < 0 ? 0 : int64_t(at) * stride + c * 16;
+        const uint32_t to = dst + chunk_at<D>(r, c);
+        cp_async16(to, kb + off, at < 0 ? 0 : 16);
+        cp_async16(to + kTileBytes, vb + off, at < 0 ? 0 : 16);
+      }
+    }
+    cp_async_commit();
+  };
+  int t_load = first + warp;
+  int row_next = lookup(t_load);
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    const int row = row_next;
+    row_next = lookup(t_load + kWarps);
+    copy_tile(t_load, s, row);
+    t_load += kWarps;
+  }
+
+  // ---- Q: row r = (node (row0 + r) / G, head (row0 + r) % G of the group) ----
+  for (int i = threadIdx.x; i < MT * 16 * kChunks; i += kWarps * 32) {
+    const int r = i / kChunks, c = i % kChunks;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      const int node = (row0 + r) / p.group, g = (row0 + r) % p.group;
+      v = __ldg(reinterpret_cast<const uint4 *>(p.q + int64_t(rq.lo + node) * p.q_token +
+                                                int64_t(kvh * p.group + g) * p.q_head + c * 16));
+    }
+    *reinterpret_cast<uint4 *>(smem + chunk_at<D>(r, c)) = v;
+  }
+  __syncthreads();
+  // node of each of this thread's rows: rows lane / 4 and lane / 4 + 8 of every 16
+  int node[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) node[m][h] = min((row0 + m * 16 + h * 8 + lane / 4) / p.group, rq.n - 1);
+
+  auto load_q = [&](int m, int k, uint32_t(&a)[4]) {
+    const int r = m * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+    ldmatrix4(a, q_smem + chunk_at<D>(r, 2 * k + (lane >> 4)));
+  };
+  uint32_t qf[MT == 1 ? kSteps : 1][4];  // 16 rows' fragments stay in registers, 32 rows' are read per tile
+  if (MT == 1) {
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) load_q(0, k, qf[MT == 1 ? k : 0]);
+  }
+
+  float o[MT][D / 8][4], m_use[MT][2], l[MT][2];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[m][j][e] = 0.0f;
+    m_use[m][0] = m_use[m][1] = -INFINITY;
+    l[m][0] = l[m][1] = 0.0f;
+  }
+
+  int stage = 0;
+  for (int t = first + warp; t < last; t += kWarps) {
+    cp_async_wait<kStages - 2>();
+    __syncwarp();  // every lane's copies of this tile have landed, and the stage filled next is no longer read
+    {
+      const int row = row_next;
+      row_next = lookup(t_load + kWarps);
+      copy_tile(t_load, (stage + kStages - 1) % kStages, row);
+      t_load += kWarps;
+    }
+    const uint32_t kt = ring + stage * (2 * kTileBytes), vt = kt + kTileBytes;
+    // S = Q K^T: keys 0-7 and 8-15 of the tile
+    float s[MT][2][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[m][j][e] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      uint32_t kb[4];
+      const int r = (lane >> 4) * 8 + (lane & 7);
+      ldmatrix4(kb, kt + chunk_at<D>(r, 2 * k + ((lane >> 3) & 1)));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        uint32_t a[4];
+        if (MT == 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] = qf[MT == 1 ? k : 0][e];
+        } else {
+          load_q(m, k, a);
+        }
+        mma16816<T>(s[m][0], a, kb[0], kb[1]);
+        mma16816<T>(s[m][1], a, kb[2], kb[3]);
+      }
+    }
+    // hidden keys: a score of -inf whatever the product gave
+    const bool draft_tile = t >= cached_tiles;
+    const int left = rq.len - t * kKeys;
+    if (draft_tile || left < kKeys) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t bits = draft_tile ? draft_bits16(p.batch, rq, node[m][h], (t - cached_tiles) * kKeys)
+                                           : (1u << left) - 1u;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (!((bits >> (j * 8 + (lane & 3) * 2 + e)) & 1u)) s[m][j][2 * h + e] = -INFINITY;
+        }
+    }
+    // The reference maximum of a row moves (and its sums scale down) only when a score passes it by more than 2^8:
+    // p stays below 2^8, and most tiles need neither the maximum over the four lanes of a row nor the rescale.
+    bool grow = false;
+    float mx[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mx[m][h] = fmaxf(fmaxf(s[m][0][2 * h], s[m][0][2 * h + 1]), fmaxf(s[m][1][2 * h], s[m][1][2 * h + 1])) *
+                   p.scale_log2;
+        grow |= mx[m][h] > m_use[m][h] + kGrowLog2;
+      }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x = mx[m][h];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          if (x > m_use[m][h]) {
+            const float f = join_factor(m_use[m][h], x);
+            m_use[m][h] = x;
+            l[m][h] *= f;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) {
+              o[m][j][2 * h] *= f;
+              o[m][j][2 * h + 1] *= f;
+            }
+          }
+        }
+    }
+    uint32_t pf[MT][4];  // P as the A operand: rounded to the type of V; the row sums take the unrounded values
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float base = m_use[m][h] == -INFINITY ? 0.0f : -m_use[m][h];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float x = exp2_approx(fmaf(s[m][j][2 * h + e], p.scale_log2, base));
+            s[m][j][2 * h + e] = x;
+            l[m][h] += x;
+          }
+      }
+      pf[m][0] = pack2<T>(s[m][0][0], s[m][0][1]);
+      pf[m][1] = pack2<T>(s[m][0][2], s[m][0][3]);
+      pf[m][2] = pack2<T>(s[m][1][0], s[m][1][1]);
+      pf[m][3] = pack2<T>(s[m][1][2], s[m][1][3]);
+    }
+    if (draft_tile) {
+      // A drafted V that holds an infinity or NaN would reach the rows that do not see it (0 x inf): such values
+      // are taken out of the tile and added, by p x v, to the rows that do.
+      constexpr uint32_t kExp = exponent_bits<T>();
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const uint32_t at = vt + chunk_at<D>((i * 32 + lane) / kChunks, (i * 32 + lane) % kChunks);
+        uint4 v;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "r"(at)
+                     : "memory");
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        bool here = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool lo = (w[e] & kExp) == kExp, hi = ((w[e] >> 16) & kExp) == kExp;
+          here |= lo || hi;
+          w[e] = (lo ? 0u : (w[e] & 0xffffu)) | (hi ? 0u : (w[e] & 0xffff0000u));
+        }
+        if (here) {
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                       : "memory");
+          odd = true;
+        }
+      }
+      __syncwarp();
+      if (__any_sync(0xffffffffu, odd)) {
+        const int j0 = (t - cached_tiles) * kKeys;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t bits = draft_bits16(p.batch, rq, node[m][h], j0);
+#pragma unroll
+            for (int key = 0; key < kKeys; ++key) {
+              // this key's p of the row lies with lane (key % 8) / 2 of the row's four
+              const float pk =
+                  __shfl_sync(0xffffffffu, s[m][key / 8][2 * h + (key & 1)], (lane & ~3) | ((key & 7) >> 1));
+              if (!((bits >> key) & 1u)) continue;
+              const T *v = reinterpret_cast<const T *>(p.v_draft + int64_t(rq.lo + j0 + key) * p.draft_token +
+                                                       int64_t(kvh) * p.draft_head);
+#pragma unroll
+              for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float x = to_float(v[j * 8 + (lane & 3) * 2 + e]);
+                  if (!(fabsf(x) < INFINITY)) o[m][j][2 * h + e] += pk * x;
+                }
+            }
+          }
+      }
+    }
+    // O += P V
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      uint32_t vb[4];
+      const int r = ((lane >> 3) & 1) * 8 + (lane & 7);
+      ldmatrix4_trans(vb, vt + chunk_at<D>(r, 2 * j + (lane >> 4)));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        mma16816<T>(o[m][2 * j], pf[m], vb[0], vb[1]);
+        mma16816<T>(o[m][2 * j + 1], pf[m], vb[2], vb[3]);
+      }
+    }
+    stage = (stage + 1) % kStages;
+  }
+  cp_async_wait<0>();
+
+  // ---- join the warps through shared memory (the ring is free once every warp is here) ----
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[m][h] += __shfl_xor_sync(0xffffffffu, l[m][h], 1);
+      l[m][h] += __shfl_xor_sync(0xffffffffu, l[m][h], 2);
+    }
+  __syncthreads();
+  constexpr int kRows = MT * 16;
+  float *so = reinterpret_cast<float *>(smem + kRows * kRow);     // [warp][row][D]
+  float *sm = so + kWarps * kRows * D, *sl = sm + kWarps * kRows;  // [warp][row]
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = warp * kRows + m * 16 + h * 8 + lane / 4;
+      if ((lane & 3) == 0) {
+        sm[r] = m_use[m][h];
+        sl[r] = l[m][h];
+      }
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+        *reinterpret_cast<float2 *>(so + int64_t(r) * D + j * 8 + (lane & 3) * 2) =
+            make_float2(o[m][j][2 * h], o[m][j][2 * h + 1]);
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (D / 8); i += kWarps * 32) {  // 8 columns of a row each
+    const int r = i / (D / 8), c = (i % (D / 8)) * 8;
+    float m_all = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m_all = fmaxf(m_all, sm[w * kRows + r]);
+    float l_all = 0.0f, acc[8] = {};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = join_factor(sm[w * kRows + r], m_all);
+      l_all += f * sl[w * kRows + r];
+      const float4 *src = reinterpret_cast<const float4 *>(so + int64_t(w * kRows + r) * D + c);
+      const float4 x = src[0], y = src[1];
+      acc[0] += f * x.x, acc[1] += f * x.y, acc[2] += f * x.z, acc[3] += f * x.w;
+      acc[4] += f * y.x, acc[5] += f * y.y, acc[6] += f * y.z, acc[7] += f * y.w;
+    }
+    const int token = rq.lo + (row0 + r) / p.group, head = kvh * p.group + (row0 + r) % p.group;
+    if (whole) {
+      const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;  // no key seen: zeros
+      uint4 v;
+      v.x = pack2<T>(acc[0] * inv, acc[1] * inv);
+      v.y = pack2<T>(acc[2] * inv, acc[3] * inv);
+      v.z = pack2<T>(acc[4] * inv, acc[5] * inv);
+      v.w = pack2<T>(acc[6] * inv, acc[7] * inv);
+      *reinterpret_cast<uint4 *>(p.out + int64_t(token) * p.out_token + int64_t(head) * p.out_head + c * 2) = v;
+      if (p.lse && c == 0)
+        p.lse[int64_t(head) * p.batch.total + token] =
+            l_all == 0.0f ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
+    } else {
+      const int64_t at = (int64_t(blockIdx.x) * p.batch.total + token) * p.heads_q + head;
+      float4 *dst = reinterpret_cast<float4 *>(p.part_o + at * D + c);
+      dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (c == 0) p.part_ml[at] = make_float2(m_all, l_all);
+    }
+  }
+}
+
+// Joins the splits of the requests that have more than one: a warp per (node, head) row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
+  const int lane = threadIdx.x & 31;
+  const int b = blockIdx.y;
+  const int at = int(blockIdx.x) * 8 + int(threadIdx.x >> 5);
+  grid_dep_wait();
+  grid_dep_launch();
+  const Request rq = request_of(p.batch, b);
+  if (at >= rq.n * p.heads_q) return;
+  const int tiles = tiles_of(rq.len, p.k_draft ? rq.n : 0);
+  if (tiles <= p.tiles_per_cta) return;
+  const int splits = min((tiles + p.tiles_per_cta - 1) / p.tiles_per_cta, p.splits);
+  const int token = rq.lo + at / p.heads_q, head = at % p.heads_q;
+  const int64_t row = int64_t(token) * p.heads_q + head, step = int64_t(p.batch.total) * p.heads_q;
+  float m_all = -INFINITY;
+  for (int s = lane; s < splits; s += 32) m_all = fmaxf(m_all, p.part_ml[s * step + row].x);
+#pragma unroll
+  for (int x = 16; x; x >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, x));
+  constexpr int kPer = D / 32;  // columns per lane
+  float acc[kPer] = {}, l_all = 0.0f;
+  for (int s = 0; s < splits; ++s) {
+    const float2 ml = p.part_ml[s * step + row];
+    const float f = join_factor(ml.x, m_all);
+    l_all += f * ml.y;
+    const float *src = p.part_o + (s * step + row) * D + lane * kPer;
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+      const float2 v = *reinterpret_cast<const float2 *>(src + e);
+      acc[e] += f * v.x;
+      acc[e + 1] += f * v.y;
+    }
+  }
+  const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
+  uint32_t *dst = reinterpret_cast<uint32_t *>(p.out + int64_t(token) * p.out_token + int64_t(head) * p.out_head) +
+                  lane * (kPer / 2);
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2) dst[e / 2] = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
+  if (p.lse && lane == 0)
+    p.lse[int64_t(head) * p.batch.total + token] = l_all == 0.0f ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------
+
+struct TreePlan {
+  int m_tiles;        // 16-row tiles per CTA: 1 or 2
+  int tiles_per_cta;  // 16-key tiles
+  int splits;
+  int64_t workspace;
+};
+
+TreePlan tree_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head_dim) {
+  TreePlan t{};
+  const int64_t rows = int64_t(in.max_nodes) * (heads_q / heads_kv);
+  t.m_tiles = rows <= 16 ? 1 : 2;
+  const int64_t row_ctas = std::max<int64_t>(1, (rows + t.m_tiles * 16 - 1) / (t.m_tiles * 16)) * heads_kv;
+  const int64_t max_tiles = std::max(1, tiles_of(in.max_length, in.max_nodes));
+  // tiles of the whole batch, spread over two CTAs per SM
+  const int64_t all = (in.sum_length + kKeys - 1) / kKeys + int64_t(in.batch) * tiles_of(0, in.max_nodes);
+  int64_t per = (all * row_ctas + 2 * sm_count() - 1) / (2 * sm_count());
+  per = std::max<int64_t>((per + kWarps - 1) / kWarps * kWarps, kWarps);
+  if (per >= max_tiles) per = max_tiles;
+  t.tiles_per_cta = int(per);
+  t.splits = int((max_tiles + per - 1) / per);
+  if (t.splits > 1) t.workspace = int64_t(t.splits) * in.total * heads_q * (head_dim + 2) * 4;
+  return t;
+}
+
+template <auto kKernel>
+int launch(dim3 grid, int threads, int smem, cudaStream_t stream, const TreeParams &p, const char *what) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = size_t(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (smem > 48 * 1024) {
+    static std::atomic<bool> raised[64];  // per device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (!raised[dev].load(std::memory_order_relaxed)) {
+      cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return cuda_status(e, what);
+      raised[dev].store(true, std::memory_order_relaxed);
+    }
+  }
+  return cuda_status(cudaLaunchKernelEx(&cfg, kKernel, p), what);
+}
+
+template <typename T, int D>
+int run_tree(const TreeParams &p, const TreePlan &t, const qe_draft_batch &in, cudaStream_t stream) {
+  const int rows = in.max_nodes * p.group;
+  const dim3 grid(unsigned(t.splits), unsigned((rows + t.m_tiles * 16 - 1) / (t.m_tiles * 16) * p.heads_kv),
+                  unsigned(in.batch));
+  const int s = t.m_tiles == 1 ? launch<tree_attention_kernel<T, D, 1>>(grid, kWarps * 32, tree_smem_bytes<D, 1>(),
+                                                                        stream, p, "qe_tree_attention launch")
+                               : launch<tree_attention_kernel<T, D, 2>>(grid, kWarps * 32, tree_smem_bytes<D, 2>(),
+                                                                        stream, p, "qe_tree_attention launch");
+  if (s || t.splits == 1) return s;
+  const dim3 join(unsigned((in.max_nodes * p.heads_q + 7) / 8), unsigned(in.batch));
+  return launch<tree_join_kernel<T, D>>(join, 256, 0, stream, p, "qe_tree_attention join launch");
+}
+
+bool al16(int64_t v) { return v % 16 == 0; }
+
+}  // namespace
+}  // namespace qe
+
+extern "C" int qe_tree_masks(const int32_t *parents, const int32_t *starts, int32_t batch, int32_t total,
+                             int32_t max_nodes, int32_t mask_words, int32_t *masks, int32_t *err_flag, void *stream) {
+  using namespace qe;
+  QE_CHECK_ARG(batch >= 0 && batch <= 65535 && total >= 0 && max_nodes >= 0, "qe_tree_masks: bad size");
+  if (batch == 0 || total == 0 || max_nodes == 0) return ok();
+  QE_CHECK_ARG(parents && starts && masks, "qe_tree_masks: null pointer");
+  QE_CHECK_ARG(int64_t(mask_words) * 32 >= max_nodes, "qe_tree_masks: mask_words hold fewer than max_nodes bits");
+  tree_masks_kernel<<<dim3(unsigned((max_nodes + 127) / 128), unsigned(batch)), 128, 0,
+                      static_cast<cudaStream_t>(stream)>>>(parents, starts, total, max_nodes, mask_words, masks,
+                                                           err_flag);
+  const int s = cuda_status(cudaGetLastError(), "qe_tree_masks launch");
+  return s ? s : ok();
+}
+
+extern "C" int qe_tree_attention_workspace(qe_draft_batch batch, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+                                           int64_t *bytes) {
+  using namespace qe;
+  QE_CHECK_ARG(bytes, "qe_tree_attention_workspace: null pointer");
+  QE_CHECK_ARG(batch.batch >= 0 && batch.total >= 0 && batch.max_nodes >= 0 && batch.max_length >= 0 &&
+                   batch.sum_length >= 0 && heads_q >= 1 && heads_kv >= 1 && heads_q % heads_kv == 0 &&
+                   (head_dim == 64 || head_dim == 128),
+               "qe_tree_attention_workspace: bad size");
+  *bytes = tree_plan(batch, heads_q, heads_kv, head_dim).workspace;
+  return ok();
+}
+
+extern "C" int qe_tree_attention(qe_draft_batch batch, const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                                 int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t dtype,
+                                 const void *k_pool, const void *v_pool, int64_t pool_rows, const void *k_draft,
+                                 const void *v_draft, int64_t draft_token_stride, int64_t draft_head_stride,
+                                 float scale, void *out, int64_t out_token_stride, int64_t out_head_stride, float *lse,
+                                 void *workspace, int64_t workspace_bytes, int32_t *err_flag, void *stream) {
+  using namespace qe;
+  TreeParams p{};
+  QE_CHECK_ARG((k_pool == nullptr) == (v_pool == nullptr) && (k_draft == nullptr) == (v_draft == nullptr),
+               "qe_tree_attention: K and V go together");
+  int s = decode_batch("qe_tree_attention", batch, heads_q, heads_kv, head_dim, dtype, pool_rows, k_pool != nullptr,
+                       err_flag, &p.batch);
+  if (s) return s;
+  if (batch.batch == 0 || batch.total == 0 || batch.max_nodes == 0) return ok();
+  const int64_t row = int64_t(head_dim) * 2;
+  QE_CHECK_ARG(q && out, "qe_tree_attention: null q or out");
+  QE_CHECK_ARG(aligned16(q) && aligned16(out) && aligned16(k_pool) && aligned16(v_pool) && aligned16(k_draft) &&
+                   aligned16(v_draft) && al16(q_token_stride) && al16(q_head_stride) && al16(out_token_stride) &&
+                   al16(out_head_stride) && al16(draft_token_stride) && al16(draft_head_stride),
+               "qe_tree_attention: pointers must be 16-byte aligned with strides of a multiple of 16 bytes");
+  QE_CHECK_ARG(q_head_stride >= row && q_token_stride >= row && out_head_stride >= row && out_token_stride >= row &&
+                   (!k_draft || (draft_head_stride >= row && draft_token_stride >= row)),
+               "qe_tree_attention: strides must hold a row of head_dim");
+  QE_CHECK_ARG(std::isfinite(scale) && scale > 0.0f, "qe_tree_attention: scale must be positive and finite");
+  QE_CHECK_ARG((int64_t(batch.max_nodes) * (heads_q / heads_kv) + 15) / 16 * heads_kv <= 65535,
+               "qe_tree_attention: too many rows (max_nodes x heads_q / 16 passes 65535)");
+  const TreePlan t = tree_plan(batch, heads_q, heads_kv, head_dim);
+  QE_CHECK_ARG(t.workspace == 0 || (workspace && aligned16(workspace) && workspace_bytes >= t.workspace),
+               "qe_tree_attention: needs %lld bytes of 16-byte aligned workspace", (long long)t.workspace);
+  p.q = static_cast<const char *>(q);
+  p.k_pool = static_cast<const char *>(k_pool);
+  p.v_pool = static_cast<const char *>(v_pool);
+  p.k_draft = static_cast<const char *>(k_draft);
+  p.v_draft = static_cast<const char *>(v_draft);
+  p.q_token = q_token_stride;
+  p.q_head = q_head_stride;
+  p.pool_row = row * heads_kv;
+  p.draft_token = draft_token_stride;
+  p.draft_head = draft_head_stride;
+  p.out = static_cast<char *>(out);
+  p.out_token = out_token_stride;
+  p.out_head = out_head_stride;
+  p.lse = lse;
+  p.heads_q = heads_q;
+  p.heads_kv = heads_kv;
+  p.group = heads_q / heads_kv;
+  p.tiles_per_cta = t.tiles_per_cta;
+  p.splits = t.splits;
+  p.scale_log2 = scale * kLog2e;
+  p.part_o = static_cast<float *>(workspace);
+  p.part_ml = reinterpret_cast<float2 *>(p.part_o + int64_t(t.splits) * batch.total * heads_q * head_dim);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == 1)
+    s = head_dim == 128 ? run_tree<__nv_bfloat16, 128>(p, t, batch, st) : run_tree<__nv_bfloat16, 64>(p, t, batch, st);
+  else
+    s = head_dim == 128 ? run_tree<__half, 128>(p, t, batch, st) : run_tree<__half, 64>(p, t, batch, st);
+  return s ? s : ok();
+}

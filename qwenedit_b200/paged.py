@@ -404,6 +404,46 @@ class PagedKVPool:
             t.record_stream(stream)
         table.record_stream(stream)
 
+    def retain(self, indices: torch.Tensor, keep: torch.Tensor, slots: torch.Tensor) -> None:
+        """Moves the kept tokens of a cached sequence to other slots, each layer and K/V head its own choice:
+        ``kv[l, :, slots[i], h] = kv[l, :, indices[keep[l, h, i]], h]`` in one launch (an addition; ``evict.heaviest``
+        makes `keep`, [layers, heads, n] int32 on the device; ``alloc(n)`` makes `slots`). An entry of -1 leaves its
+        place as it was; one past the sequence is skipped and shows in ``device_errors``. `slots` must hold no slot
+        twice and none of `indices`. ``extra`` rows are not moved (a position's hidden row has no head)."""
+        n = slots.numel()
+        if keep.dtype != torch.int32 or tuple(keep.shape) != (self.layers, self.heads, n):
+            raise ValueError(f"keep must be [{self.layers}, {self.heads}, {n}] int32, got {tuple(keep.shape)} "
+                             f"{keep.dtype}")
+        e = self.kv.element_size()
+        if self.head_dim * e % 16:
+            raise ValueError(f"retain needs heads of a multiple of 16 bytes, not {self.head_dim * e}")
+        if n == 0:
+            return
+        self._require_cuda(indices, keep, slots)
+        src, dst = self._host_slots(indices), self._host_slots(slots)
+        for host in (src, dst):
+            if len(host) and (host.min() < 0 or host.max() >= self.rows):
+                raise ValueError(f"slots outside the pool's {self.rows} rows")
+        mark = np.zeros(self.rows, np.int8)
+        mark[src] = 1
+        hit = bool(mark[dst].any())
+        mark[dst] = 2
+        if hit or int(np.count_nonzero(mark == 2)) != n:
+            raise ValueError("retain: `slots` must hold no slot twice and none of `indices`")
+        keep = keep.contiguous()
+        src_t = (indices if indices.dtype == torch.int64 else indices.to(torch.int64)).contiguous()
+        dst_t = (slots if slots.dtype == torch.int64 else slots.to(torch.int64)).contiguous()
+        pool = _lib.planes(self.kv.data_ptr(), self.kv.stride(0) * e, self.kv.stride(1) * e, 2)
+        with _lib.on_device(self.device):
+            _lib.call("qe_retain", pool, self.rows, self.layers, self.heads, self.head_dim * e, src_t.data_ptr(),
+                      src_t.numel(), keep.data_ptr(), n, dst_t.data_ptr(), self._err.data_ptr(), self._stream())
+
+    def free(self, indices: torch.Tensor) -> None:
+        """Gives slots from ``alloc`` that were never given to ``insert`` back to the allocator (an addition: e.g. a
+        request's own cache after ``retain``). In page mode whole pages: all the slots of an ``alloc``."""
+        with self.lock:
+            self.index.free(self._host_slots(indices))
+
     def gather_extra(self, indices: torch.Tensor) -> torch.Tensor:
         """``extra.index_select(0, indices)`` (encoder.py:114) as one gather launch."""
         if self.extra is None:

@@ -1,0 +1,161 @@
+"""What the decoding and cache-eviction operators refuse, on the CPU: bad shapes, types, counts and slots raise before
+any launch, and the C entry points reject bad arguments without touching the GPU."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from qwenedit_b200 import _lib
+from qwenedit_b200.drafts import DraftTree, PagedBatch, tree_attention
+from qwenedit_b200.evict import attention_weights, heaviest
+from qwenedit_b200.paged import PagedKVPool
+
+
+def _pool(page=4, dtype=torch.bfloat16, d=64, heads=2):
+    return PagedKVPool("host", 1, heads, d, 32 * 2 * heads * d * 2, dtype, "cpu", page_size=page)
+
+
+def test_batch_needs_whole_pages_in_the_pool():
+    pool = _pool()
+    run = torch.arange(8, 14)
+    b = PagedBatch(pool, [run, None, torch.empty(0, dtype=torch.int64)])
+    assert b.tables.tolist() == [[2, 3], [-1, -1], [-1, -1]] and b.lengths.tolist() == [6, 0, 0]
+    assert (b.max_length, b.sum_length, b.table_width) == (6, 6, 2)
+    for bad in (torch.tensor([8, 9, 11]), torch.tensor([9, 10]), torch.tensor([8, 9, 10, 11, 13])):
+        with pytest.raises(ValueError, match="whole-page runs"):
+            PagedBatch(pool, [bad])
+    for bad in (torch.tensor([-4, -3]), torch.arange(pool.rows - 1, pool.rows + 1)):
+        with pytest.raises(ValueError, match="outside the pool"):
+            PagedBatch(pool, [bad])
+    for lengths in ([7, 0, 0], [-1, 0, 0], [1, 1, 0], [1, 0]):
+        with pytest.raises(ValueError, match="lengths"):
+            PagedBatch(pool, [run, None, None], lengths)
+    assert PagedBatch(_pool(page=1), [torch.tensor([5, 3, 9])]).tables.tolist() == [[5, 3, 9]]
+
+
+def test_tree_counts_parents_and_masks():
+    t = DraftTree([2, 0, 3], device="cpu")
+    assert t.starts.tolist() == [0, 2, 2, 5] and (t.total, t.max_nodes, t.batch) == (5, 3, 3)
+    with pytest.raises(ValueError, match="negative"):
+        DraftTree([1, -1], device="cpu")
+    with pytest.raises(ValueError, match="exclude"):
+        DraftTree([2], [-1, 0], full=True, device="cpu")
+    with pytest.raises(ValueError, match="made without parents"):
+        t.set_parents([-1] * 5)
+    for parents in ([-1], [-1, 1], [0, 0], [-2, 0], [-1, 0, 1]):
+        with pytest.raises(ValueError, match="before its child"):
+            DraftTree([2], parents, device="cpu")
+    with pytest.raises(ValueError, match="before its child"):
+        DraftTree([1, 2], [-1, -1, 1], device="cpu")  # indices count within the request
+    with pytest.raises(RuntimeError, match="CUDA"):
+        DraftTree([2], [-1, 0], device="cpu")
+    see = np.zeros((40, 40), bool)
+    see[3, [0, 31, 32, 39]] = True
+    m = DraftTree([1, 40], visible=[np.ones((1, 1), bool), see], device="cpu").masks
+    assert m.shape == (41, 2) and m[0].tolist() == [1, 0] and m[1].tolist() == [0, 0]
+    assert m[4].tolist() == [1 - 2**31, 1 | 1 << 7]
+    for bad in ([see], [np.ones((1, 1), bool), see[:3]], [np.ones((1, 1), np.int8), see]):
+        with pytest.raises(ValueError, match="visible"):
+            DraftTree([1, 40], visible=bad, device="cpu")
+
+
+def _args(pool=None, n=3, hq=4, dtype=torch.bfloat16):
+    pool = _pool() if pool is None else pool
+    rand = lambda h: torch.zeros(n, h, pool.head_dim, dtype=dtype)  # noqa: E731
+    return rand(hq), PagedBatch(pool, [torch.arange(4, 8)]), DraftTree([n], device="cpu"), 0, rand(pool.heads), rand(pool.heads)
+
+
+def test_tree_attention_refuses_before_any_launch():
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        tree_attention(*_args())
+    with pytest.raises(ValueError, match="multiple of the pool's 2"):
+        tree_attention(*_args(hq=3))
+    q, cache, tree, layer, kn, vn = _args()
+    with pytest.raises(ValueError, match="layer 1 outside"):
+        tree_attention(q, cache, tree, 1, kn, vn)
+    with pytest.raises(ValueError, match="bf16 or fp16"):
+        tree_attention(*_args(_pool(dtype=torch.float32)))
+    with pytest.raises(ValueError, match="bf16 or fp16 heads"):
+        tree_attention(*_args(_pool(d=32)))
+
+
+def test_weights_refuse_before_any_launch():
+    q, cache, tree, layer, kn, _ = _args()
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        attention_weights(q, torch.zeros(4, 3), cache, tree, layer, kn)
+    with pytest.raises(ValueError, match="layer"):
+        attention_weights(q, torch.zeros(4, 3), cache, tree, -1, kn)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        heaviest(torch.zeros(2, 9), 4)
+
+
+def test_retain_and_free():
+    pool = _pool()
+    keep = torch.zeros(1, 2, 4, dtype=torch.int32)
+    src, dst = torch.arange(4, 12), torch.arange(16, 20)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        pool.retain(src, keep, dst)
+    for bad in (keep.long(), keep[:, :1], keep[..., :3]):
+        with pytest.raises(ValueError, match="keep must be"):
+            pool.retain(src, bad, dst)
+    with pytest.raises(ValueError, match="16 bytes"):
+        _pool(d=4).retain(src, keep, dst)
+    slots = pool.alloc(6)
+    free = pool.usage()["free"]
+    pool.free(slots)
+    assert pool.usage()["free"] == free + 8
+    with pytest.raises(_lib.QEError, match="already free"):
+        pool.free(slots)
+
+
+def _batch(**over):
+    base = dict(starts=16, lengths=16, tables=16, masks=None, batch=1, table_width=2, page_size=4, mask_words=0, mode=0,
+                total=3, max_nodes=3, max_length=8, sum_length=8)
+    base.update(over)
+    return _lib.DraftBatch(**base)
+
+
+def _attend(batch=None, hq=4, hkv=2, d=64, dtype=1, rows=32, qt=512, scale=0.1, work=None, size=0, kd=16, q=16):
+    _lib.call("qe_tree_attention", batch or _batch(), q, qt, 128, hq, hkv, d, dtype, 16, 16, rows, kd, kd, 256, 128, scale,
+              16, 512, 128, None, work, size, None, None)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(hq=3), "multiple of heads_kv"), (dict(d=96), "head_dim"), (dict(dtype=0), "dtype"), (dict(rows=30), "pool_rows"),
+    (dict(qt=24), "16 bytes"), (dict(qt=64), "row of head_dim"), (dict(scale=0.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(q=24), "16-byte"), (dict(kd=8), "16-byte"), (dict(q=None), "null"),
+    (dict(batch=_batch(batch=-1)), "negative"), (dict(batch=_batch(mode=3)), "mode"),
+    (dict(batch=_batch(mode=1)), "masks"), (dict(batch=_batch(mode=1, masks=16, mask_words=1, max_nodes=33, total=33)), "masks"),
+    (dict(batch=_batch(page_size=0)), "page_size"), (dict(batch=_batch(tables=None)), "null tables"),
+    (dict(batch=_batch(starts=None)), "null starts"), (dict(batch=_batch(total=2**30)), "2\\^31"),
+    (dict(batch=_batch(max_length=1 << 20, sum_length=1 << 20, table_width=1 << 18)), "workspace")])
+def test_c_tree_attention_rejects(kw, match):
+    with pytest.raises(ValueError, match=match):
+        _attend(**kw)
+
+
+def test_c_entry_points_reject_and_accept_nothing():
+    size = ctypes.c_int64(-1)
+    _lib.call("qe_tree_attention_workspace", _batch(max_length=1 << 20, sum_length=1 << 20), 4, 2, 64, ctypes.byref(size))
+    assert size.value > 0 and size.value % 8 == 0
+    with pytest.raises(ValueError):
+        _lib.call("qe_tree_attention_workspace", _batch(), 4, 3, 64, ctypes.byref(size))
+    for empty in (_batch(batch=0), _batch(total=0), _batch(max_nodes=0)):
+        _attend(empty)
+    with pytest.raises(ValueError, match="mask_words"):
+        _lib.call("qe_tree_masks", 16, 16, 1, 40, 40, 1, 16, None, None)
+    with pytest.raises(ValueError, match="width"):
+        _lib.call("qe_attention_weights", _batch(), 16, 512, 128, 4, 2, 64, 1, 16, 32, 16, 256, 128, 16, 3, 0.1, 0, 16, 20,
+                  10, 10, None, None)
+    with pytest.raises(ValueError, match="null weights"):
+        _lib.call("qe_attention_weights", _batch(), 16, 512, 128, 4, 2, 64, 1, 16, 32, 16, 256, 128, 16, 3, 0.1, 0, None, 22,
+                  11, 11, None, None)
+    for args in ((4, 3, 2), (4, -1, 2)):
+        with pytest.raises(ValueError):
+            _lib.call("qe_heaviest", 16, 1, 1, 1, 0, 0, 0, 9, None, *args, 16, None, None)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        _lib.call("qe_retain", _lib.planes(16, 0, 0, 2), 8, 1, 1, 24, 16, 4, 16, 2, 16, None, None)
+    with pytest.raises(ValueError, match=r"\[layers, 2\]"):
+        _lib.call("qe_retain", _lib.planes(16, 0, 0, 1), 8, 1, 1, 32, 16, 4, 16, 2, 16, None, None)
