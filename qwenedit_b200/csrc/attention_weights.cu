@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "qe_decode.cuh"
 #include "qe_tcgen05.cuh"
@@ -193,7 +194,8 @@ struct WSmem {
   static constexpr int node = lse + kTcStages * kTile * 4;
   static constexpr int plain = node + kTcStages * kTile * 4;  // int [stage][4]: every lse of the warp's rows finite
   static constexpr int part = plain + kTcStages * 16;         // float [256]: this CTA's sums
-  static constexpr int bars = part + 256 * 4;
+  static constexpr int rows = part + 256 * 4;                 // int [256]: the keys' pool rows
+  static constexpr int bars = rows + 256 * 4;
   static constexpr int slot = bars + wBars * 8;
   static constexpr int abort = slot + 4;
   // slack to align the base; never so few that two CTAs, each with all of the tensor memory, would share an SM
@@ -289,16 +291,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_weights_tc_kernel(con
     const int c = int(threadIdx.x) & (kChunks - 1), r0 = (int(threadIdx.x) - 256) / kChunks;
     const uint32_t chunk = uint32_t(c >> 3) * S::half;  // its 64-dim half
     auto place = [&](int r) { return chunk + uint32_t(r) * 128u + uint32_t(((c & 7) ^ (r & 7)) << 4); };
+    // the pool rows of the 256 keys, two lookups a thread, then every thread copies its rows' chunk
+    int *key_row = reinterpret_cast<int *>(smem + S::rows);
     for (int t = 0; t < mine; ++t) {
-      const int tile = t0 + t;
+      const int tile = t0 + t, r = int(threadIdx.x) - 256;
       const bool draft = tile >= cached_tiles;
-      const int k0 = (draft ? tile - cached_tiles : tile) * kTile, there = (draft ? drafted : rq.len) - k0;
+      const int k = (draft ? tile - cached_tiles : tile) * kTile + r;
+      key_row[t * kTile + r] = k >= (draft ? drafted : rq.len) ? -1 : draft ? rq.lo + k : pool_row(p.batch, b, k);
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    for (int t = 0; t < mine; ++t) {
+      const bool draft = t0 + t >= cached_tiles;
       const char *src = draft ? p.k_draft + int64_t(kvh) * p.draft_head : p.k_pool + int64_t(kvh) * (D * 2);
+      const int64_t stride = draft ? p.draft_token : p.pool_row;
+#pragma unroll 4
       for (int r = r0; r < kTile; r += kRowsPass) {
-        int row = -1;
-        if (r < there) row = draft ? rq.lo + k0 + r : pool_row(p.batch, b, k0 + r);
-        cp_async16(base + S::k + t * S::tile + place(r),
-                   row < 0 ? src : src + int64_t(row) * (draft ? p.draft_token : p.pool_row) + c * 16, row < 0 ? 0 : 16);
+        const int row = key_row[t * kTile + r];
+        cp_async16(base + S::k + t * S::tile + place(r), row < 0 ? src : src + int64_t(row) * stride + c * 16,
+                   row < 0 ? 0 : 16);
       }
     }
     cp_async_commit();
@@ -396,58 +406,94 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_weights_tc_kernel(con
     // The total of up to 10^5 weights is kept with its rounding error (Fast2Sum after each tile): plain fp32 sums of
     // this length lose two digits.
     float total = 0.0f, lost = 0.0f;
-    for (int i = 0; i < n_q; ++i) {
+    // The first columns of a tile are loaded under the last exponentials of the tile before.
+    uint32_t v[2][32];
+    auto enter = [&](int i) {  // query tile i's S and lse are there: load its first 32 columns
+      bool ok = mbar_wait(bar(wSFull + t * 2 + (i & 1)), (i >> 1) & 1, abort, p.batch.err);
+      ok = ok && mbar_wait(bar(wQFull + i % kTcStages), (i / kTcStages) & 1, abort, p.batch.err);  // the copy warps' lse
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        tc_fence_after();
+        tmem_ld32_async(lanes + uint32_t((i & 1) * kTile), v[0]);
+      }
+      return ok;
+    };
+    bool ok = n_q == 0 || enter(0);
+    for (int i = 0; i < n_q && ok; ++i) {
       const int s = i % kTcStages, buf = i & 1;
-      bool ok = mbar_wait(bar(wSFull + t * 2 + buf), (i >> 1) & 1, abort, p.batch.err);
-      ok = ok && mbar_wait(bar(wQFull + s), (i / kTcStages) & 1, abort, p.batch.err);  // its lse, written by the copy warps
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
       const float *nl = reinterpret_cast<const float *>(smem + S::lse) + s * kTile;
       const int *node = reinterpret_cast<const int *>(smem + S::node) + s * kTile;
       const int4 all = *reinterpret_cast<const int4 *>(smem + S::plain + s * 16);
-      bool plain = all.x & all.y & all.z & all.w;
-      if (draft && p.batch.mode == 0) plain = plain && (qa + i) * kTile / p.group >= j_warp + 31;
-      if (draft && p.batch.mode == 1) plain = false;
+      // Which of the tile's columns this thread's key counts: all (plain), those whose node is at least `from` (a
+      // chain's drafted key: its own node and the later ones; else any row that counts), or by the bit masks.
+      bool plain = all.x & all.y & all.z & all.w, skip = false;
+      const bool masked = draft && p.batch.mode == 1;
+      int from = 0;
+      if (draft && p.batch.mode == 0) {
+        from = j;
+        plain = plain && (qa + i) * kTile / p.group >= j_warp + 31;
+        skip = ((qa + i) * kTile + kTile - 1) / p.group < j_warp;
+      }
+      plain = plain && !masked;
       const uint32_t col = lanes + uint32_t(buf * kTile);
       f32x2 sum[4] = {pk2(0.0f, 0.0f), pk2(0.0f, 0.0f), pk2(0.0f, 0.0f), pk2(0.0f, 0.0f)};
-      uint32_t v[2][32];
-      tmem_ld32_async(col, v[0]);
-      tmem_ld_wait(v[0]);
+      auto leave = [&]() {  // S is read: its buffer goes back to the products, and the next tile's load starts
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(wSEmpty + t * 2 + buf));
+        if (i + 1 < n_q) ok = enter(i + 1);
+      };
+      auto add_up = [&](auto kind) {  // 0: plain, 1: by node, 2: by mask (a loop of its own each: the plain one is hot)
+        constexpr int kKind = decltype(kind)::value;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (c + 1 < 4) tmem_ld32_async(col + 32 * (c + 1), v[(c + 1) & 1]);
-        const uint32_t(&x)[32] = v[c & 1];
-        if (plain) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float2 l = *reinterpret_cast<const float2 *>(nl + 32 * c + 2 * e);
-            const float2 y = up2(fma2(pk2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale2, pk2(l.x, l.y)));
-            sum[e & 3] = add2(sum[e & 3], pk2(ex2(y.x), ex2(y.y)));
+        for (int c = 0; c < 4; ++c) {
+          tmem_ld_wait(v[c & 1]);
+          if (c + 1 < 4) {
+            tmem_ld32_async(col + 32 * (c + 1), v[(c + 1) & 1]);
+          } else {
+            leave();
           }
-        } else {
+          const uint32_t(&x)[32] = v[c & 1];
+          uint32_t word = 0;  // of column 32 c + lane
+          if (kKind == 2) {
+            const int at = node[32 * c + lane];
+            if (at >= 0 && j_warp / 32 < p.batch.mask_words)
+              word = uint32_t(__ldg(p.batch.masks + int64_t(rq.lo + at) * p.batch.mask_words + j_warp / 32));
+          }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int at = node[32 * c + e];
-            bool seen = at >= 0;
-            if (draft && p.batch.mode == 0) seen = seen && j <= at;
-            if (draft && p.batch.mode == 1) {
-              uint32_t w = 0;
-              if (at >= 0 && j_warp / 32 < p.batch.mask_words)
-                w = uint32_t(__ldg(p.batch.masks + int64_t(rq.lo + at) * p.batch.mask_words + j_warp / 32));
-              seen = (w >> lane) & 1u;
+          for (int e = 0; e < 32; e += 4) {
+            const float4 l = *reinterpret_cast<const float4 *>(nl + 32 * c + e);
+            const float2 a = up2(fma2(pk2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), scale2, pk2(l.x, l.y)));
+            const float2 z = up2(fma2(pk2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), scale2, pk2(l.z, l.w)));
+            float y[4] = {ex2(a.x), ex2(a.y), ex2(z.x), ex2(z.y)};
+            if (kKind == 1) {
+              const int4 at = *reinterpret_cast<const int4 *>(node + 32 * c + e);
+              y[0] = at.x >= from ? y[0] : 0.0f;
+              y[1] = at.y >= from ? y[1] : 0.0f;
+              y[2] = at.z >= from ? y[2] : 0.0f;
+              y[3] = at.w >= from ? y[3] : 0.0f;
             }
-            const float y = ex2(fmaf(__uint_as_float(x[e]), p.scale_log2, nl[32 * c + e]));
-            sum[e & 3] = add2(sum[e & 3], pk2(seen ? y : 0.0f, 0.0f));
+            if (kKind == 2) {
+#pragma unroll
+              for (int u = 0; u < 4; ++u) y[u] = (__shfl_sync(0xffffffffu, word, e + u) >> lane) & 1u ? y[u] : 0.0f;
+            }
+            sum[(e / 4) & 1] = add2(sum[(e / 4) & 1], pk2(y[0], y[1]));
+            sum[2 + ((e / 4) & 1)] = add2(sum[2 + ((e / 4) & 1)], pk2(y[2], y[3]));
           }
         }
-        if (c + 1 < 4) tmem_ld_wait(v[(c + 1) & 1]);
+      };
+      if (plain)
+        add_up(std::integral_constant<int, 0>{});
+      else if (masked)
+        add_up(std::integral_constant<int, 2>{});
+      else if (!skip)
+        add_up(std::integral_constant<int, 1>{});
+      else {
+        tmem_ld_wait(v[0]);
+        leave();
       }
-      tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(bar(wSEmpty + t * 2 + buf));
-        mbar_arrive(bar(wQEmpty + s));
-      }
+      if (lane == 0) mbar_arrive(bar(wQEmpty + s));  // the tile's lse and nodes are read
       const float2 a = up2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
       const float add = a.x + a.y, before = total;
       total = before + add;
