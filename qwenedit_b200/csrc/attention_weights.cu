@@ -163,39 +163,42 @@ __global__ void __launch_bounds__(kWarps * 32) attention_weights_kernel(const We
   }
 }
 
-// ---- many rows: S^T = K Q^T on the fifth-generation tensor cores ------------------------------------------------
+// ---- many rows: S = Q K^T on the fifth-generation tensor cores ----------------------------------------------------
 //
-// A CTA holds two tiles of 128 keys and streams tiles of 128 query rows past them: S^T has a key per tensor-memory
-// lane, so a thread adds up its own key's weights over the columns and nothing crosses lanes. Two S buffers per key
-// tile let the products of the next query tile run under the exponentials of this one.
-//   warps 0-3, 4-7   key tile 0, key tile 1: a thread per key, exponentials and sums
-//   warps 8-11       copies: K once, then a four-stage ring of query tiles and their lse (cp.async through the block
-//                    table and the (node, head) rows, which no tensor map describes for every group size)
-//   warp 12          tcgen05.mma (one thread) and the tensor memory's 512 columns: S of (tile, buffer) pairs
+// A CTA keeps 128 keys in shared memory and streams tiles of 128 query rows past them; S has a query row per
+// tensor-memory lane and a key per column. A thread's row has its lse in a register, and a thread adds up 32 keys'
+// weights over all the rows that pass its lane: 32 sums in registers, brought together over the lanes once, at the
+// end. (With the keys in the lanes every weight needs its column's lse from shared memory, which feeds the products
+// too: 16,384 queries over 32,768 keys took 3.87-4.08 ms in three forms of that, 3.59 ms in this one.) The bound is
+// the exponential unit, 16 a clock and SM: 1,024 clocks a tile, of about 1,290 used; 2^x on the FMA pipe for a quarter
+// of the weights (degree 5) took 3.82 ms, for three quarters 5.13.
+//   warps 0-15   K at the start (cp.async through the block table); then lanes 32 (w % 4) .. + 31, keys 32 (w / 4) ..
+//                + 31: exponentials and sums
+//   warp 16      tcgen05.mma (one thread) and the tensor memory's 512 columns: four S buffers
+//   warp 17      query tiles into a five-stage ring by TMA: the G heads of as many whole nodes as fit 128 rows (box
+//                [64 dims, G, 128 / G]), so that a tile's rows are (node, head) in order for every G
 // The query tiles are split over the CTAs of a cluster where the key tiles alone would leave SMs idle; the cluster's
 // first CTA adds the others' sums in rank order.
 
-constexpr int kTile = 128;      // keys per tile and query rows per tile
-constexpr int kTcStages = 4;    // query tiles in the ring
-constexpr int kTcThreads = 13 * 32;
-constexpr int kCopyThreads = 128;
+constexpr int kTile = 128;      // keys per CTA and query rows per tile
+constexpr int kTcStages = 5;    // query tiles in the ring
+constexpr int kBuffers = 4;     // S buffers
+constexpr int kSumWarps = 16;
+constexpr int kTcThreads = (kSumWarps + 2) * 32;
 constexpr int kMaxCluster = 8;
 
-enum WBar { wKFull = 0, wQFull = 1, wQEmpty = wQFull + kTcStages, wSFull = wQEmpty + kTcStages, wSEmpty = wSFull + 4,
-            wDrain = wSEmpty + 4, wBars = wDrain + 1 };
+enum WBar { wKFull = 0, wQFull = 1, wQEmpty = wQFull + kTcStages, wSFull = wQEmpty + kTcStages,
+            wSEmpty = wSFull + kBuffers, wDrain = wSEmpty + kBuffers, wBars = wDrain + 1 };
 
 template <int D>
 struct WSmem {
   static constexpr int half = kTile * 128;            // 128 rows of 64 dims: one 128-byte swizzle span each
   static constexpr int tile = half * (D / 64);
   static constexpr int k = 0;
-  static constexpr int q = 2 * tile;
-  static constexpr int lse = q + kTcStages * tile;    // float [stage][128]: -lse in log2 units
-  static constexpr int node = lse + kTcStages * kTile * 4;
-  static constexpr int plain = node + kTcStages * kTile * 4;  // int [stage][4]: every lse of the warp's rows finite
-  static constexpr int part = plain + kTcStages * 16;         // float [256]: this CTA's sums
-  static constexpr int rows = part + 256 * 4;                 // int [256]: the keys' pool rows
-  static constexpr int bars = rows + 256 * 4;
+  static constexpr int q = tile;
+  static constexpr int part = q + kTcStages * tile;   // float [4][128]: the sums, a quarter of the lanes each
+  static constexpr int rows = part + 512 * 4;         // int [128]: the keys' pool rows
+  static constexpr int bars = rows + 128 * 4;
   static constexpr int slot = bars + wBars * 8;
   static constexpr int abort = slot + 4;
   // slack to align the base; never so few that two CTAs, each with all of the tensor memory, would share an SM
@@ -227,10 +230,11 @@ __device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kTcThreads, 1) attention_weights_tc_kernel(const WeightParams p) {
+__global__ void __launch_bounds__(kTcThreads, 1)
+    attention_weights_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const WeightParams p) {
   using S = WSmem<D>;
-  constexpr int kChunks = D / 8;                       // 16-byte chunks of a row
-  constexpr int kRowsPass = kCopyThreads / kChunks;    // rows the copy warps cover at once
+  constexpr int kChunks = D / 8;                            // 16-byte chunks of a row
+  constexpr int kRowsPass = kSumWarps * 32 / kChunks;       // K rows copied at once
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t base = smem_addr(smem);
@@ -242,43 +246,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_weights_tc_kernel(con
   const int kvh = int(blockIdx.y) % p.heads_kv, b = int(blockIdx.y) / p.heads_kv;
   const Request rq = request_of(p.batch, b);
   const int drafted = p.k_draft ? rq.n : 0;
-  const int rows = rq.n * p.group;
+  const int nodes = kTile / p.group, filled = nodes * p.group;  // nodes of a query tile, rows of it that hold one
   const int cached_tiles = (rq.len + kTile - 1) / kTile;
   const int tiles = cached_tiles + (drafted + kTile - 1) / kTile;
-  const int t0 = int(blockIdx.z) * 2;
+  const int tile = int(blockIdx.z);
   float *out = p.weights + int64_t(b) * p.weights_batch + int64_t(kvh) * p.weights_head;
   if (!p.accumulate)  // positions past the request's keys
     for (int64_t j = int64_t(rq.len) + drafted + (int64_t(blockIdx.z) * splits + split) * kTcThreads + threadIdx.x;
          j < p.width; j += int64_t(gridDim.z) * splits * kTcThreads)
       out[j] = 0.0f;
-  if (t0 >= tiles) return;  // the whole cluster
-  const int mine = min(2, tiles - t0);
-  // query tiles: a chain's drafted keys are seen by later nodes only
-  int first_row = 0;
-  if (p.batch.mode == 0 && t0 >= cached_tiles) first_row = (t0 - cached_tiles) * kTile * p.group;
-  const int q_first = first_row / kTile, q_tiles = (rows + kTile - 1) / kTile - q_first;
+  if (tile >= tiles) return;  // the whole cluster
+  const bool draft = tile >= cached_tiles;
+  const int k0 = (draft ? tile - cached_tiles : tile) * kTile;
+  // query tiles: a chain's drafted keys are seen by their own and later nodes only
+  const int q_first = draft && p.batch.mode == 0 ? k0 / nodes : 0;
+  const int q_tiles = (rq.n + nodes - 1) / nodes - q_first;
   const int qa = q_first + int(int64_t(q_tiles) * split / splits);
   const int n_q = q_first + int(int64_t(q_tiles) * (split + 1) / splits) - qa;
 
   if (threadIdx.x == 0) {
-    mbar_init(bar(wKFull), kCopyThreads);
+    mbar_init(bar(wKFull), kSumWarps);
     for (int s = 0; s < kTcStages; ++s) {
-      mbar_init(bar(wQFull + s), kCopyThreads);
-      mbar_init(bar(wQEmpty + s), 1 + 4 * mine);
+      mbar_init(bar(wQFull + s), 1);
+      mbar_init(bar(wQEmpty + s), 1);
     }
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < kBuffers; ++s) {
       mbar_init(bar(wSFull + s), 1);
-      mbar_init(bar(wSEmpty + s), 4);
+      mbar_init(bar(wSEmpty + s), kSumWarps);
     }
     mbar_init(bar(wDrain), 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == kSumWarps) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                  "r"(512u)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  int *key_row = reinterpret_cast<int *>(smem + S::rows);
+  if (threadIdx.x < kTile) {
+    const int k = k0 + int(threadIdx.x);
+    key_row[threadIdx.x] = k >= (draft ? drafted : rq.len) ? -1 : draft ? rq.lo + k : pool_row(p.batch, b, k);
   }
   tc_fence_before();
   __syncthreads();
@@ -286,108 +295,44 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_weights_tc_kernel(con
   const uint32_t tmem = *tmem_slot;
   float *part = reinterpret_cast<float *>(smem + S::part);
 
-  if (warp >= 8 && warp < 12) {
-    // ---- copies ----
-    const int c = int(threadIdx.x) & (kChunks - 1), r0 = (int(threadIdx.x) - 256) / kChunks;
-    const uint32_t chunk = uint32_t(c >> 3) * S::half;  // its 64-dim half
-    auto place = [&](int r) { return chunk + uint32_t(r) * 128u + uint32_t(((c & 7) ^ (r & 7)) << 4); };
-    // the pool rows of the 256 keys, two lookups a thread, then every thread copies its rows' chunk
-    int *key_row = reinterpret_cast<int *>(smem + S::rows);
-    for (int t = 0; t < mine; ++t) {
-      const int tile = t0 + t, r = int(threadIdx.x) - 256;
-      const bool draft = tile >= cached_tiles;
-      const int k = (draft ? tile - cached_tiles : tile) * kTile + r;
-      key_row[t * kTile + r] = k >= (draft ? drafted : rq.len) ? -1 : draft ? rq.lo + k : pool_row(p.batch, b, k);
-    }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    for (int t = 0; t < mine; ++t) {
-      const bool draft = t0 + t >= cached_tiles;
-      const char *src = draft ? p.k_draft + int64_t(kvh) * p.draft_head : p.k_pool + int64_t(kvh) * (D * 2);
-      const int64_t stride = draft ? p.draft_token : p.pool_row;
-#pragma unroll 4
-      for (int r = r0; r < kTile; r += kRowsPass) {
-        const int row = key_row[t * kTile + r];
-        cp_async16(base + S::k + t * S::tile + place(r), row < 0 ? src : src + int64_t(row) * stride + c * 16,
-                   row < 0 ? 0 : 16);
+  if (warp == kSumWarps + 1) {
+    if (lane == 0) {
+      // ---- query tiles ----
+      int asked = 0;
+      for (; asked < n_q; ++asked) {
+        const int s = asked % kTcStages;
+        if (!mbar_wait(bar(wQEmpty + s), ((asked / kTcStages) & 1) ^ 1, abort, p.batch.err)) break;
+        mbar_expect_tx(bar(wQFull + s), uint32_t(filled) * (D * 2));
+        for (int h = 0; h < D / 64; ++h)
+          tma_load_3d(base + S::q + s * S::tile + h * S::half, &tm_q, h * 64, kvh * p.group, rq.lo + (qa + asked) * nodes,
+                      bar(wQFull + s));
       }
-    }
-    cp_async_commit();
-    // This thread's query rows are r0, r0 + kRowsPass, ... of the first tile, then of the next: (node, head) and the
-    // address step along without divisions. Likewise the row whose lse it fetches, one tile ahead.
-    const int first = qa * kTile;
-    int row = first + r0, g = row % p.group;
-    const char *src = p.q + int64_t(rq.lo + row / p.group) * p.q_token + int64_t(kvh * p.group + g) * p.q_head + c * 16;
-    const int step_g = kRowsPass % p.group;
-    const int64_t step = int64_t(kRowsPass / p.group) * p.q_token + int64_t(step_g) * p.q_head;
-    const int64_t wrap = p.q_token - int64_t(p.group) * p.q_head;
-    const int lse_r = int(threadIdx.x) - 256;
-    int l_row = first + lse_r, l_node = l_row / p.group, l_g = l_row - l_node * p.group;
-    auto fetch_lse = [&]() {
-      return l_row < rows ? __ldg(p.lse + int64_t(kvh * p.group + l_g) * p.lse_head + rq.lo + l_node) : INFINITY;
-    };
-    float l_next = fetch_lse();
-    auto load_q = [&](int i) {  // query tile qa + i into its stage
-      const int s = i % kTcStages;
-#pragma unroll
-      for (int r = 0; r < kTile; r += kRowsPass) {
-        cp_async16(base + S::q + s * S::tile + place(r0 + r), row < rows ? src : p.q, row < rows ? 16 : 0);
-        row += kRowsPass;
-        src += step;
-        g += step_g;
-        if (g >= p.group) {
-          g -= p.group;
-          src += wrap;
+      if (asked < n_q) {  // a wait gave up: time for the copies in flight before the shared memory is given back
+        const uint64_t since = globaltimer();
+        while (globaltimer() - since < 200000ull) {
         }
       }
-      const bool counts = !(fabsf(l_next) == INFINITY);
-      reinterpret_cast<float *>(smem + S::lse)[s * kTile + lse_r] = counts ? -l_next * kLog2e : -INFINITY;
-      reinterpret_cast<int *>(smem + S::node)[s * kTile + lse_r] = counts ? l_node : -1;
-      const bool all = __all_sync(0xffffffffu, counts);
-      if (lane == 0) reinterpret_cast<int *>(smem + S::plain)[s * 4 + warp - 8] = all;
-      l_row += kTile;
-      l_node += kTile / p.group;
-      l_g += kTile % p.group;
-      if (l_g >= p.group) {
-        l_g -= p.group;
-        ++l_node;
-      }
-      l_next = fetch_lse();
-    };
-    // A tile is handed over after the next one's copies are issued; the ring holds four, so that waiting for a free
-    // stage never keeps back a tile that the products could start on.
-    for (int i = 0; i <= n_q; ++i) {
-      if (i < n_q) {
-        const bool ok = mbar_wait(bar(wQEmpty + i % kTcStages), ((i / kTcStages) & 1) ^ 1, abort, p.batch.err);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        load_q(i);
-      }
-      cp_async_commit();
-      cp_async_wait<1>();  // the tile before (at first: K)
-      fence_async_smem();
-      mbar_arrive(bar(i == 0 ? wKFull : wQFull + (i - 1) % kTcStages));
     }
-    cp_async_wait<0>();
-  } else if (warp == 12) {
+  } else if (warp == kSumWarps) {
     if (lane == 0) {
       // ---- products ----
       constexpr uint32_t idesc = idesc_128<T>();
+      const uint64_t k_desc = sw128_desc(base + S::k, 16, 1024);
       bool ok = mbar_wait(bar(wKFull), 0, abort, p.batch.err);
       for (int i = 0; i < n_q && ok; ++i) {
-        const int s = i % kTcStages, buf = i & 1;
-        ok = mbar_wait(bar(wQFull + s), (i / kTcStages) & 1, abort, p.batch.err);
-        for (int t = 0; t < mine && ok; ++t) {
-          ok = mbar_wait(bar(wSEmpty + t * 2 + buf), ((i >> 1) & 1) ^ 1, abort, p.batch.err);
-          if (!ok) break;
-          tc_fence_after();
+        const int s = i % kTcStages, buf = i % kBuffers;
+        ok = mbar_wait(bar(wQFull + s), (i / kTcStages) & 1, abort, p.batch.err) &&
+             mbar_wait(bar(wSEmpty + buf), ((i / kBuffers) & 1) ^ 1, abort, p.batch.err);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t q_desc = sw128_desc(base + S::q + s * S::tile, 16, 1024);
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = uint32_t((k >> 2) * S::half + (k & 3) * 32);
-            mma_ss(tmem + (t * 2 + buf) * kTile, sw128_desc(base + S::k + t * S::tile + off, 16, 1024),
-                   sw128_desc(base + S::q + s * S::tile + off, 16, 1024), idesc, k > 0);
-          }
-          mma_commit(bar(wSFull + t * 2 + buf));
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t off = uint64_t((k >> 2) * S::half + (k & 3) * 32) >> 4;
+          mma_ss(tmem + buf * kTile, q_desc + off, k_desc + off, idesc, k > 0);
         }
-        if (ok) mma_commit(bar(wQEmpty + s));
+        mma_commit(bar(wSFull + buf));
+        mma_commit(bar(wQEmpty + s));
       }
       // the tensor memory is released once every product issued has landed
       mma_commit(bar(wDrain));
@@ -395,125 +340,140 @@ __global__ void __launch_bounds__(kTcThreads, 1) attention_weights_tc_kernel(con
       while (!mbar_try(bar(wDrain), 0) && globaltimer() - since < kWaitNs) {
       }
     }
-  } else if ((warp >> 2) < mine) {
-    // ---- exponentials and sums: this thread's key ----
-    const int t = warp >> 2, tile = t0 + t;
-    const bool draft = tile >= cached_tiles;
-    const int j_warp = (draft ? tile - cached_tiles : 0) * kTile + (warp & 3) * 32;  // drafted key of lane 0
-    const int j = j_warp + lane;
-    const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(t * 2 * kTile);
-    const f32x2 scale2 = pk2(p.scale_log2, p.scale_log2);
-    // The total of up to 10^5 weights is kept with its rounding error (Fast2Sum after each tile): plain fp32 sums of
-    // this length lose two digits.
-    float total = 0.0f, lost = 0.0f;
-    // The first columns of a tile are loaded under the last exponentials of the tile before.
-    uint32_t v[2][32];
-    auto enter = [&](int i) {  // query tile i's S and lse are there: load its first 32 columns
-      bool ok = mbar_wait(bar(wSFull + t * 2 + (i & 1)), (i >> 1) & 1, abort, p.batch.err);
-      ok = ok && mbar_wait(bar(wQFull + i % kTcStages), (i / kTcStages) & 1, abort, p.batch.err);  // the copy warps' lse
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        tc_fence_after();
-        tmem_ld32_async(lanes + uint32_t((i & 1) * kTile), v[0]);
+  } else {
+    // ---- K ----
+    {
+      const int c = int(threadIdx.x) & (kChunks - 1);
+      const char *src = (draft ? p.k_draft + int64_t(kvh) * p.draft_head : p.k_pool + int64_t(kvh) * (D * 2)) + c * 16;
+      const int64_t stride = draft ? p.draft_token : p.pool_row;
+#pragma unroll
+      for (int r = int(threadIdx.x) / kChunks; r < kTile; r += kRowsPass) {
+        const int row = key_row[r];
+        cp_async16(base + S::k + uint32_t(c >> 3) * S::half + uint32_t(r) * 128u + uint32_t(((c & 7) ^ (r & 7)) << 4),
+                   row < 0 ? src : src + int64_t(row) * stride, row < 0 ? 0 : 16);
       }
-      return ok;
+      cp_async_commit();
+      cp_async_wait<0>();
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(wKFull));
+    }
+    // ---- exponentials and sums ----
+    const int row = (warp & 3) * 32 + lane, quarter = warp >> 2;
+    const int dn = row / p.group;                 // this row's node within a tile
+    const bool used = row < filled;
+    const int key0 = k0 + quarter * 32;           // first of this thread's keys
+    const float *lse = p.lse + int64_t(kvh * p.group + row - dn * p.group) * p.lse_head + rq.lo;
+    int node = qa * nodes + dn;
+    auto fetch_lse = [&]() { return used && node < rq.n ? __ldg(lse + node) : INFINITY; };
+    // the keys of the 32 that the row counts, a bit each
+    auto fetch_bits = [&](float l) -> uint32_t {
+      if (fabsf(l) == INFINITY) return 0u;
+      if (!draft || p.batch.mode == 2) return ~0u;
+      if (p.batch.mode == 1)
+        return key0 / 32 < p.batch.mask_words
+                   ? uint32_t(__ldg(p.batch.masks + int64_t(rq.lo + node) * p.batch.mask_words + key0 / 32))
+                   : 0u;
+      const int seen = node - key0 + 1;
+      return seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1u;
     };
+    const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16) + uint32_t(quarter * 32);
+    const f32x2 scale2 = pk2(p.scale_log2, p.scale_log2);
+    f32x2 acc[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = pk2(0.0f, 0.0f);
+    // 16 columns at a time; the next 16, of the next tile too, are loaded under the exponentials of these.
+    uint32_t v[2][16];
+    auto enter = [&](int i) {
+      const bool there = mbar_wait(bar(wSFull + i % kBuffers), (i / kBuffers) & 1, abort, p.batch.err);
+      const bool all = __all_sync(0xffffffffu, there);
+      if (all) {
+        tc_fence_after();
+        tmem_ld16_async(lanes + uint32_t(i % kBuffers * kTile), v[0]);
+      }
+      return all;
+    };
+    float l_next = fetch_lse();
+    uint32_t bits_next = fetch_bits(l_next);
     bool ok = n_q == 0 || enter(0);
     for (int i = 0; i < n_q && ok; ++i) {
-      const int s = i % kTcStages, buf = i & 1;
-      const float *nl = reinterpret_cast<const float *>(smem + S::lse) + s * kTile;
-      const int *node = reinterpret_cast<const int *>(smem + S::node) + s * kTile;
-      const int4 all = *reinterpret_cast<const int4 *>(smem + S::plain + s * 16);
-      // Which of the tile's columns this thread's key counts: all (plain), those whose node is at least `from` (a
-      // chain's drafted key: its own node and the later ones; else any row that counts), or by the bit masks.
-      bool plain = all.x & all.y & all.z & all.w, skip = false;
-      const bool masked = draft && p.batch.mode == 1;
-      int from = 0;
-      if (draft && p.batch.mode == 0) {
-        from = j;
-        plain = plain && (qa + i) * kTile / p.group >= j_warp + 31;
-        skip = ((qa + i) * kTile + kTile - 1) / p.group < j_warp;
-      }
-      plain = plain && !masked;
-      const uint32_t col = lanes + uint32_t(buf * kTile);
-      f32x2 sum[4] = {pk2(0.0f, 0.0f), pk2(0.0f, 0.0f), pk2(0.0f, 0.0f), pk2(0.0f, 0.0f)};
+      const uint32_t bits = bits_next;
+      const float nl = bits ? -l_next * kLog2e : 0.0f;
+      node += nodes;
+      l_next = fetch_lse();  // of the next tile
+      const f32x2 nl2 = pk2(nl, nl);
+      const uint32_t col = lanes + uint32_t(i % kBuffers * kTile);
+      const bool plain = __all_sync(0xffffffffu, bits == ~0u), none = __all_sync(0xffffffffu, bits == 0u);
       auto leave = [&]() {  // S is read: its buffer goes back to the products, and the next tile's load starts
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(wSEmpty + t * 2 + buf));
+        if (lane == 0) mbar_arrive(bar(wSEmpty + i % kBuffers));
         if (i + 1 < n_q) ok = enter(i + 1);
       };
-      auto add_up = [&](auto kind) {  // 0: plain, 1: by node, 2: by mask (a loop of its own each: the plain one is hot)
-        constexpr int kKind = decltype(kind)::value;
+      auto add_up = [&](auto kind) {
+        constexpr bool kPlain = decltype(kind)::value;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_ld_wait(v[c & 1]);
-          if (c + 1 < 4) {
-            tmem_ld32_async(col + 32 * (c + 1), v[(c + 1) & 1]);
-          } else {
+        for (int c = 0; c < 2; ++c) {
+          tmem_ld16_wait(v[c]);
+          if (c == 0)
+            tmem_ld16_async(col + 16, v[1]);
+          else
             leave();
-          }
-          const uint32_t(&x)[32] = v[c & 1];
-          uint32_t word = 0;  // of column 32 c + lane
-          if (kKind == 2) {
-            const int at = node[32 * c + lane];
-            if (at >= 0 && j_warp / 32 < p.batch.mask_words)
-              word = uint32_t(__ldg(p.batch.masks + int64_t(rq.lo + at) * p.batch.mask_words + j_warp / 32));
-          }
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 l = *reinterpret_cast<const float4 *>(nl + 32 * c + e);
-            const float2 a = up2(fma2(pk2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), scale2, pk2(l.x, l.y)));
-            const float2 z = up2(fma2(pk2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), scale2, pk2(l.z, l.w)));
-            float y[4] = {ex2(a.x), ex2(a.y), ex2(z.x), ex2(z.y)};
-            if (kKind == 1) {
-              const int4 at = *reinterpret_cast<const int4 *>(node + 32 * c + e);
-              y[0] = at.x >= from ? y[0] : 0.0f;
-              y[1] = at.y >= from ? y[1] : 0.0f;
-              y[2] = at.z >= from ? y[2] : 0.0f;
-              y[3] = at.w >= from ? y[3] : 0.0f;
+          for (int e = 0; e < 8; ++e) {
+            const float2 x = up2(fma2(pk2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), scale2, nl2));
+            if (kPlain) {
+              acc[c * 8 + e] = add2(acc[c * 8 + e], pk2(ex2(x.x), ex2(x.y)));
+            } else {
+              const float y0 = (bits >> (c * 16 + 2 * e)) & 1u ? ex2(x.x) : 0.0f;
+              const float y1 = (bits >> (c * 16 + 2 * e + 1)) & 1u ? ex2(x.y) : 0.0f;
+              acc[c * 8 + e] = add2(acc[c * 8 + e], pk2(y0, y1));
             }
-            if (kKind == 2) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u) y[u] = (__shfl_sync(0xffffffffu, word, e + u) >> lane) & 1u ? y[u] : 0.0f;
-            }
-            sum[(e / 4) & 1] = add2(sum[(e / 4) & 1], pk2(y[0], y[1]));
-            sum[2 + ((e / 4) & 1)] = add2(sum[2 + ((e / 4) & 1)], pk2(y[2], y[3]));
           }
         }
       };
-      if (plain)
-        add_up(std::integral_constant<int, 0>{});
-      else if (masked)
-        add_up(std::integral_constant<int, 2>{});
-      else if (!skip)
-        add_up(std::integral_constant<int, 1>{});
-      else {
-        tmem_ld_wait(v[0]);
+      if (plain) {
+        add_up(std::true_type{});
+      } else if (!none) {
+        add_up(std::false_type{});
+      } else {
+        tmem_ld16_wait(v[0]);
         leave();
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(wQEmpty + s));  // the tile's lse and nodes are read
-      const float2 a = up2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
-      const float add = a.x + a.y, before = total;
-      total = before + add;
-      lost += fmaxf(before, add) - total + fminf(before, add);
+      bits_next = fetch_bits(l_next);
     }
-    part[t * kTile + (warp & 3) * 32 + lane] = lost == lost ? total + lost : total;  // an infinite total stays one
+    // sums over the 32 lanes: halves of the columns go to halves of the lanes until a lane holds one column
+    float a[32];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float2 x = up2(acc[e]);
+      a[2 * e] = x.x;
+      a[2 * e + 1] = x.y;
+    }
+#pragma unroll
+    for (int h = 16; h; h >>= 1) {
+      const bool upper = lane & h;
+#pragma unroll
+      for (int e = 0; e < h; ++e) {
+        const float give = upper ? a[e] : a[e + h], keep = upper ? a[e + h] : a[e];
+        a[e] = keep + __shfl_xor_sync(0xffffffffu, give, h);
+      }
+    }
+    part[(warp & 3) * kTile + quarter * 32 + lane] = a[0];
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == kSumWarps) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
   if (splits > 1) cluster_sync();  // every CTA's sums are in its shared memory
-  if (split == 0 && int(threadIdx.x) < mine * kTile) {
-    const int tile = t0 + int(threadIdx.x) / kTile, r = int(threadIdx.x) % kTile;
-    const bool draft = tile >= cached_tiles;
-    const int key = (draft ? tile - cached_tiles : tile) * kTile + r;
-    float w = part[threadIdx.x];
-    for (int x = 1; x < splits; ++x) w += ld_cluster(base + S::part + 4 * threadIdx.x, uint32_t(x));
+  if (split == 0 && int(threadIdx.x) < kTile) {
+    const int key = k0 + int(threadIdx.x);
+    float w = 0.0f;
+    for (int x = 0; x < splits; ++x)
+      for (int u = 0; u < 4; ++u)
+        w += x == 0 ? part[u * kTile + threadIdx.x] : ld_cluster(base + S::part + 4 * (u * kTile + threadIdx.x), uint32_t(x));
     if (key < (draft ? drafted : rq.len)) {
       float *dst = out + (draft ? rq.len : 0) + key;
       *dst = p.accumulate ? *dst + w : w;
@@ -552,16 +512,33 @@ int run_weights_tc(const WeightParams &p, const qe_draft_batch &in, int nodes, c
     if (e != cudaSuccess) return cuda_status(e, "qe_attention_weights: smem attribute");
     raised[dev].store(true, std::memory_order_relaxed);
   }
-  const int64_t max_tiles = (in.max_length + kTile - 1) / kTile + (nodes + kTile - 1) / kTile;
-  const int64_t pairs = std::max<int64_t>(1, (max_tiles + 1) / 2);
-  const int64_t q_tiles = (int64_t(in.max_nodes) * p.group + kTile - 1) / kTile;
-  // key-tile pairs of the batch; split the query tiles until the CTAs fill the SMs
+  const int64_t max_tiles = std::max<int64_t>(1, (in.max_length + kTile - 1) / kTile + (nodes + kTile - 1) / kTile);
+  const int nodes_tile = kTile / p.group;
+  const int64_t q_tiles = (in.max_nodes + nodes_tile - 1) / nodes_tile;
+  CUtensorMap map;
+  const uint64_t dims[3] = {uint64_t(D), uint64_t(p.heads_q), uint64_t(in.total)};
+  const uint64_t strides[2] = {uint64_t(p.q_head), uint64_t(p.q_token)};
+  const uint32_t box[3] = {64, uint32_t(p.group), uint32_t(nodes_tile)};
+  const int e = tensor_map_16bit("qe_attention_weights", &map,
+                                 std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                 p.q, 3, dims, strides, box, "q");
+  if (e) return e;
+  // Key tiles of the batch over the SMs; a cluster splits the query tiles where that shortens the longest SM's work
+  // (in query tiles, a CTA's start and end counted as four).
   const int64_t all = std::max<int64_t>(
-      1, ((in.sum_length + kTile - 1) / kTile + int64_t(in.batch) * ((nodes + kTile - 1) / kTile) + 1) / 2 * p.heads_kv);
+      1, ((in.sum_length + kTile - 1) / kTile + int64_t(in.batch) * ((nodes + kTile - 1) / kTile)) * p.heads_kv);
   int splits = 1;
-  while (splits < kMaxCluster && all * splits * 2 <= sm_count() && q_tiles >= splits * 2) splits *= 2;
+  int64_t best = INT64_MAX;
+  for (int x = 1; x <= kMaxCluster && x <= q_tiles; ++x) {
+    const int64_t cost = (all * x + sm_count() - 1) / sm_count() * ((q_tiles + x - 1) / x + 4);
+    if (cost < best) {
+      best = cost;
+      splits = x;
+    }
+  }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(splits), unsigned(p.heads_kv * in.batch), unsigned(pairs));
+  cfg.gridDim = dim3(unsigned(splits), unsigned(p.heads_kv * in.batch), unsigned(max_tiles));
   cfg.blockDim = dim3(kTcThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -571,7 +548,7 @@ int run_weights_tc(const WeightParams &p, const qe_draft_batch &in, int nodes, c
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p), "qe_attention_weights launch");
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, map, p), "qe_attention_weights launch");
 }
 
 bool al16(int64_t v) { return v % 16 == 0; }
@@ -633,8 +610,8 @@ extern "C" int qe_attention_weights(qe_draft_batch batch, const void *q, int64_t
   per = std::min<int64_t>(std::max<int64_t>((per + kWarps - 1) / kWarps * kWarps, kWarps), 1 << 20);
   p.tiles_per_cta = int(per);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int64_t(batch.max_nodes) * p.group > kTcRows) {
-    QE_CHECK_ARG(int64_t(heads_kv) * batch.batch <= 65535 && (max_tiles + 7) / 8 / 2 < 65535,
+  if (int64_t(batch.max_nodes) * p.group > kTcRows && p.group <= kTile) {
+    QE_CHECK_ARG(int64_t(heads_kv) * batch.batch <= 65535 && (max_tiles + 7) / 8 < 65535,
                  "qe_attention_weights: too many requests x heads_kv, or keys, for one launch");
     if (dtype == 1)
       s = head_dim == 128 ? run_weights_tc<__nv_bfloat16, 128>(p, batch, nodes, st)
