@@ -140,11 +140,11 @@ __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
 // the exponent bits of a 16-bit type: all set in an infinity or NaN
 template <typename T>
-__device__ __forceinline__ constexpr uint32_t exponent_bits();
+__host__ __device__ __forceinline__ constexpr uint32_t exponent_bits();
 template <>
-__device__ __forceinline__ constexpr uint32_t exponent_bits<__nv_bfloat16>() { return 0x7f80u; }
+__host__ __device__ __forceinline__ constexpr uint32_t exponent_bits<__nv_bfloat16>() { return 0x7f80u; }
 template <>
-__device__ __forceinline__ constexpr uint32_t exponent_bits<__half>() { return 0x7c00u; }
+__host__ __device__ __forceinline__ constexpr uint32_t exponent_bits<__half>() { return 0x7c00u; }
 
 __device__ __forceinline__ float exp2_approx(float x) {  // relative error below 2^-22
   float y;

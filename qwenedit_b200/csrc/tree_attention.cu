@@ -12,6 +12,7 @@
 #include <cstring>
 
 #include "qe_decode.cuh"
+#include "qe_tcgen05.cuh"
 
 namespace qe {
 
@@ -112,7 +113,8 @@ struct TreeParams {
   int64_t out_token, out_head;  // bytes
   float *lse;
   int heads_q, heads_kv, group;
-  int tiles_per_cta;  // 16-key tiles
+  int key_tile;       // keys per tile
+  int tiles_per_cta;
   int splits;         // splits of the longest request (the workspace's)
   float scale_log2;
   float *part_o;   // [splits][total * heads_q][D]
@@ -129,8 +131,8 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return uint32_t(r * row_bytes<D>() + ((c ^ (r & 7)) << 4));
 }
 
-__host__ __device__ inline int tiles_of(int len, int drafted) {
-  return (len + kKeys - 1) / kKeys + (drafted + kKeys - 1) / kKeys;
+__host__ __device__ inline int tiles_of(int len, int drafted, int tile) {
+  return (len + tile - 1) / tile + (drafted + tile - 1) / tile;
 }
 
 template <int D, int MT>
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
   if (rows <= 0) return;
   const int drafted = p.k_draft ? rq.n : 0;
   const int cached_tiles = (rq.len + kKeys - 1) / kKeys;
-  const int tiles = tiles_of(rq.len, drafted);
+  const int tiles = tiles_of(rq.len, drafted, kKeys);
   const int first = int(blockIdx.x) * p.tiles_per_cta;
   if (first >= tiles && blockIdx.x > 0) return;  // split 0 writes the rows of a request without keys
   const int last = min(tiles, first + p.tiles_per_cta);
@@ -488,6 +490,436 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
   }
 }
 
+// ---- many rows: both products on the fifth-generation tensor cores -----------------------------------------------
+//
+// A CTA takes up to two tiles of 128 rows (the G heads of as many whole nodes as fit) of one K/V head and runs over
+// its share of the keys, 128 at a time: S = Q K^T, softmax in registers, O += P V with P from tensor memory.
+//   warps 0-7   softmax, one warpgroup per row tile, a thread per row (tensor-memory lane)
+//   warps 8, 9  K and V tiles into two-stage rings. Cached keys: warp 8, a lane per four keys, one TMA gather of four
+//               pool rows per 64 dims (any page size; keys past the length or in bad pages read zeros). Drafted keys:
+//               both warps through registers, because values that are not finite are taken out of V (0 x inf would
+//               reach the rows that do not see them) and put back at the end, for the rows that do.
+//   warp 10     Q by TMA, tcgen05.mma (one thread), and the tensor memory: S0 | O0 | S1 | O1, P_t over S_t
+// The products of one thread execute in issue order, so P_t V(j) reads P_t(j) before Q_t K^T(j + 1) rewrites S_t, and
+// S_t(j + 1) being there means that O_t holds every product up to tile j.
+
+constexpr int kTcTile = 128;
+constexpr int kTcThreads = 11 * 32;
+enum TBar { tQFull = 0, tKFull = 1, tKEmpty = 3, tVFull = 5, tVEmpty = 7, tSFull = 9, tPReady = 11, tOFinal = 13,
+            tDrain = 14, tBars = 15 };
+
+template <int D>
+struct TSmem {
+  static constexpr int half = kTcTile * 128;  // 128 rows of 64 dims: one 128-byte swizzle span each
+  static constexpr int tile = half * (D / 64);
+  static constexpr int q = 0;
+  static constexpr int k = 2 * tile;
+  static constexpr int v = 4 * tile;
+  static constexpr int bars = 6 * tile;
+  static constexpr int slot = bars + tBars * 8;
+  static constexpr int abort = slot + 4;
+  static constexpr int odd = abort + 4;
+  // slack to align the base; never so few that two CTAs, each with all of the tensor memory, would share an SM
+  static constexpr int bytes = odd + 4 + 1024 > 116 * 1024 ? odd + 4 + 1024 : 116 * 1024;
+};
+
+// kind::f16 instruction descriptor: fp32 accumulator (bit 4), operand types (bits 7-12: bf16 1, fp16 0), N >> 3 at
+// bits 17-22, M >> 4 at bits 24-28; bit 16: B is MN-major (V)
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t idesc_of(int n, bool b_mn_major) {
+  return (1u << 4) | (exponent_bits<T>() == 0x7f80u ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u) |
+         (uint32_t(n >> 3) << 17) | (uint32_t(kTcTile >> 4) << 24);
+}
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// four rows of a 2-D map (box [64, 1]) to four consecutive 128-byte rows of shared memory
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, int32_t x, const int (&row)[4],
+                                            uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+      "%4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
+      : "memory");
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                             const __grid_constant__ CUtensorMap tm_v, const int pool_rows, const TreeParams p) {
+  using S = TSmem<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t base = smem_addr(smem);
+  auto bar = [&](int i) { return base + S::bars + 8u * uint32_t(i); };
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + S::slot);
+  volatile int *abort = reinterpret_cast<volatile int *>(smem + S::abort);
+  volatile int *odd = reinterpret_cast<volatile int *>(smem + S::odd);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z, kvh = int(blockIdx.y) % p.heads_kv;
+  grid_dep_wait();
+  grid_dep_launch();
+  const Request rq = request_of(p.batch, b);
+  const int nodes = kTcTile / p.group, filled = nodes * p.group;  // nodes of a row tile, rows of it that hold one
+  const int node0 = int(blockIdx.y) / p.heads_kv * 2 * nodes;     // first node of this CTA
+  if (node0 >= rq.n) return;
+  const int q_tiles = rq.n - node0 > nodes ? 2 : 1;
+  const int drafted = p.k_draft ? rq.n : 0;
+  const int cached_tiles = (rq.len + kTcTile - 1) / kTcTile;
+  const int tiles = tiles_of(rq.len, drafted, kTcTile);
+  const int first = int(blockIdx.x) * p.tiles_per_cta;
+  if (first >= tiles && blockIdx.x > 0) return;  // split 0 writes the rows of a request without keys
+  const int n_tiles = min(tiles, first + p.tiles_per_cta) - first;
+  const bool whole = tiles <= p.tiles_per_cta;
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar(tQFull), 3);  // the copy of Q, and the two warps that clear the rows it leaves
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar(tKFull + s), 2);
+      mbar_init(bar(tKEmpty + s), 1);
+      mbar_init(bar(tVFull + s), 2);
+      mbar_init(bar(tVEmpty + s), 1);
+      mbar_init(bar(tSFull + s), 1);
+      mbar_init(bar(tPReady + s), 4);
+    }
+    mbar_init(bar(tOFinal), 1);
+    mbar_init(bar(tDrain), 1);
+    *abort = 0;
+    *odd = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 10) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  constexpr int kChunks = D / 8;
+
+  if (warp == 8 || warp == 9) {
+    // ---- rows of the Q tiles that hold no node: zeros ----
+    const int me = (warp - 8) * 32 + lane, rest = kTcTile - filled;
+    for (int i = me; i < q_tiles * rest * kChunks; i += 64) {
+      const int c = i % kChunks, r = filled + i / kChunks % rest, t = i / kChunks / rest;
+      const uint32_t at = base + S::q + t * S::tile + uint32_t(c >> 3) * S::half + uint32_t(r) * 128u +
+                          uint32_t(((c & 7) ^ (r & 7)) << 4);
+      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+    }
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(tQFull));
+    // ---- K and V tiles ----
+    // pool rows of this lane's four keys of a tile, looked up a tile ahead; pool_rows (outside the map: zeros) where
+    // there is none
+    auto lookup = [&](int t, int(&row)[4]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = t * kTcTile + lane * 4 + e;
+        row[e] = t < cached_tiles && key < rq.len ? pool_row(p.batch, b, key) : -1;
+        if (row[e] < 0) row[e] = pool_rows;
+      }
+    };
+    // 64 rows of a drafted tile, 16 bytes a lane and step
+    auto copy_draft = [&](const char *src, uint32_t dst, int j0, bool clean) {
+      for (int i = lane; i < 64 * kChunks; i += 32) {
+        const int r = (warp - 8) * 64 + i / kChunks, c = i % kChunks;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (j0 + r < drafted)
+          x = __ldg(reinterpret_cast<const uint4 *>(src + int64_t(rq.lo + j0 + r) * p.draft_token +
+                                                    int64_t(kvh) * p.draft_head + c * 16));
+        if (clean) {
+          constexpr uint32_t kExp = exponent_bits<T>();
+          uint32_t w[4] = {x.x, x.y, x.z, x.w};
+          bool here = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool lo = (w[e] & kExp) == kExp, hi = ((w[e] >> 16) & kExp) == kExp;
+            here |= lo || hi;
+            w[e] = (lo ? 0u : (w[e] & 0xffffu)) | (hi ? 0u : (w[e] & 0xffff0000u));
+          }
+          if (here) *odd = 1;
+          x = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                         dst + uint32_t(c >> 3) * S::half + uint32_t(r) * 128u + uint32_t(((c & 7) ^ (r & 7)) << 4)),
+                     "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
+                     : "memory");
+      }
+      fence_async_smem();
+    };
+    int row[4];
+    if (warp == 8) lookup(first, row);
+    bool ok = true;
+    for (int i = 0; i < n_tiles && ok; ++i) {
+      const int s = i & 1, t = first + i;
+      const uint32_t empty = ((i >> 1) & 1) ^ 1;
+      const bool draft = t >= cached_tiles;
+#pragma unroll
+      for (int kv = 0; kv < 2 && ok; ++kv) {
+        const uint32_t full = bar((kv ? tVFull : tKFull) + s), dst = base + (kv ? S::v : S::k) + s * S::tile;
+        ok = __all_sync(0xffffffffu, mbar_wait(bar((kv ? tVEmpty : tKEmpty) + s), empty, abort, p.batch.err));
+        if (!ok) break;
+        if (draft) {
+          copy_draft(kv ? p.v_draft : p.k_draft, dst, (t - cached_tiles) * kTcTile, kv);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full);
+        } else if (warp == 9) {
+          if (lane == 0) mbar_arrive(full);
+        } else {
+          if (lane == 0) mbar_expect_tx(full, S::tile);
+          __syncwarp();
+          for (int h = 0; h < D / 64; ++h)
+            tma_gather4(dst + h * S::half + lane * 512, kv ? &tm_v : &tm_k, kvh * D + h * 64, row, full);
+        }
+      }
+      if (warp == 8 && ok) lookup(t + 1, row);
+    }
+    if (!ok) {  // a wait gave up: time for the copies in flight before the shared memory is given back
+      const uint64_t since = globaltimer();
+      while (globaltimer() - since < 200000ull) {
+      }
+    }
+  } else if (warp == 10) {
+    if (lane == 0) {
+      // ---- Q, and the products ----
+      mbar_expect_tx(bar(tQFull), uint32_t(q_tiles) * uint32_t(filled) * (D * 2));
+      for (int t = 0; t < q_tiles; ++t)
+        for (int h = 0; h < D / 64; ++h)
+          tma_load_3d(base + S::q + t * S::tile + h * S::half, &tm_q, h * 64, kvh * p.group, rq.lo + node0 + t * nodes,
+                      bar(tQFull));
+      constexpr uint32_t idesc_qk = idesc_of<T>(kTcTile, false), idesc_pv = idesc_of<T>(D, true);
+      auto qk = [&](int t, int s) {
+        const uint64_t a = sw128_desc(base + S::q + t * S::tile, 16, 1024), k = sw128_desc(base + S::k + s * S::tile, 16, 1024);
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) {
+          const uint64_t off = uint64_t((x >> 2) * S::half + (x & 3) * 32) >> 4;
+          mma_ss(tmem + t * 256, a + off, k + off, idesc_qk, x > 0);
+        }
+      };
+      auto pv = [&](int t, int s, bool acc) {
+        const uint64_t v = sw128_desc(base + S::v + s * S::tile, S::half, 1024);
+#pragma unroll
+        for (int x = 0; x < kTcTile / 16; ++x)
+          mma_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * x, v + uint64_t(x * 2048 >> 4), idesc_pv, acc || x > 0);
+      };
+      bool ok = mbar_wait(bar(tQFull), 0, abort, p.batch.err);
+      if (ok && n_tiles > 0) {
+        ok = mbar_wait(bar(tKFull), 0, abort, p.batch.err);
+        if (ok) {
+          tc_fence_after();
+          for (int t = 0; t < q_tiles; ++t) {
+            qk(t, 0);
+            mma_commit(bar(tSFull + t));
+          }
+          mma_commit(bar(tKEmpty));
+        }
+        for (int i = 0; i < n_tiles && ok; ++i) {
+          const int s = i & 1, s1 = s ^ 1;
+          ok = mbar_wait(bar(tVFull + s), (i >> 1) & 1, abort, p.batch.err);
+          for (int t = 0; t < q_tiles && ok; ++t) {
+            ok = mbar_wait(bar(tPReady + t), i & 1, abort, p.batch.err);
+            if (!ok) break;
+            tc_fence_after();
+            pv(t, s, i > 0);
+            if (i + 1 < n_tiles) {
+              if (t == 0) {
+                ok = mbar_wait(bar(tKFull + s1), ((i + 1) >> 1) & 1, abort, p.batch.err);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              qk(t, s1);
+              mma_commit(bar(tSFull + t));
+            }
+          }
+          if (!ok) break;
+          mma_commit(bar(tVEmpty + s));
+          if (i + 1 < n_tiles) mma_commit(bar(tKEmpty + s1));
+        }
+      }
+      mma_commit(bar(tOFinal));
+      if (!ok) {  // the products already issued land before the tensor memory is released
+        mma_commit(bar(tDrain));
+        const uint64_t since = globaltimer();
+        while (!mbar_try(bar(tDrain), 0) && globaltimer() - since < kWaitNs) {
+        }
+      }
+    }
+  } else if ((warp >> 2) < q_tiles) {
+    // ---- softmax: this thread's row ----
+    const int t = warp >> 2, r = (warp & 3) * 32 + lane;
+    const int dn = r / p.group, node = node0 + t * nodes + dn;
+    const bool mine = r < filled && node < rq.n;
+    const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
+    const uint32_t s_col = lanes + t * 256, o_col = s_col + 128;
+    // keys 32 c .. 32 c + 31 of tile `at` that the row sees, a bit each
+    auto bits32 = [&](int at, int c) -> uint32_t {
+      int seen;
+      if (at < cached_tiles) {
+        seen = rq.len - at * kTcTile - 32 * c;
+      } else {
+        const int j0 = (at - cached_tiles) * kTcTile + 32 * c;
+        if (!mine) return 0u;
+        if (p.batch.mode == 1)
+          return j0 / 32 < p.batch.mask_words && j0 < rq.n
+                     ? uint32_t(__ldg(p.batch.masks + int64_t(rq.lo + node) * p.batch.mask_words + j0 / 32)) &
+                           (rq.n - j0 >= 32 ? ~0u : (1u << (rq.n - j0)) - 1u)
+                     : 0u;
+        seen = (p.batch.mode == 0 ? node + 1 : rq.n) - j0;
+      }
+      return seen >= 32 ? ~0u : seen <= 0 ? 0u : (1u << seen) - 1u;
+    };
+    float m_use = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int i = 0; i < n_tiles; ++i) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(tSFull + t), i & 1, abort, p.batch.err));
+      if (!ok) break;
+      tc_fence_after();
+      const int at = first + i;
+      const bool masked = at >= cached_tiles || (at + 1) * kTcTile > rq.len;  // the same for the whole CTA
+      uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) bits[c] = bits32(at, c);
+      }
+      uint32_t buf[2][32];
+      // the row's maximum over the visible keys; the columns are read again for the exponentials
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      tmem_ld32_async(s_col, buf[0]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_wait(buf[c & 1]);
+        if (c + 1 < 4) tmem_ld32_async(s_col + 32 * (c + 1), buf[(c + 1) & 1]);
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) m4[e & 3] = (bits[c] >> e) & 1u ? fmaxf(m4[e & 3], __uint_as_float(buf[c & 1][e])) : m4[e & 3];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              m4[x] = max3(m4[x], __uint_as_float(buf[c & 1][e + 2 * x]), __uint_as_float(buf[c & 1][e + 2 * x + 1]));
+          }
+        }
+      }
+      const float mx = max3(m4[0], m4[1], fmaxf(m4[2], m4[3])) * p.scale_log2;
+      // The reference maximum moves only when the row's maximum passes it by more than 2^8 (or is its first); O and
+      // the sum scale down with it. The tensor-memory accesses are the warp's, so rows that keep theirs scale by 1.
+      const bool grow = mx > m_use + kGrowLog2;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float f = grow && m_use != -INFINITY ? join_factor(m_use, mx) : 1.0f;
+        if (i > 0) {
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t w[32];
+            tmem_ld32_async(o_col + 32 * c, w);
+            tmem_ld_wait(w);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
+            tmem_st32(o_col + 32 * c, w);
+          }
+        }
+        l *= f;
+        if (grow) m_use = mx;
+      }
+      const float nbase = m_use == -INFINITY ? 0.0f : -m_use;
+      const f32x2 scale2 = pk2(p.scale_log2, p.scale_log2), nbase2 = pk2(nbase, nbase);
+      f32x2 sum[2] = {pk2(0.0f, 0.0f), pk2(0.0f, 0.0f)};
+      tmem_ld32_async(s_col, buf[0]);
+      // p = 2^(s scale - base), rounded to the type of V and written over the scores already read: keys 32 c .. to
+      // columns 16 c .. 16 c + 15. The row sum takes the unrounded values.
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_wait(buf[c & 1]);
+        if (c + 1 < 4) tmem_ld32_async(s_col + 32 * (c + 1), buf[(c + 1) & 1]);
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float2 x = up2(fma2(pk2(__uint_as_float(buf[c & 1][2 * e]), __uint_as_float(buf[c & 1][2 * e + 1])), scale2, nbase2));
+          float y0 = ex2(x.x), y1 = ex2(x.y);
+          if (masked) {
+            y0 = (bits[c] >> (2 * e)) & 1u ? y0 : 0.0f;
+            y1 = (bits[c] >> (2 * e + 1)) & 1u ? y1 : 0.0f;
+          }
+          sum[e & 1] = add2(sum[e & 1], pk2(y0, y1));
+          w[e] = pack2<T>(y0, y1);
+        }
+        tmem_st16(s_col + 16 * c, w);
+      }
+      const float2 a = up2(add2(sum[0], sum[1]));
+      l += a.x + a.y;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(tPReady + t));
+    }
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(tOFinal), 0, abort, p.batch.err));
+    const bool drafts = first + n_tiles > cached_tiles;
+    if (ok && drafts)  // what the copying warps found in V
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(tVFull + ((n_tiles - 1) & 1)), ((n_tiles - 1) >> 1) & 1, abort, p.batch.err));
+    if (ok) {
+      tc_fence_after();
+      const int token = rq.lo + node, head = kvh * p.group + r - dn * p.group;
+      const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+      const bool put_back = drafts && *odd;
+      char *dst = p.out + int64_t(token) * p.out_token + int64_t(head) * p.out_head;
+      const int64_t part = (int64_t(blockIdx.x) * p.batch.total + token) * p.heads_q + head;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t w[32];
+        __syncwarp();
+        tmem_ld32_async(o_col + 32 * c, w);
+        tmem_ld_wait(w);
+        if (!mine) continue;
+        float o[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : __uint_as_float(w[e]);  // no key seen: O may be unwritten
+        if (put_back) {
+          for (int j = max(first - cached_tiles, 0) * kTcTile; j < min(rq.n, (first + n_tiles - cached_tiles) * kTcTile); ++j) {
+            if (!((bits32(cached_tiles + j / kTcTile, j % kTcTile / 32) >> (j & 31)) & 1u)) continue;
+            const T *v = reinterpret_cast<const T *>(p.v_draft + int64_t(rq.lo + j) * p.draft_token + int64_t(kvh) * p.draft_head) + 32 * c;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float x = to_float(v[e]);
+              if (!(fabsf(x) < INFINITY)) o[e] += x;
+            }
+          }
+        }
+        if (whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint4 x;
+            x.x = pack2<T>(o[e] * inv, o[e + 1] * inv);
+            x.y = pack2<T>(o[e + 2] * inv, o[e + 3] * inv);
+            x.z = pack2<T>(o[e + 4] * inv, o[e + 5] * inv);
+            x.w = pack2<T>(o[e + 6] * inv, o[e + 7] * inv);
+            *reinterpret_cast<uint4 *>(dst + (32 * c + e) * 2) = x;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4 *>(p.part_o + part * D + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      }
+      if (mine) {
+        if (!whole)
+          p.part_ml[part] = make_float2(m_use, l);
+        else if (p.lse)
+          p.lse[int64_t(head) * p.batch.total + token] = l == 0.0f ? -INFINITY : (m_use + log2f(l)) * kLn2;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 10) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
 // Joins the splits of the requests that have more than one: a warp per (node, head) row.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
@@ -498,7 +930,7 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
   grid_dep_launch();
   const Request rq = request_of(p.batch, b);
   if (at >= rq.n * p.heads_q) return;
-  const int tiles = tiles_of(rq.len, p.k_draft ? rq.n : 0);
+  const int tiles = tiles_of(rq.len, p.k_draft ? rq.n : 0, p.key_tile);
   if (tiles <= p.tiles_per_cta) return;
   const int splits = min((tiles + p.tiles_per_cta - 1) / p.tiles_per_cta, p.splits);
   const int token = rq.lo + at / p.heads_q, head = at % p.heads_q;
@@ -533,22 +965,36 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
 // ---- host -------------------------------------------------------------------------------------------------------
 
 struct TreePlan {
-  int m_tiles;        // 16-row tiles per CTA: 1 or 2
-  int tiles_per_cta;  // 16-key tiles
+  bool tc;            // the tensor-memory kernel
+  int m_tiles;        // else: 16-row tiles per CTA, 1 or 2
+  int tiles_per_cta;  // of key_tile keys
+  int key_tile;
+  int row_ctas;       // CTAs for the rows of a request, all K/V heads
   int splits;
   int64_t workspace;
 };
 
+// More rows a K/V head than this take the tensor-memory kernel, whose row tile is 128 (the groups must fit it).
+#ifndef QE_TREE_TC_ROWS
+#define QE_TREE_TC_ROWS 32
+#endif
+constexpr int kTcRows = QE_TREE_TC_ROWS;
+
 TreePlan tree_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head_dim) {
   TreePlan t{};
-  const int64_t rows = int64_t(in.max_nodes) * (heads_q / heads_kv);
+  const int group = heads_q / heads_kv;
+  const int64_t rows = int64_t(in.max_nodes) * group;
+  t.tc = rows > kTcRows && group <= kTcTile;
   t.m_tiles = rows <= 16 ? 1 : 2;
-  const int64_t row_ctas = std::max<int64_t>(1, (rows + t.m_tiles * 16 - 1) / (t.m_tiles * 16)) * heads_kv;
-  const int64_t max_tiles = std::max(1, tiles_of(in.max_length, in.max_nodes));
-  // tiles of the whole batch, spread over two CTAs per SM
-  const int64_t all = (in.sum_length + kKeys - 1) / kKeys + int64_t(in.batch) * tiles_of(0, in.max_nodes);
-  int64_t per = (all * row_ctas + 2 * sm_count() - 1) / (2 * sm_count());
-  per = std::max<int64_t>((per + kWarps - 1) / kWarps * kWarps, kWarps);
+  t.key_tile = t.tc ? kTcTile : kKeys;
+  const int64_t per_cta = t.tc ? int64_t(2 * (kTcTile / group)) * group : t.m_tiles * 16;  // rows
+  t.row_ctas = int(std::min<int64_t>(std::max<int64_t>(1, (rows + per_cta - 1) / per_cta) * heads_kv, 1 << 30));
+  const int64_t max_tiles = std::max(1, tiles_of(in.max_length, in.max_nodes, t.key_tile));
+  // tiles of the whole batch, spread over the CTAs that the SMs hold: two, or one with all of the tensor memory
+  const int64_t all = (in.sum_length + t.key_tile - 1) / t.key_tile + int64_t(in.batch) * tiles_of(0, in.max_nodes, t.key_tile);
+  const int64_t ctas = (t.tc ? 1 : 2) * sm_count(), step = t.tc ? 1 : kWarps;
+  int64_t per = (all * t.row_ctas + ctas - 1) / ctas;
+  per = std::max<int64_t>((per + step - 1) / step * step, step);
   if (per >= max_tiles) per = max_tiles;
   t.tiles_per_cta = int(per);
   t.splits = int((max_tiles + per - 1) / per);
@@ -556,8 +1002,8 @@ TreePlan tree_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head
   return t;
 }
 
-template <auto kKernel>
-int launch(dim3 grid, int threads, int smem, cudaStream_t stream, const TreeParams &p, const char *what) {
+template <auto kKernel, typename... Args>
+int launch(dim3 grid, int threads, int smem, cudaStream_t stream, const char *what, const Args &...args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(unsigned(threads));
@@ -578,21 +1024,37 @@ int launch(dim3 grid, int threads, int smem, cudaStream_t stream, const TreePara
       raised[dev].store(true, std::memory_order_relaxed);
     }
   }
-  return cuda_status(cudaLaunchKernelEx(&cfg, kKernel, p), what);
+  return cuda_status(cudaLaunchKernelEx(&cfg, kKernel, args...), what);
 }
 
 template <typename T, int D>
-int run_tree(const TreeParams &p, const TreePlan &t, const qe_draft_batch &in, cudaStream_t stream) {
-  const int rows = in.max_nodes * p.group;
-  const dim3 grid(unsigned(t.splits), unsigned((rows + t.m_tiles * 16 - 1) / (t.m_tiles * 16) * p.heads_kv),
-                  unsigned(in.batch));
-  const int s = t.m_tiles == 1 ? launch<tree_attention_kernel<T, D, 1>>(grid, kWarps * 32, tree_smem_bytes<D, 1>(),
-                                                                        stream, p, "qe_tree_attention launch")
-                               : launch<tree_attention_kernel<T, D, 2>>(grid, kWarps * 32, tree_smem_bytes<D, 2>(),
-                                                                        stream, p, "qe_tree_attention launch");
+int run_tree(const TreeParams &p, const TreePlan &t, const qe_draft_batch &in, int64_t pool_rows, cudaStream_t stream) {
+  const dim3 grid(unsigned(t.splits), unsigned(t.row_ctas), unsigned(in.batch));
+  int s;
+  if (t.tc) {
+    const CUtensorMapDataType type = exponent_bits<T>() == 0x7f80u ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap q, kv[2];
+    std::memset(kv, 0, sizeof(kv));
+    const uint64_t q_dims[3] = {uint64_t(D), uint64_t(p.heads_q), uint64_t(in.total)};
+    const uint64_t q_strides[2] = {uint64_t(p.q_head), uint64_t(p.q_token)};
+    const uint32_t q_box[3] = {64, uint32_t(p.group), uint32_t(kTcTile / p.group)};
+    if ((s = tensor_map_16bit("qe_tree_attention", &q, type, p.q, 3, q_dims, q_strides, q_box, "q"))) return s;
+    if (p.batch.table_width > 0 && in.max_length > 0) {
+      const uint64_t dims[2] = {uint64_t(p.heads_kv) * D, uint64_t(pool_rows)}, strides[1] = {uint64_t(p.pool_row)};
+      const uint32_t box[2] = {64, 1};
+      if ((s = tensor_map_16bit("qe_tree_attention", &kv[0], type, p.k_pool, 2, dims, strides, box, "the K plane"))) return s;
+      if ((s = tensor_map_16bit("qe_tree_attention", &kv[1], type, p.v_pool, 2, dims, strides, box, "the V plane"))) return s;
+    }
+    s = launch<tree_attention_tc_kernel<T, D>>(grid, kTcThreads, TSmem<D>::bytes, stream, "qe_tree_attention launch", q, kv[0],
+                                               kv[1], int(pool_rows), p);
+  } else if (t.m_tiles == 1) {
+    s = launch<tree_attention_kernel<T, D, 1>>(grid, kWarps * 32, tree_smem_bytes<D, 1>(), stream, "qe_tree_attention launch", p);
+  } else {
+    s = launch<tree_attention_kernel<T, D, 2>>(grid, kWarps * 32, tree_smem_bytes<D, 2>(), stream, "qe_tree_attention launch", p);
+  }
   if (s || t.splits == 1) return s;
   const dim3 join(unsigned((in.max_nodes * p.heads_q + 7) / 8), unsigned(in.batch));
-  return launch<tree_join_kernel<T, D>>(join, 256, 0, stream, p, "qe_tree_attention join launch");
+  return launch<tree_join_kernel<T, D>>(join, 256, 0, stream, "qe_tree_attention join launch", p);
 }
 
 bool al16(int64_t v) { return v % 16 == 0; }
@@ -672,6 +1134,7 @@ extern "C" int qe_tree_attention(qe_draft_batch batch, const void *q, int64_t q_
   p.heads_q = heads_q;
   p.heads_kv = heads_kv;
   p.group = heads_q / heads_kv;
+  p.key_tile = t.key_tile;
   p.tiles_per_cta = t.tiles_per_cta;
   p.splits = t.splits;
   p.scale_log2 = scale * kLog2e;
@@ -679,8 +1142,10 @@ extern "C" int qe_tree_attention(qe_draft_batch batch, const void *q, int64_t q_
   p.part_ml = reinterpret_cast<float2 *>(p.part_o + int64_t(t.splits) * batch.total * heads_q * head_dim);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == 1)
-    s = head_dim == 128 ? run_tree<__nv_bfloat16, 128>(p, t, batch, st) : run_tree<__nv_bfloat16, 64>(p, t, batch, st);
+    s = head_dim == 128 ? run_tree<__nv_bfloat16, 128>(p, t, batch, pool_rows, st)
+                        : run_tree<__nv_bfloat16, 64>(p, t, batch, pool_rows, st);
   else
-    s = head_dim == 128 ? run_tree<__half, 128>(p, t, batch, st) : run_tree<__half, 64>(p, t, batch, st);
+    s = head_dim == 128 ? run_tree<__half, 128>(p, t, batch, pool_rows, st)
+                        : run_tree<__half, 64>(p, t, batch, pool_rows, st);
   return s ? s : ok();
 }
