@@ -38,23 +38,20 @@ __device__ __forceinline__ Request request_of(const DecodeBatch &p, int b) {
   return r;
 }
 
-// Pool row of cached token `key` of request b; -1 (read as zeros) when its page lies outside the pool, which is
-// reported in bit 1 of the error flag.
-__device__ __forceinline__ int pool_row(const DecodeBatch &p, int b, int key) {
-  int page_index, offset;
-  if (p.page_shift >= 0) {
-    page_index = key >> p.page_shift;
-    offset = key & (p.page_size - 1);
-  } else {
-    page_index = key / p.page_size;
-    offset = key - page_index * p.page_size;
-  }
-  const int page = __ldg(p.tables + int64_t(b) * p.table_width + page_index);
+// Where cached token `key` lies: its index in the request's table, and, given the page found there, its pool row; -1
+// (read as zeros) when the page lies outside the pool, which is reported in bit 1 of the error flag.
+__device__ __forceinline__ int page_index(const DecodeBatch &p, int key) {
+  return p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size;
+}
+__device__ __forceinline__ int row_in_page(const DecodeBatch &p, int page, int key) {
   if (page < 0 || page >= p.pool_pages) {
     if (p.err) atomicOr(p.err, 1);
     return -1;
   }
-  return page * p.page_size + offset;
+  return page * p.page_size + (p.page_shift >= 0 ? key & (p.page_size - 1) : key % p.page_size);
+}
+__device__ __forceinline__ int pool_row(const DecodeBatch &p, int b, int key) {
+  return row_in_page(p, __ldg(p.tables + int64_t(b) * p.table_width + page_index(p, key)), key);
 }
 
 // Drafted keys [j0, j0 + 16) that drafted node i sees, one bit each (j0 a multiple of 16). mode 0: a chain (node i
@@ -84,6 +81,11 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// arrives at an mbarrier for this thread once its copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {

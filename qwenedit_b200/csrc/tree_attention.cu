@@ -8,6 +8,7 @@
 // by out = sum_w e^{m_w - m} O_w / sum_w e^{m_w - m} l_w.
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <cstring>
 
@@ -172,14 +173,18 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
 
   // ---- K/V tiles: lanes 0-15 look up a key's row each, every lane copies 16-byte chunks ----
   const int64_t head_off = int64_t(kvh) * kRow;
-  auto lookup = [&](int t) -> int {  // pool row or drafted token of key `lane` of tile t; -1: nothing there
-    if (t >= last || lane >= kKeys) return -1;
-    if (t < cached_tiles) {
-      const int key = t * kKeys + lane;
-      return key < rq.len ? pool_row(p.batch, b, key) : -1;
-    }
+  // key `lane` of tile t: fetch reads its table entry, settle makes of it, a tile later, the pool row (or the drafted
+  // token; -1: nothing there), so that no one waits for the table
+  auto fetch = [&](int t) -> int {
+    const int key = t * kKeys + lane;
+    return t < last && t < cached_tiles && lane < kKeys && key < rq.len
+               ? __ldg(p.batch.tables + int64_t(b) * p.batch.table_width + page_index(p.batch, key))
+               : INT_MIN;
+  };
+  auto settle = [&](int t, int page) -> int {
+    if (t < cached_tiles) return page == INT_MIN ? -1 : row_in_page(p.batch, page, t * kKeys + lane);
     const int j = (t - cached_tiles) * kKeys + lane;
-    return j < drafted ? rq.lo + j : -1;
+    return t < last && lane < kKeys && j < drafted ? rq.lo + j : -1;
   };
   auto copy_tile = [&](int t, int stage, int row) {
     if (t < last) {
@@ -201,14 +206,15 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
     cp_async_commit();
   };
   int t_load = first + warp;
-  int row_next = lookup(t_load);
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    const int row = row_next;
-    row_next = lookup(t_load + kWarps);
-    copy_tile(t_load, s, row);
+  int page = fetch(t_load);
+  auto copy_next = [&](int stage) {
+    const int row = settle(t_load, page);
+    page = fetch(t_load + kWarps);
+    copy_tile(t_load, stage, row);
     t_load += kWarps;
-  }
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) copy_next(s);
 
   // ---- Q: row r = (node (row0 + r) / G, head (row0 + r) % G of the group) ----
   for (int i = threadIdx.x; i < MT * 16 * kChunks; i += kWarps * 32) {
@@ -254,12 +260,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
   for (int t = first + warp; t < last; t += kWarps) {
     cp_async_wait<kStages - 2>();
     __syncwarp();  // every lane's copies of this tile have landed, and the stage filled next is no longer read
-    {
-      const int row = row_next;
-      row_next = lookup(t_load + kWarps);
-      copy_tile(t_load, (stage + kStages - 1) % kStages, row);
-      t_load += kWarps;
-    }
+    copy_next((stage + kStages - 1) % kStages);
     const uint32_t kt = ring + stage * (2 * kTileBytes), vt = kt + kTileBytes;
     // S = Q K^T: keys 0-7 and 8-15 of the tile
     float s[MT][2][4];
@@ -495,16 +496,17 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
 // A CTA takes up to two tiles of 128 rows (the G heads of as many whole nodes as fit) of one K/V head and runs over
 // its share of the keys, 128 at a time: S = Q K^T, softmax in registers, O += P V with P from tensor memory.
 //   warps 0-7   softmax, one warpgroup per row tile, a thread per row (tensor-memory lane)
-//   warps 8, 9  K and V tiles into two-stage rings. Cached keys: warp 8, a lane per four keys, one TMA gather of four
-//               pool rows per 64 dims (any page size; keys past the length or in bad pages read zeros). Drafted keys:
-//               both warps through registers, because values that are not finite are taken out of V (0 x inf would
-//               reach the rows that do not see them) and put back at the end, for the rows that do.
-//   warp 10     Q by TMA, tcgen05.mma (one thread), and the tensor memory: S0 | O0 | S1 | O1, P_t over S_t
+//   warps 8-10  K and V tiles into two-stage rings: cached keys by cp.async through the block table (any page size;
+//               keys past the length or in bad pages read zeros; a TMA gather of four rows a lane took 10 us a tile),
+//               drafted keys through registers, because values that are not finite are taken out of V (0 x inf would
+//               reach the rows that do not see them) and put back at the end, for the rows that do
+//   warp 11     Q by TMA, tcgen05.mma (one thread), and the tensor memory: S0 | O0 | S1 | O1, P_t over S_t
 // The products of one thread execute in issue order, so P_t V(j) reads P_t(j) before Q_t K^T(j + 1) rewrites S_t, and
 // S_t(j + 1) being there means that O_t holds every product up to tile j.
 
 constexpr int kTcTile = 128;
-constexpr int kTcThreads = 11 * 32;
+constexpr int kCopyWarps = 3;
+constexpr int kTcThreads = (8 + kCopyWarps + 1) * 32;
 enum TBar { tQFull = 0, tKFull = 1, tKEmpty = 3, tVFull = 5, tVEmpty = 7, tSFull = 9, tPReady = 11, tOFinal = 13,
             tDrain = 14, tBars = 15 };
 
@@ -533,20 +535,9 @@ __device__ __forceinline__ constexpr uint32_t idesc_of(int n, bool b_mn_major) {
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// four rows of a 2-D map (box [64, 1]) to four consecutive 128-byte rows of shared memory
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap *map, int32_t x, const int (&row)[4],
-                                            uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-      "%4, %5, %6}], [%7];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
-      : "memory");
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                             const __grid_constant__ CUtensorMap tm_v, const int pool_rows, const TreeParams p) {
+    tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const TreeParams p) {
   using S = TSmem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -573,11 +564,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const bool whole = tiles <= p.tiles_per_cta;
 
   if (threadIdx.x == 0) {
-    mbar_init(bar(tQFull), 3);  // the copy of Q, and the two warps that clear the rows it leaves
+    mbar_init(bar(tQFull), 1 + kCopyWarps);  // the copy of Q, and the warps that clear the rows it leaves
     for (int s = 0; s < 2; ++s) {
-      mbar_init(bar(tKFull + s), 2);
+      mbar_init(bar(tKFull + s), kCopyWarps * 32);
       mbar_init(bar(tKEmpty + s), 1);
-      mbar_init(bar(tVFull + s), 2);
+      mbar_init(bar(tVFull + s), kCopyWarps * 32);
       mbar_init(bar(tVEmpty + s), 1);
       mbar_init(bar(tSFull + s), 1);
       mbar_init(bar(tPReady + s), 4);
@@ -588,7 +579,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     *odd = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 10) {
+  if (warp == 8 + kCopyWarps) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
                  "r"(512u)
                  : "memory");
@@ -600,10 +591,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t tmem = *tmem_slot;
   constexpr int kChunks = D / 8;
 
-  if (warp == 8 || warp == 9) {
+  if (warp >= 8 && warp < 8 + kCopyWarps) {
     // ---- rows of the Q tiles that hold no node: zeros ----
-    const int me = (warp - 8) * 32 + lane, rest = kTcTile - filled;
-    for (int i = me; i < q_tiles * rest * kChunks; i += 64) {
+    const int me = warp - 8, rest = kTcTile - filled;
+    for (int i = me * 32 + lane; i < q_tiles * rest * kChunks; i += kCopyWarps * 32) {
       const int c = i % kChunks, r = filled + i / kChunks % rest, t = i / kChunks / rest;
       const uint32_t at = base + S::q + t * S::tile + uint32_t(c >> 3) * S::half + uint32_t(r) * 128u +
                           uint32_t(((c & 7) ^ (r & 7)) << 4);
@@ -613,24 +604,42 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(tQFull));
     // ---- K and V tiles ----
-    // pool rows of this lane's four keys of a tile, looked up a tile ahead; pool_rows (outside the map: zeros) where
-    // there is none
-    auto lookup = [&](int t, int(&row)[4]) {
+    // A pass of a warp copies kRowsPass rows, 16 bytes a lane; the warps take the passes in turn. The pool rows of a
+    // warp's 44 keys of a tile are held by its lanes, two each, looked up a tile ahead.
+    constexpr int kRowsPass = 32 / kChunks, kPasses = (kTcTile / kRowsPass + kCopyWarps - 1) / kCopyWarps;
+    static_assert(kPasses * kRowsPass <= 64, "two keys a lane");
+    const int c = lane % kChunks;
+    auto row_of = [&](int q) { return (kCopyWarps * (q / kRowsPass) + me) * kRowsPass + q % kRowsPass; };
+    int page[2], row[2];
+    auto fetch = [&](int t) {  // the table entries; checked when they are used, a tile later
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = t * kTcTile + lane * 4 + e;
-        row[e] = t < cached_tiles && key < rq.len ? pool_row(p.batch, b, key) : -1;
-        if (row[e] < 0) row[e] = pool_rows;
+      for (int e = 0; e < 2; ++e) {
+        const int q = e * 32 + lane, r = row_of(q), key = t * kTcTile + r;
+        const bool there = t < cached_tiles && q < kPasses * kRowsPass && r < kTcTile && key < rq.len;
+        page[e] = there ? __ldg(p.batch.tables + int64_t(b) * p.batch.table_width + page_index(p.batch, key)) : INT_MIN;
       }
     };
-    // 64 rows of a drafted tile, 16 bytes a lane and step
+    auto settle = [&](int t) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) row[e] = page[e] == INT_MIN ? -1 : row_in_page(p.batch, page[e], t * kTcTile + row_of(e * 32 + lane));
+    };
+    const uint32_t place0 = uint32_t(c >> 3) * S::half;
+    auto copy_cached = [&](const char *src, uint32_t dst) {
+      src += int64_t(kvh) * (D * 2) + c * 16;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int q = i * kRowsPass + lane / kChunks, r = row_of(q);
+        const int at = __shfl_sync(0xffffffffu, i * kRowsPass < 32 ? row[0] : row[1], q & 31);
+        if (r < kTcTile)
+          cp_async16(dst + place0 + uint32_t(r) * 128u + uint32_t(((c & 7) ^ (r & 7)) << 4),
+                     at < 0 ? src : src + int64_t(at) * p.pool_row, at < 0 ? 0 : 16);
+      }
+    };
     auto copy_draft = [&](const char *src, uint32_t dst, int j0, bool clean) {
-      for (int i = lane; i < 64 * kChunks; i += 32) {
-        const int r = (warp - 8) * 64 + i / kChunks, c = i % kChunks;
+      src += int64_t(kvh) * p.draft_head + c * 16;
+      for (int r = me * kRowsPass + lane / kChunks; r < kTcTile; r += kCopyWarps * kRowsPass) {
         uint4 x = make_uint4(0, 0, 0, 0);
-        if (j0 + r < drafted)
-          x = __ldg(reinterpret_cast<const uint4 *>(src + int64_t(rq.lo + j0 + r) * p.draft_token +
-                                                    int64_t(kvh) * p.draft_head + c * 16));
+        if (j0 + r < drafted) x = __ldg(reinterpret_cast<const uint4 *>(src + int64_t(rq.lo + j0 + r) * p.draft_token));
         if (clean) {
           constexpr uint32_t kExp = exponent_bits<T>();
           uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -645,45 +654,33 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           x = make_uint4(w[0], w[1], w[2], w[3]);
         }
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
-                         dst + uint32_t(c >> 3) * S::half + uint32_t(r) * 128u + uint32_t(((c & 7) ^ (r & 7)) << 4)),
+                         dst + place0 + uint32_t(r) * 128u + uint32_t(((c & 7) ^ (r & 7)) << 4)),
                      "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
                      : "memory");
       }
-      fence_async_smem();
     };
-    int row[4];
-    if (warp == 8) lookup(first, row);
-    bool ok = true;
-    for (int i = 0; i < n_tiles && ok; ++i) {
-      const int s = i & 1, t = first + i;
-      const uint32_t empty = ((i >> 1) & 1) ^ 1;
-      const bool draft = t >= cached_tiles;
-#pragma unroll
-      for (int kv = 0; kv < 2 && ok; ++kv) {
-        const uint32_t full = bar((kv ? tVFull : tKFull) + s), dst = base + (kv ? S::v : S::k) + s * S::tile;
-        ok = __all_sync(0xffffffffu, mbar_wait(bar((kv ? tVEmpty : tKEmpty) + s), empty, abort, p.batch.err));
-        if (!ok) break;
-        if (draft) {
-          copy_draft(kv ? p.v_draft : p.k_draft, dst, (t - cached_tiles) * kTcTile, kv);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full);
-        } else if (warp == 9) {
-          if (lane == 0) mbar_arrive(full);
-        } else {
-          if (lane == 0) mbar_expect_tx(full, S::tile);
-          __syncwarp();
-          for (int h = 0; h < D / 64; ++h)
-            tma_gather4(dst + h * S::half + lane * 512, kv ? &tm_v : &tm_k, kvh * D + h * 64, row, full);
-        }
+    // K 0, V 0, K 1, V 1, ...: a slot's barrier counts a thread when its copies have landed, nobody waits for them here
+    fetch(first);
+    for (int n = 0; n < 2 * n_tiles; ++n) {
+      const int i = n >> 1, s = i & 1, t = first + i;
+      const bool v = n & 1;
+      if (!v) {
+        settle(t);
+        fetch(t + 1);
       }
-      if (warp == 8 && ok) lookup(t + 1, row);
-    }
-    if (!ok) {  // a wait gave up: time for the copies in flight before the shared memory is given back
-      const uint64_t since = globaltimer();
-      while (globaltimer() - since < 200000ull) {
+      const bool ok = mbar_wait(bar((v ? tVEmpty : tKEmpty) + s), ((i >> 1) & 1) ^ 1, abort, p.batch.err);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const uint32_t dst = base + (v ? S::v : S::k) + s * S::tile, full = bar((v ? tVFull : tKFull) + s);
+      if (t >= cached_tiles) {
+        copy_draft(v ? p.v_draft : p.k_draft, dst, (t - cached_tiles) * kTcTile, v);
+        mbar_arrive(full);
+      } else {
+        copy_cached(v ? p.v_pool : p.k_pool, dst);
+        cp_async_arrive(full);
       }
     }
-  } else if (warp == 10) {
+    cp_async_wait<0>();
+  } else if (warp == 8 + kCopyWarps) {
     if (lane == 0) {
       // ---- Q, and the products ----
       mbar_expect_tx(bar(tQFull), uint32_t(q_tiles) * uint32_t(filled) * (D * 2));
@@ -710,6 +707,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (ok && n_tiles > 0) {
         ok = mbar_wait(bar(tKFull), 0, abort, p.batch.err);
         if (ok) {
+          fence_async_smem();  // the copying threads' writes, which the barrier showed, before the products' reads
           tc_fence_after();
           for (int t = 0; t < q_tiles; ++t) {
             qk(t, 0);
@@ -720,6 +718,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int i = 0; i < n_tiles && ok; ++i) {
           const int s = i & 1, s1 = s ^ 1;
           ok = mbar_wait(bar(tVFull + s), (i >> 1) & 1, abort, p.batch.err);
+          fence_async_smem();
           for (int t = 0; t < q_tiles && ok; ++t) {
             ok = mbar_wait(bar(tPReady + t), i & 1, abort, p.batch.err);
             if (!ok) break;
@@ -729,6 +728,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               if (t == 0) {
                 ok = mbar_wait(bar(tKFull + s1), ((i + 1) >> 1) & 1, abort, p.batch.err);
                 if (!ok) break;
+                fence_async_smem();
                 tc_fence_after();
               }
               qk(t, s1);
@@ -914,7 +914,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 10) {
+  if (warp == 8 + kCopyWarps) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
@@ -1028,25 +1028,17 @@ int launch(dim3 grid, int threads, int smem, cudaStream_t stream, const char *wh
 }
 
 template <typename T, int D>
-int run_tree(const TreeParams &p, const TreePlan &t, const qe_draft_batch &in, int64_t pool_rows, cudaStream_t stream) {
+int run_tree(const TreeParams &p, const TreePlan &t, const qe_draft_batch &in, cudaStream_t stream) {
   const dim3 grid(unsigned(t.splits), unsigned(t.row_ctas), unsigned(in.batch));
   int s;
   if (t.tc) {
     const CUtensorMapDataType type = exponent_bits<T>() == 0x7f80u ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    CUtensorMap q, kv[2];
-    std::memset(kv, 0, sizeof(kv));
+    CUtensorMap q;
     const uint64_t q_dims[3] = {uint64_t(D), uint64_t(p.heads_q), uint64_t(in.total)};
     const uint64_t q_strides[2] = {uint64_t(p.q_head), uint64_t(p.q_token)};
     const uint32_t q_box[3] = {64, uint32_t(p.group), uint32_t(kTcTile / p.group)};
     if ((s = tensor_map_16bit("qe_tree_attention", &q, type, p.q, 3, q_dims, q_strides, q_box, "q"))) return s;
-    if (p.batch.table_width > 0 && in.max_length > 0) {
-      const uint64_t dims[2] = {uint64_t(p.heads_kv) * D, uint64_t(pool_rows)}, strides[1] = {uint64_t(p.pool_row)};
-      const uint32_t box[2] = {64, 1};
-      if ((s = tensor_map_16bit("qe_tree_attention", &kv[0], type, p.k_pool, 2, dims, strides, box, "the K plane"))) return s;
-      if ((s = tensor_map_16bit("qe_tree_attention", &kv[1], type, p.v_pool, 2, dims, strides, box, "the V plane"))) return s;
-    }
-    s = launch<tree_attention_tc_kernel<T, D>>(grid, kTcThreads, TSmem<D>::bytes, stream, "qe_tree_attention launch", q, kv[0],
-                                               kv[1], int(pool_rows), p);
+    s = launch<tree_attention_tc_kernel<T, D>>(grid, kTcThreads, TSmem<D>::bytes, stream, "qe_tree_attention launch", q, p);
   } else if (t.m_tiles == 1) {
     s = launch<tree_attention_kernel<T, D, 1>>(grid, kWarps * 32, tree_smem_bytes<D, 1>(), stream, "qe_tree_attention launch", p);
   } else {
@@ -1142,10 +1134,10 @@ extern "C" int qe_tree_attention(qe_draft_batch batch, const void *q, int64_t q_
   p.part_ml = reinterpret_cast<float2 *>(p.part_o + int64_t(t.splits) * batch.total * heads_q * head_dim);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == 1)
-    s = head_dim == 128 ? run_tree<__nv_bfloat16, 128>(p, t, batch, pool_rows, st)
-                        : run_tree<__nv_bfloat16, 64>(p, t, batch, pool_rows, st);
+    s = head_dim == 128 ? run_tree<__nv_bfloat16, 128>(p, t, batch, st)
+                        : run_tree<__nv_bfloat16, 64>(p, t, batch, st);
   else
-    s = head_dim == 128 ? run_tree<__half, 128>(p, t, batch, pool_rows, st)
-                        : run_tree<__half, 64>(p, t, batch, pool_rows, st);
+    s = head_dim == 128 ? run_tree<__half, 128>(p, t, batch, st)
+                        : run_tree<__half, 64>(p, t, batch, st);
   return s ? s : ok();
 }
