@@ -346,11 +346,6 @@ typedef struct qe_draft_batch {
 int qe_tree_masks(const int32_t *parents, const int32_t *starts, int32_t batch, int32_t total, int32_t max_nodes,
                   int32_t mask_words, int32_t *masks, int32_t *err_flag, void *stream);
 
-/* Bytes of device workspace that qe_tree_attention needs for this batch on the current device (0: none); 16-byte
- * aligned. It is scratch of one call: calls that may overlap need one each. */
-int qe_tree_attention_workspace(qe_draft_batch batch, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
-                                int64_t *bytes);
-
 /* Attention of a batch's drafted tokens over [the request's cached tokens; the drafted ones they see]:
  *   out[i][h] = sum_j softmax_j(scale q[i][h] . K[j][h / G]) V[j][h / G],   G = heads_q / heads_kv
  * and, optionally, lse[h][i] (fp32, [heads_q][total]), the natural log of the softmax's denominator.
@@ -361,12 +356,29 @@ int qe_tree_attention_workspace(qe_draft_batch batch, int32_t heads_q, int32_t h
  *        not read and their rows of out and lse are left as they were.
  * Everything 16-byte aligned with strides that are multiples of 16 bytes. A hidden key contributes nothing, whatever
  * its K and V hold (NaN and infinities too). Results do not depend on the run. */
-int qe_tree_attention(qe_draft_batch batch, const void *q, int64_t q_token_stride, int64_t q_head_stride,
-                      int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t dtype, const void *k_pool,
-                      const void *v_pool, int64_t pool_rows, const void *k_draft, const void *v_draft,
-                      int64_t draft_token_stride, int64_t draft_head_stride, float scale, void *out,
-                      int64_t out_token_stride, int64_t out_head_stride, float *lse, void *workspace,
-                      int64_t workspace_bytes, int32_t *err_flag, void *stream);
+typedef struct qe_tree_attention_args {
+  qe_draft_batch batch;
+  const void *q;
+  int64_t q_token_stride, q_head_stride;
+  const void *k_pool, *v_pool;
+  int64_t pool_rows;
+  const void *k_draft, *v_draft;
+  int64_t draft_token_stride, draft_head_stride;
+  void *out;
+  int64_t out_token_stride, out_head_stride;
+  float *lse;
+  void *workspace;
+  int64_t workspace_bytes;
+  int32_t *err_flag;
+  int32_t heads_q, heads_kv, head_dim, dtype;
+  float scale;
+} qe_tree_attention_args;
+
+/* Bytes of device workspace that qe_tree_attention needs for this batch and these heads on the current device (0:
+ * none; the pointers of `args` are not looked at); 16-byte aligned. It is scratch of one call: calls that may overlap
+ * need one each. */
+int qe_tree_attention_workspace(const qe_tree_attention_args *args, int64_t *bytes);
+int qe_tree_attention(const qe_tree_attention_args *args, void *stream);
 
 /* The attention weight of every key, from the queries' lse (what qe_tree_attention and qe_paged_attention return):
  *   w[b][g][j] (+)= sum over request b's nodes i that see j and the G query heads h of K/V head g of
@@ -377,12 +389,23 @@ int qe_tree_attention(qe_draft_batch batch, const void *q, int64_t q_token_strid
  * (k_draft ? max_nodes : 0). lse [heads_q] rows, lse_head_stride elements apart. A query whose lse is -inf (it saw
  * nothing) or +inf (taken out by the caller) counts nothing. Sums are fp32, in an order that does not depend on the
  * run. Other arguments as qe_tree_attention's. */
-int qe_attention_weights(qe_draft_batch batch, const void *q, int64_t q_token_stride, int64_t q_head_stride,
-                         int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t dtype, const void *k_pool,
-                         int64_t pool_rows, const void *k_draft, int64_t draft_token_stride, int64_t draft_head_stride,
-                         const float *lse, int64_t lse_head_stride, float scale, int32_t accumulate, float *weights,
-                         int64_t weights_batch_stride, int64_t weights_head_stride, int64_t width, int32_t *err_flag,
-                         void *stream);
+typedef struct qe_attention_weights_args {
+  qe_draft_batch batch;
+  const void *q;
+  int64_t q_token_stride, q_head_stride;
+  const void *k_pool;
+  int64_t pool_rows;
+  const void *k_draft;
+  int64_t draft_token_stride, draft_head_stride;
+  const float *lse;
+  int64_t lse_head_stride;
+  float *weights;
+  int64_t weights_batch_stride, weights_head_stride, width;
+  int32_t *err_flag;
+  int32_t heads_q, heads_kv, head_dim, dtype, accumulate;
+  float scale;
+} qe_attention_weights_args;
+int qe_attention_weights(const qe_attention_weights_args *args, void *stream);
 
 /* Per row the positions a cache of `budget` tokens keeps, in rising order: the first `sinks`, the last `recent`, and
  * of the others the heaviest (of equal weights the lowest position first; a NaN counts as -inf).
@@ -399,11 +422,12 @@ int qe_heaviest(const float *weights, int64_t n0, int64_t n1, int64_t n2, int64_
 /* Moves kept tokens inside a pool, each K/V head its own: for every layer l, K and V, head h and i < n_keep with
  * p = keep[l][h][i] >= 0:  row dst_slots[i] of the plane, head h = row src_slots[p], head h. keep: int32
  * [layers][heads][n_keep], contiguous; a negative entry leaves its place as it was; one past n_src, or a slot
- * outside the pool, is skipped and sets bit 1 of *err_flag. The source and destination slots must not overlap.
+ * outside the pool, is skipped and sets bit 1 of *err_flag. src_host / dst_host: the same slots in host memory; no
+ * destination slot may be there twice or among the sources (QE_ERR_INVALID).
  * pool: plane 2 l + c is layer l's K (c = 0) or V plane; rows of heads x head_bytes; everything 16-byte aligned. */
 int qe_retain(qe_planes pool, int64_t pool_rows, int32_t layers, int32_t heads, int64_t head_bytes,
-              const int64_t *src_slots, int64_t n_src, const int32_t *keep, int64_t n_keep, const int64_t *dst_slots,
-              int32_t *err_flag, void *stream);
+              const int64_t *src_slots, const int64_t *src_host, int64_t n_src, const int32_t *keep, int64_t n_keep,
+              const int64_t *dst_slots, const int64_t *dst_host, int32_t *err_flag, void *stream);
 
 /* ---- prefix index: radix tree + slot allocator + LRU eviction (host) -------------------------
  *

@@ -7,6 +7,7 @@ The library is the only implementation of the path: if it is missing this module
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_uint8, c_uint64, c_void_p
 from pathlib import Path
@@ -31,13 +32,11 @@ class Planes(ctypes.Structure):
                 ("planes_inner", c_int32), ("_pad", c_int32)]
 
 
-class DraftBatch(ctypes.Structure):
-    """``qe_draft_batch``: the cached and drafted tokens of a batch of requests."""
-
-    _fields_ = [("starts", c_void_p), ("lengths", c_void_p), ("tables", c_void_p), ("masks", c_void_p),
-                ("batch", c_int32), ("table_width", c_int32), ("page_size", c_int32), ("mask_words", c_int32),
-                ("mode", c_int32), ("total", c_int32), ("max_nodes", c_int32), ("max_length", c_int32),
-                ("sum_length", c_int64)]
+# Argument structs of the decoding operators, packed by ``struct`` in one go (a call passes their bytes):
+# qe_draft_batch, and what follows it in qe_tree_attention_args and qe_attention_weights_args.
+DRAFT_BATCH = struct.Struct("@4P8iq")
+TREE_ATTENTION = struct.Struct("@PqqPPqPPqqPqqPPqP4if0q")
+ATTENTION_WEIGHTS = struct.Struct("@PqqPqPqqPqPqqqP5if0q")
 
 
 _P64 = POINTER(c_int64)
@@ -84,17 +83,13 @@ SIGNATURES: dict[str, list] = {
                                   c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                   c_void_p],
     "qe_tree_masks": [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p],
-    "qe_tree_attention_workspace": [DraftBatch, c_int32, c_int32, c_int32, _P64],
-    "qe_tree_attention": [DraftBatch, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p,
-                          c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_float, c_void_p, c_int64,
-                          c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
-    "qe_attention_weights": [DraftBatch, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p,
-                             c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_float, c_int32, c_void_p,
-                             c_int64, c_int64, c_int64, c_void_p, c_void_p],
+    "qe_tree_attention_workspace": [c_char_p, _P64],
+    "qe_tree_attention": [c_char_p, c_void_p],
+    "qe_attention_weights": [c_char_p, c_void_p],
     "qe_heaviest": [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64,
                     c_int64, c_int64, c_void_p, c_void_p, c_void_p],
-    "qe_retain": [Planes, c_int64, c_int32, c_int32, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-                  c_void_p, c_void_p],
+    "qe_retain": [Planes, c_int64, c_int32, c_int32, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                  c_void_p, c_void_p, c_void_p, c_void_p],
     "qe_norm_scale_amax": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                            c_int64, c_int64, c_int64, c_int64, c_float, c_void_p, c_void_p],
     "qe_silu_mul_amax": [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p],
@@ -202,5 +197,5 @@ def ptr64(array) -> "ctypes._Pointer":
     return array.ctypes.data_as(_P64)
 
 
-__all__ = ["LIB_PATH", "QEError", "DraftBatch", "Planes", "SIGNATURES", "call", "lib", "on_device", "planes", "ptr64",
+__all__ = ["LIB_PATH", "ATTENTION_WEIGHTS", "DRAFT_BATCH", "QEError", "Planes", "SIGNATURES", "TREE_ATTENTION", "call", "lib", "on_device", "planes", "ptr64",
            "stream_of", "version", "c_uint8"]

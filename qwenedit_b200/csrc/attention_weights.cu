@@ -556,14 +556,12 @@ bool al16(int64_t v) { return v % 16 == 0; }
 }  // namespace
 }  // namespace qe
 
-extern "C" int qe_attention_weights(qe_draft_batch batch, const void *q, int64_t q_token_stride, int64_t q_head_stride,
-                                    int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t dtype,
-                                    const void *k_pool, int64_t pool_rows, const void *k_draft,
-                                    int64_t draft_token_stride, int64_t draft_head_stride, const float *lse,
-                                    int64_t lse_head_stride, float scale, int32_t accumulate, float *weights,
-                                    int64_t weights_batch_stride, int64_t weights_head_stride, int64_t width,
-                                    int32_t *err_flag, void *stream) {
+extern "C" int qe_attention_weights(const qe_attention_weights_args *args, void *stream) {
   using namespace qe;
+  QE_CHECK_ARG(args, "qe_attention_weights: null arguments");
+  const auto &[batch, q, q_token_stride, q_head_stride, k_pool, pool_rows, k_draft, draft_token_stride,
+               draft_head_stride, lse, lse_head_stride, weights, weights_batch_stride, weights_head_stride, width,
+               err_flag, heads_q, heads_kv, head_dim, dtype, accumulate, scale] = *args;
   WeightParams p{};
   int s = decode_batch("qe_attention_weights", batch, heads_q, heads_kv, head_dim, dtype, pool_rows, k_pool != nullptr,
                        err_flag, &p.batch);

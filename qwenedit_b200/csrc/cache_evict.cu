@@ -2,6 +2,8 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <new>
+#include <vector>
 
 #include "qe_decode.cuh"
 
@@ -225,18 +227,34 @@ extern "C" int qe_heaviest(const float *weights, int64_t n0, int64_t n1, int64_t
 }
 
 extern "C" int qe_retain(qe_planes pool, int64_t pool_rows, int32_t layers, int32_t heads, int64_t head_bytes,
-                         const int64_t *src_slots, int64_t n_src, const int32_t *keep, int64_t n_keep,
-                         const int64_t *dst_slots, int32_t *err_flag, void *stream) {
+                         const int64_t *src_slots, const int64_t *src_host, int64_t n_src, const int32_t *keep,
+                         int64_t n_keep, const int64_t *dst_slots, const int64_t *dst_host, int32_t *err_flag,
+                         void *stream) {
   using namespace qe;
   QE_CHECK_ARG(layers >= 0 && heads >= 1 && n_src >= 0 && n_keep >= 0 && pool_rows >= 0 &&
                    pool_rows < (int64_t(1) << 31),
                "qe_retain: bad size");
   QE_CHECK_ARG(head_bytes >= 16 && head_bytes % 16 == 0, "qe_retain: head_bytes must be a multiple of 16");
   if (layers == 0 || n_keep == 0) return ok();
-  QE_CHECK_ARG(pool.base && keep && dst_slots && (src_slots || n_src == 0), "qe_retain: null pointer");
+  QE_CHECK_ARG(pool.base && keep && dst_slots && dst_host && ((src_slots && src_host) || n_src == 0),
+               "qe_retain: null pointer");
   QE_CHECK_ARG(pool.planes_inner == 2 && aligned16(pool.base) && pool.outer_stride % 16 == 0 &&
                    pool.inner_stride % 16 == 0,
                "qe_retain: pool planes must be 16-byte aligned [layers, 2]");
+  try {
+    std::vector<uint8_t> taken(static_cast<size_t>(pool_rows), 0);
+    for (int64_t i = 0; i < n_src; ++i) {
+      QE_CHECK_ARG(src_host[i] >= 0 && src_host[i] < pool_rows, "qe_retain: source slots outside the pool");
+      taken[size_t(src_host[i])] = 1;
+    }
+    for (int64_t i = 0; i < n_keep; ++i) {
+      QE_CHECK_ARG(dst_host[i] >= 0 && dst_host[i] < pool_rows, "qe_retain: destination slots outside the pool");
+      QE_CHECK_ARG(!taken[size_t(dst_host[i])], "qe_retain: a destination slot twice, or among the sources");
+      taken[size_t(dst_host[i])] = 1;
+    }
+  } catch (const std::bad_alloc &) {
+    return fail(QE_ERR_NOMEM, "qe_retain: out of host memory");
+  }
   RetainParams p{};
   p.base = static_cast<char *>(pool.base);
   p.outer = pool.outer_stride;

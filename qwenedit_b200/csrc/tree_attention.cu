@@ -920,7 +920,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 }
 
-// Joins the splits of the requests that have more than one: a warp per (node, head) row.
+// Joins the splits of the requests that have more than one: a warp per (node, head) row. The lanes hold the splits'
+// factors, 32 at a time; the partial rows are read eight at a time (one after the other, 37 splits took 9 us).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
   const int lane = threadIdx.x & 31;
@@ -935,24 +936,42 @@ __global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
   const int splits = min((tiles + p.tiles_per_cta - 1) / p.tiles_per_cta, p.splits);
   const int token = rq.lo + at / p.heads_q, head = at % p.heads_q;
   const int64_t row = int64_t(token) * p.heads_q + head, step = int64_t(p.batch.total) * p.heads_q;
-  float m_all = -INFINITY;
-  for (int s = lane; s < splits; s += 32) m_all = fmaxf(m_all, p.part_ml[s * step + row].x);
+  const float2 none = make_float2(-INFINITY, 0.0f);
+  float2 ml = lane < splits ? p.part_ml[lane * step + row] : none;
+  float m_all = ml.x;
+  for (int s = 32 + lane; s < splits; s += 32) m_all = fmaxf(m_all, p.part_ml[s * step + row].x);
 #pragma unroll
   for (int x = 16; x; x >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, x));
   constexpr int kPer = D / 32;  // columns per lane
   float acc[kPer] = {}, l_all = 0.0f;
-  for (int s = 0; s < splits; ++s) {
-    const float2 ml = p.part_ml[s * step + row];
-    const float f = join_factor(ml.x, m_all);
+  for (int s0 = 0; s0 < splits; s0 += 32) {
+    if (s0 > 0) ml = s0 + lane < splits ? p.part_ml[(s0 + lane) * step + row] : none;
+    const float f = s0 + lane < splits ? join_factor(ml.x, m_all) : 0.0f;
     l_all += f * ml.y;
-    const float *src = p.part_o + (s * step + row) * D + lane * kPer;
+    const int here = min(splits - s0, 32);
+    for (int u0 = 0; u0 < here; u0 += 8) {
+      float2 v[8][kPer / 2];
 #pragma unroll
-    for (int e = 0; e < kPer; e += 2) {
-      const float2 v = *reinterpret_cast<const float2 *>(src + e);
-      acc[e] += f * v.x;
-      acc[e + 1] += f * v.y;
+      for (int u = 0; u < 8; ++u) {
+        const float *src = p.part_o + ((s0 + min(u0 + u, here - 1)) * step + row) * D + lane * kPer;
+#pragma unroll
+        for (int e = 0; e < kPer / 2; ++e) v[u][e] = *reinterpret_cast<const float2 *>(src + 2 * e);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float fu = __shfl_sync(0xffffffffu, f, (u0 + u) & 31);
+        if (u0 + u < here) {
+#pragma unroll
+          for (int e = 0; e < kPer / 2; ++e) {
+            acc[2 * e] += fu * v[u][e].x;
+            acc[2 * e + 1] += fu * v[u][e].y;
+          }
+        }
+      }
     }
   }
+#pragma unroll
+  for (int x = 16; x; x >>= 1) l_all += __shfl_xor_sync(0xffffffffu, l_all, x);
   const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
   uint32_t *dst = reinterpret_cast<uint32_t *>(p.out + int64_t(token) * p.out_token + int64_t(head) * p.out_head) +
                   lane * (kPer / 2);
@@ -990,12 +1009,24 @@ TreePlan tree_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head
   const int64_t per_cta = t.tc ? int64_t(2 * (kTcTile / group)) * group : t.m_tiles * 16;  // rows
   t.row_ctas = int(std::min<int64_t>(std::max<int64_t>(1, (rows + per_cta - 1) / per_cta) * heads_kv, 1 << 30));
   const int64_t max_tiles = std::max(1, tiles_of(in.max_length, in.max_nodes, t.key_tile));
-  // tiles of the whole batch, spread over the CTAs that the SMs hold: two, or one with all of the tensor memory
+  // Tiles a CTA: of the whole batch's tiles, over the CTAs that the SMs hold (two, or one with all of the tensor
+  // memory), the count that ends first. The model: waves x (tiles + `fixed`, what a CTA's start and end cost in tiles),
+  // half a CTA more per request for the last, shorter one. One wave for all took 64 requests of 313 to 8,191 tokens
+  // from N to M us.
   const int64_t all = (in.sum_length + t.key_tile - 1) / t.key_tile + int64_t(in.batch) * tiles_of(0, in.max_nodes, t.key_tile);
-  const int64_t ctas = (t.tc ? 1 : 2) * sm_count(), step = t.tc ? 1 : kWarps;
-  int64_t per = (all * t.row_ctas + ctas - 1) / ctas;
-  per = std::max<int64_t>((per + step - 1) / step * step, step);
-  if (per >= max_tiles) per = max_tiles;
+  const int64_t slots = (t.tc ? 1 : 2) * sm_count(), step = t.tc ? 1 : kWarps, fixed = t.tc ? 4 : 8;
+  const int64_t ragged = in.batch > 1 ? in.batch / 2 : 0;
+  int64_t per = max_tiles, best = INT64_MAX;
+  for (int64_t x = step;; x = std::max(x + step, x * 9 / 8 / step * step)) {
+    x = std::min(x, max_tiles);
+    const int64_t ctas = t.row_ctas * ((all + x - 1) / x + (x < max_tiles ? ragged : 0));
+    const int64_t cost = (ctas + slots - 1) / slots * (x + fixed);
+    if (cost < best) {
+      best = cost;
+      per = x;
+    }
+    if (x == max_tiles) break;
+  }
   t.tiles_per_cta = int(per);
   t.splits = int((max_tiles + per - 1) / per);
   if (t.splits > 1) t.workspace = int64_t(t.splits) * in.total * heads_q * (head_dim + 2) * 4;
@@ -1068,25 +1099,24 @@ extern "C" int qe_tree_masks(const int32_t *parents, const int32_t *starts, int3
   return s ? s : ok();
 }
 
-extern "C" int qe_tree_attention_workspace(qe_draft_batch batch, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
-                                           int64_t *bytes) {
+extern "C" int qe_tree_attention_workspace(const qe_tree_attention_args *args, int64_t *bytes) {
   using namespace qe;
-  QE_CHECK_ARG(bytes, "qe_tree_attention_workspace: null pointer");
+  QE_CHECK_ARG(args && bytes, "qe_tree_attention_workspace: null pointer");
+  const qe_draft_batch &batch = args->batch;
   QE_CHECK_ARG(batch.batch >= 0 && batch.total >= 0 && batch.max_nodes >= 0 && batch.max_length >= 0 &&
-                   batch.sum_length >= 0 && heads_q >= 1 && heads_kv >= 1 && heads_q % heads_kv == 0 &&
-                   (head_dim == 64 || head_dim == 128),
+                   batch.sum_length >= 0 && args->heads_q >= 1 && args->heads_kv >= 1 &&
+                   args->heads_q % args->heads_kv == 0 && (args->head_dim == 64 || args->head_dim == 128),
                "qe_tree_attention_workspace: bad size");
-  *bytes = tree_plan(batch, heads_q, heads_kv, head_dim).workspace;
+  *bytes = tree_plan(batch, args->heads_q, args->heads_kv, args->head_dim).workspace;
   return ok();
 }
 
-extern "C" int qe_tree_attention(qe_draft_batch batch, const void *q, int64_t q_token_stride, int64_t q_head_stride,
-                                 int32_t heads_q, int32_t heads_kv, int32_t head_dim, int32_t dtype,
-                                 const void *k_pool, const void *v_pool, int64_t pool_rows, const void *k_draft,
-                                 const void *v_draft, int64_t draft_token_stride, int64_t draft_head_stride,
-                                 float scale, void *out, int64_t out_token_stride, int64_t out_head_stride, float *lse,
-                                 void *workspace, int64_t workspace_bytes, int32_t *err_flag, void *stream) {
+extern "C" int qe_tree_attention(const qe_tree_attention_args *args, void *stream) {
   using namespace qe;
+  QE_CHECK_ARG(args, "qe_tree_attention: null arguments");
+  const auto &[batch, q, q_token_stride, q_head_stride, k_pool, v_pool, pool_rows, k_draft, v_draft, draft_token_stride,
+               draft_head_stride, out, out_token_stride, out_head_stride, lse, workspace, workspace_bytes, err_flag,
+               heads_q, heads_kv, head_dim, dtype, scale] = *args;
   TreeParams p{};
   QE_CHECK_ARG((k_pool == nullptr) == (v_pool == nullptr) && (k_draft == nullptr) == (v_draft == nullptr),
                "qe_tree_attention: K and V go together");

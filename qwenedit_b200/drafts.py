@@ -164,12 +164,22 @@ class DraftTree:
 
 
 class _View:
-    """The C view of a cache and a tree, and the workspace sizes asked of it."""
+    """The C view of a cache and a tree (``qe_draft_batch`` as bytes), the workspace sizes asked of it, and the tensor
+    layouts that its calls have checked."""
 
-    __slots__ = ("cache", "batch", "workspace")
+    __slots__ = ("cache", "batch", "workspace", "checked")
 
     def __init__(self, cache, batch):
-        self.cache, self.batch, self.workspace = cache, batch, {}
+        self.cache, self.batch, self.workspace, self.checked = cache, batch, {}, {}
+
+    def check(self, name: str, t: torch.Tensor, n: int, heads: int, head_dim: int, dtype, device) -> tuple:
+        """The strides of a [tokens, heads, head_dim] tensor, after checks that equal layouts pass without repeating."""
+        stride = t.stride()
+        layout = (t.shape, stride, t.dtype, t.device, heads)
+        if self.checked.get(name) != layout:
+            _check_rows(name, t, n, heads, head_dim, dtype, device)
+            self.checked[name] = layout
+        return stride
 
 
 def _view(cache: PagedBatch, tree: DraftTree) -> _View:
@@ -181,10 +191,10 @@ def _view(cache: PagedBatch, tree: DraftTree) -> _View:
         raise ValueError(f"the cache holds {cache.batch} requests, the tree {tree.batch}")
     if cache.pool.device != tree.device:
         raise ValueError(f"the cache is on {cache.pool.device}, the tree on {tree.device}")
-    batch = _lib.DraftBatch(tree.starts.data_ptr(), cache.lengths.data_ptr(), cache.tables.data_ptr(),
-                            None if tree.masks is None else tree.masks.data_ptr(), cache.batch, cache.table_width,
-                            cache.pool.page_size, tree.words, tree.mode, tree.total, tree.max_nodes,
-                            cache.max_length, cache.sum_length)
+    batch = _lib.DRAFT_BATCH.pack(tree.starts.data_ptr(), cache.lengths.data_ptr(), cache.tables.data_ptr(),
+                                  0 if tree.masks is None else tree.masks.data_ptr(), cache.batch, cache.table_width,
+                                  cache.pool.page_size, tree.words, tree.mode, tree.total, tree.max_nodes,
+                                  cache.max_length, cache.sum_length)
     tree._view = _View(cache, batch)
     return tree._view
 
@@ -220,45 +230,43 @@ def tree_attention(q: torch.Tensor, cache: PagedBatch, tree: DraftTree, layer: i
     ``evict.attention_weights`` takes. A token that sees nothing gets zeros and -inf; rows of `out` past the tree's
     are left as they were (zeros where the call makes `out`). Runs on the current stream, without synchronising."""
     pool = _check_pool(cache, layer)
-    device, dtype, heads_kv, d = pool.device, pool.kv.dtype, pool.heads, pool.head_dim
+    kv, device, heads_kv, d = pool.kv, pool.device, pool.heads, pool.head_dim
+    dtype = kv.dtype
     if q.dim() != 3 or q.shape[1] % heads_kv or q.shape[1] == 0:
         raise ValueError(f"q must be [tokens, heads, {d}], its heads a multiple of the pool's {heads_kv}")
-    total, heads_q = tree.total, q.shape[1]
-    _check_rows("q", q, total, heads_q, d, dtype, device)
     if (k_draft is None) != (v_draft is None):
         raise ValueError("k_draft and v_draft go together")
+    view, total, heads_q = _view(cache, tree), tree.total, q.shape[1]
+    qs = view.check("q", q, total, heads_q, d, dtype, device)
+    draft = (0, 0, 0, 0)
     if k_draft is not None:
-        _check_rows("k_draft", k_draft, total, heads_kv, d, dtype, device)
-        _check_rows("v_draft", v_draft, total, heads_kv, d, dtype, device)
-        if k_draft.stride() != v_draft.stride():
+        ks = view.check("k_draft", k_draft, total, heads_kv, d, dtype, device)
+        if view.check("v_draft", v_draft, total, heads_kv, d, dtype, device) != ks:
             raise ValueError("k_draft and v_draft must have the same strides")
-    view = _view(cache, tree)
+        draft = (k_draft.data_ptr(), v_draft.data_ptr(), 2 * ks[0], 2 * ks[1])
     if out is None:
         make = torch.empty if q.shape[0] == total else torch.zeros
         out = make(q.shape, dtype=dtype, device=device)
-    else:
-        _check_rows("out", out, total, heads_q, d, dtype, device)
-    lse = torch.empty(heads_q, total, dtype=torch.float32, device=device) if return_lse else None
-    kv, e = pool.kv, 2
+    os = view.check("out", out, total, heads_q, d, dtype, device)
+    lse = torch.empty((heads_q, total), dtype=torch.float32, device=device) if return_lse else None
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    plane = kv.data_ptr() + 2 * layer * kv.stride(0)
     with _lib.on_device(device):
-        size = _workspace_bytes(view, heads_q, heads_kv, d)
+        size = view.workspace.get((heads_q, heads_kv, d))
+        if size is None:
+            size = view.workspace[heads_q, heads_kv, d] = _workspace_bytes(view, heads_q, heads_kv, d)
         work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        plane = kv.data_ptr() + layer * kv.stride(0) * e
-        _lib.call("qe_tree_attention", view.batch, q.data_ptr(), q.stride(0) * e, q.stride(1) * e, heads_q, heads_kv, d,
-                  DTYPES[dtype], plane, plane + kv.stride(1) * e, pool.rows,
-                  None if k_draft is None else k_draft.data_ptr(), None if v_draft is None else v_draft.data_ptr(),
-                  0 if k_draft is None else k_draft.stride(0) * e, 0 if k_draft is None else k_draft.stride(1) * e,
-                  1.0 / math.sqrt(d) if scale is None else float(scale), out.data_ptr(), out.stride(0) * e,
-                  out.stride(1) * e, None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(),
-                  size, pool._err.data_ptr(), _lib.stream_of(device))
+        args = view.batch + _lib.TREE_ATTENTION.pack(
+            q.data_ptr(), 2 * qs[0], 2 * qs[1], plane, plane + 2 * kv.stride(1), pool.rows, *draft, out.data_ptr(),
+            2 * os[0], 2 * os[1], 0 if lse is None else lse.data_ptr(), 0 if work is None else work.data_ptr(), size,
+            pool._err.data_ptr(), heads_q, heads_kv, d, DTYPES[dtype], scale)
+        _lib.call("qe_tree_attention", args, _lib.stream_of(device))
     return (out, lse) if return_lse else out
 
 
 def _workspace_bytes(view: _View, heads_q: int, heads_kv: int, d: int) -> int:
-    key = (heads_q, heads_kv, d)
-    size = view.workspace.get(key)
-    if size is None:
-        out = ctypes.c_int64()
-        _lib.call("qe_tree_attention_workspace", view.batch, heads_q, heads_kv, d, ctypes.byref(out))
-        size = view.workspace[key] = out.value
-    return size
+    out = ctypes.c_int64()
+    args = view.batch + _lib.TREE_ATTENTION.pack(*[0] * 17, heads_q, heads_kv, d, 1, 1.0)
+    _lib.call("qe_tree_attention_workspace", args, ctypes.byref(out))
+    return out.value

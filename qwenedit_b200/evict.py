@@ -19,7 +19,7 @@ import math
 import torch
 
 from qwenedit_b200 import _lib
-from qwenedit_b200.drafts import DTYPES, DraftTree, PagedBatch, _check_pool, _check_rows, _view
+from qwenedit_b200.drafts import DTYPES, DraftTree, PagedBatch, _check_pool, _view
 
 
 def attention_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedBatch, tree: DraftTree, layer: int = 0,
@@ -37,36 +37,43 @@ def attention_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedBatch, tre
     tree's largest count. With `accumulate` the weights are added to what `out` holds (positions past a request's
     keys stay); else those positions get 0. The same inputs give the same bits. One launch on the current stream."""
     pool = _check_pool(cache, layer)
-    device, dtype, heads_kv, d = pool.device, pool.kv.dtype, pool.heads, pool.head_dim
+    kv, device, heads_kv, d = pool.kv, pool.device, pool.heads, pool.head_dim
+    dtype = kv.dtype
     if q.dim() != 3 or q.shape[1] % heads_kv or q.shape[1] == 0:
         raise ValueError(f"q must be [tokens, heads, {d}], its heads a multiple of the pool's {heads_kv}")
-    total, heads_q = tree.total, q.shape[1]
-    _check_rows("q", q, total, heads_q, d, dtype, device)
+    view, total, heads_q = _view(cache, tree), tree.total, q.shape[1]
+    qs = view.check("q", q, total, heads_q, d, dtype, device)
+    draft = (0, 0, 0)
+    width = cache.max_length
     if k_draft is not None:
-        _check_rows("k_draft", k_draft, total, heads_kv, d, dtype, device)
+        ks = view.check("k_draft", k_draft, total, heads_kv, d, dtype, device)
+        draft = (k_draft.data_ptr(), 2 * ks[0], 2 * ks[1])
+        width += tree.max_nodes
     if lse.device != device or lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[0] != heads_q or \
             lse.shape[1] < total or (lse.shape[1] > 1 and lse.stride(1) != 1):
         raise ValueError(f"lse must be [{heads_q}, at least {total}] float32 on {device} with contiguous rows")
-    view = _view(cache, tree)
-    width = cache.max_length + (tree.max_nodes if k_draft is not None else 0)
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs `out`")
-        out = torch.empty(cache.batch, heads_kv, width, dtype=torch.float32, device=device)
-    elif out.device != device or out.dtype != torch.float32 or out.dim() != 3 or out.shape[0] != cache.batch or \
-            out.shape[1] != heads_kv or out.shape[2] < width or (out.shape[2] > 1 and out.stride(2) != 1):
-        raise ValueError(f"out must be [{cache.batch}, {heads_kv}, at least {width}] float32 on {device} with "
-                         "contiguous rows")
-    if out.shape[0] > 1 and out.stride(0) == 0 or out.shape[1] > 1 and out.stride(1) == 0:
-        raise ValueError("out must not be a broadcast view")
-    kv, e = pool.kv, 2
+        out = torch.empty((cache.batch, heads_kv, width), dtype=torch.float32, device=device)
+        os = (heads_kv * width, width)
+    else:
+        os = out.stride()
+        if out.device != device or out.dtype != torch.float32 or out.dim() != 3 or out.shape[0] != cache.batch or \
+                out.shape[1] != heads_kv or out.shape[2] < width or (out.shape[2] > 1 and os[2] != 1):
+            raise ValueError(f"out must be [{cache.batch}, {heads_kv}, at least {width}] float32 on {device} with "
+                             "contiguous rows")
+        width = out.shape[2]
+        if (cache.batch > 1 and abs(os[0]) < width) or (heads_kv > 1 and abs(os[1]) < width):
+            raise ValueError("out must not have rows that overlap")
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
     with _lib.on_device(device):
-        _lib.call("qe_attention_weights", view.batch, q.data_ptr(), q.stride(0) * e, q.stride(1) * e, heads_q,
-                  heads_kv, d, DTYPES[dtype], kv.data_ptr() + layer * kv.stride(0) * e, pool.rows,
-                  None if k_draft is None else k_draft.data_ptr(), 0 if k_draft is None else k_draft.stride(0) * e,
-                  0 if k_draft is None else k_draft.stride(1) * e, lse.data_ptr(), lse.stride(0),
-                  1.0 / math.sqrt(d) if scale is None else float(scale), 1 if accumulate else 0, out.data_ptr(),
-                  out.stride(0), out.stride(1), out.shape[2], pool._err.data_ptr(), _lib.stream_of(device))
+        args = view.batch + _lib.ATTENTION_WEIGHTS.pack(
+            q.data_ptr(), 2 * qs[0], 2 * qs[1], kv.data_ptr() + 2 * layer * kv.stride(0), pool.rows, *draft,
+            lse.data_ptr(), lse.stride(0), out.data_ptr(), os[0], os[1], width, pool._err.data_ptr(), heads_q, heads_kv,
+            d, DTYPES[dtype], 1 if accumulate else 0, scale)
+        _lib.call("qe_attention_weights", args, _lib.stream_of(device))
     return out
 
 

@@ -421,22 +421,14 @@ class PagedKVPool:
             return
         self._require_cuda(indices, keep, slots)
         src, dst = self._host_slots(indices), self._host_slots(slots)
-        for host in (src, dst):
-            if len(host) and (host.min() < 0 or host.max() >= self.rows):
-                raise ValueError(f"slots outside the pool's {self.rows} rows")
-        mark = np.zeros(self.rows, np.int8)
-        mark[src] = 1
-        hit = bool(mark[dst].any())
-        mark[dst] = 2
-        if hit or int(np.count_nonzero(mark == 2)) != n:
-            raise ValueError("retain: `slots` must hold no slot twice and none of `indices`")
         keep = keep.contiguous()
         src_t = (indices if indices.dtype == torch.int64 else indices.to(torch.int64)).contiguous()
         dst_t = (slots if slots.dtype == torch.int64 else slots.to(torch.int64)).contiguous()
         pool = _lib.planes(self.kv.data_ptr(), self.kv.stride(0) * e, self.kv.stride(1) * e, 2)
         with _lib.on_device(self.device):
             _lib.call("qe_retain", pool, self.rows, self.layers, self.heads, self.head_dim * e, src_t.data_ptr(),
-                      src_t.numel(), keep.data_ptr(), n, dst_t.data_ptr(), self._err.data_ptr(), self._stream())
+                      src.ctypes.data, src_t.numel(), keep.data_ptr(), n, dst_t.data_ptr(), dst.ctypes.data,
+                      self._err.data_ptr(), self._stream())
 
     def free(self, indices: torch.Tensor) -> None:
         """Gives slots from ``alloc`` that were never given to ``insert`` back to the allocator (an addition: e.g. a

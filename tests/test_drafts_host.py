@@ -111,25 +111,34 @@ def test_retain_and_free():
 
 
 def _batch(**over):
-    base = dict(starts=16, lengths=16, tables=16, masks=None, batch=1, table_width=2, page_size=4, mask_words=0, mode=0,
+    base = dict(starts=16, lengths=16, tables=16, masks=0, batch=1, table_width=2, page_size=4, mask_words=0, mode=0,
                 total=3, max_nodes=3, max_length=8, sum_length=8)
     base.update(over)
-    return _lib.DraftBatch(**base)
+    return _lib.DRAFT_BATCH.pack(*base.values())
 
 
-def _attend(batch=None, hq=4, hkv=2, d=64, dtype=1, rows=32, qt=512, scale=0.1, work=None, size=0, kd=16, q=16):
-    _lib.call("qe_tree_attention", batch or _batch(), q, qt, 128, hq, hkv, d, dtype, 16, 16, rows, kd, kd, 256, 128, scale,
-              16, 512, 128, None, work, size, None, None)
+def _tree_args(batch=None, hq=4, hkv=2, d=64, dtype=1, rows=32, qt=512, scale=0.1, work=0, size=0, kd=16, q=16):
+    return (batch or _batch()) + _lib.TREE_ATTENTION.pack(q, qt, 128, 16, 16, rows, kd, kd, 256, 128, 16, 512, 128, 0, work,
+                                                          size, 0, hq, hkv, d, dtype, scale)
+
+
+def _attend(*args, **kw):
+    _lib.call("qe_tree_attention", _tree_args(*args, **kw), None)
+
+
+def _weights_args(weights=16, width=11):
+    return _batch() + _lib.ATTENTION_WEIGHTS.pack(16, 512, 128, 16, 32, 16, 256, 128, 16, 3, weights, 22, 11, width, 0, 4, 2,
+                                                  64, 1, 0, 0.1)
 
 
 @pytest.mark.parametrize("kw,match", [
     (dict(hq=3), "multiple of heads_kv"), (dict(d=96), "head_dim"), (dict(dtype=0), "dtype"), (dict(rows=30), "pool_rows"),
     (dict(qt=24), "16 bytes"), (dict(qt=64), "row of head_dim"), (dict(scale=0.0), "scale"),
-    (dict(scale=float("nan")), "scale"), (dict(q=24), "16-byte"), (dict(kd=8), "16-byte"), (dict(q=None), "null"),
+    (dict(scale=float("nan")), "scale"), (dict(q=24), "16-byte"), (dict(kd=8), "16-byte"), (dict(q=0), "null"),
     (dict(batch=_batch(batch=-1)), "negative"), (dict(batch=_batch(mode=3)), "mode"),
     (dict(batch=_batch(mode=1)), "masks"), (dict(batch=_batch(mode=1, masks=16, mask_words=1, max_nodes=33, total=33)), "masks"),
-    (dict(batch=_batch(page_size=0)), "page_size"), (dict(batch=_batch(tables=None)), "null tables"),
-    (dict(batch=_batch(starts=None)), "null starts"), (dict(batch=_batch(total=2**30)), "2\\^31"),
+    (dict(batch=_batch(page_size=0)), "page_size"), (dict(batch=_batch(tables=0)), "null tables"),
+    (dict(batch=_batch(starts=0)), "null starts"), (dict(batch=_batch(total=2**30)), "2\\^31"),
     (dict(batch=_batch(max_length=1 << 20, sum_length=1 << 20, table_width=1 << 18)), "workspace")])
 def test_c_tree_attention_rejects(kw, match):
     with pytest.raises(ValueError, match=match):
@@ -138,24 +147,40 @@ def test_c_tree_attention_rejects(kw, match):
 
 def test_c_entry_points_reject_and_accept_nothing():
     size = ctypes.c_int64(-1)
-    _lib.call("qe_tree_attention_workspace", _batch(max_length=1 << 20, sum_length=1 << 20), 4, 2, 64, ctypes.byref(size))
+    long = _batch(max_length=1 << 20, sum_length=1 << 20)
+    _lib.call("qe_tree_attention_workspace", _tree_args(long), ctypes.byref(size))
     assert size.value > 0 and size.value % 8 == 0
     with pytest.raises(ValueError):
-        _lib.call("qe_tree_attention_workspace", _batch(), 4, 3, 64, ctypes.byref(size))
+        _lib.call("qe_tree_attention_workspace", _tree_args(hkv=3), ctypes.byref(size))
+    for name in ("qe_tree_attention", "qe_attention_weights"):
+        with pytest.raises(ValueError, match="null arguments"):
+            _lib.call(name, None, None)
     for empty in (_batch(batch=0), _batch(total=0), _batch(max_nodes=0)):
         _attend(empty)
     with pytest.raises(ValueError, match="mask_words"):
         _lib.call("qe_tree_masks", 16, 16, 1, 40, 40, 1, 16, None, None)
     with pytest.raises(ValueError, match="width"):
-        _lib.call("qe_attention_weights", _batch(), 16, 512, 128, 4, 2, 64, 1, 16, 32, 16, 256, 128, 16, 3, 0.1, 0, 16, 20,
-                  10, 10, None, None)
+        _lib.call("qe_attention_weights", _weights_args(width=10), None)
     with pytest.raises(ValueError, match="null weights"):
-        _lib.call("qe_attention_weights", _batch(), 16, 512, 128, 4, 2, 64, 1, 16, 32, 16, 256, 128, 16, 3, 0.1, 0, None, 22,
-                  11, 11, None, None)
+        _lib.call("qe_attention_weights", _weights_args(weights=0), None)
     for args in ((4, 3, 2), (4, -1, 2)):
         with pytest.raises(ValueError):
             _lib.call("qe_heaviest", 16, 1, 1, 1, 0, 0, 0, 9, None, *args, 16, None, None)
+    src, dst = np.array([1, 2, 3, 4], np.int64), np.array([5, 6], np.int64)
+
+    def retain(dst, inner=2, head=32, rows=8):
+        _lib.call("qe_retain", _lib.planes(16, 0, 0, inner), rows, 1, 1, head, 16, src.ctypes.data, 4, 16, 2, 16,
+                  dst.ctypes.data, None, None)
+
     with pytest.raises(ValueError, match="multiple of 16"):
-        _lib.call("qe_retain", _lib.planes(16, 0, 0, 2), 8, 1, 1, 24, 16, 4, 16, 2, 16, None, None)
+        retain(dst, head=24)
     with pytest.raises(ValueError, match=r"\[layers, 2\]"):
-        _lib.call("qe_retain", _lib.planes(16, 0, 0, 1), 8, 1, 1, 32, 16, 4, 16, 2, 16, None, None)
+        retain(dst, inner=1)
+    for bad in ([5, 5], [5, 3]):
+        with pytest.raises(ValueError, match="twice, or among"):
+            retain(np.array(bad, np.int64))
+    for bad in ([5, 8], [-1, 5]):
+        with pytest.raises(ValueError, match="destination slots outside"):
+            retain(np.array(bad, np.int64))
+    with pytest.raises(ValueError, match="source slots outside"):
+        retain(np.array([0, 1], np.int64), rows=4)
