@@ -218,17 +218,6 @@ __device__ __forceinline__ constexpr uint32_t idesc_128<__half>() {
 }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster(uint32_t local, uint32_t rank) {
-  uint32_t at;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
     attention_weights_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const WeightParams p) {
@@ -473,7 +462,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     float w = 0.0f;
     for (int x = 0; x < splits; ++x)
       for (int u = 0; u < 4; ++u)
-        w += x == 0 ? part[u * kTile + threadIdx.x] : ld_cluster(base + S::part + 4 * (u * kTile + threadIdx.x), uint32_t(x));
+        w += x == 0 ? part[u * kTile + threadIdx.x] : ld_cluster1(base + S::part + 4 * (u * kTile + threadIdx.x), uint32_t(x));
     if (key < (draft ? drafted : rq.len)) {
       float *dst = out + (draft ? rq.len : 0) + key;
       *dst = p.accumulate ? *dst + w : w;

@@ -154,6 +154,30 @@ __device__ __forceinline__ float exp2_approx(float x) {  // relative error below
   return y;
 }
 
+// Clusters: a barrier of all their threads, and loads from the shared memory of the CTA of a rank (by the address of
+// the same place in one's own).
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_at(uint32_t local, uint32_t rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(local), "r"(rank));
+  return at;
+}
+__device__ __forceinline__ float ld_cluster1(uint32_t local, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_at(local, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t local, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(cluster_at(local, rank))
+               : "memory");
+  return v;
+}
+
 // Lets the next kernel of the stream be placed while this one drains / waits for the ones before it.
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

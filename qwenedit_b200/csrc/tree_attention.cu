@@ -103,6 +103,7 @@ __global__ void tree_masks_kernel(const int32_t *parents, const int32_t *starts,
 constexpr int kWarps = 4;    // per CTA; two CTAs an SM
 constexpr int kStages = 3;   // 16-key tiles (K and V) in flight per warp
 constexpr int kKeys = 16;    // keys per tile
+constexpr int kMaxCluster = 8;
 constexpr float kGrowLog2 = 8.0f;  // a row's reference maximum moves when a score passes it by more than this
 
 struct TreeParams {
@@ -116,7 +117,8 @@ struct TreeParams {
   int heads_q, heads_kv, group;
   int key_tile;       // keys per tile
   int tiles_per_cta;
-  int splits;         // splits of the longest request (the workspace's)
+  int splits;         // splits of the longest request (the workspace's), or of every request (a cluster's CTAs)
+  int cluster;        // the splits of a (request, head, rows) are one cluster, which joins them
   float scale_log2;
   float *part_o;   // [splits][total * heads_q][D]
   float2 *part_ml;  // [splits][total * heads_q]: (m in log2 units, l)
@@ -151,7 +153,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
   constexpr int kSteps = D / 16;         // k-steps of Q K^T
   constexpr int kTileBytes = kKeys * kRow;
   constexpr int kCopies = kKeys * kChunks / 32;  // per lane and tile, K or V
-  static_assert(kWarps * MT * 16 * (D + 2) * 4 <= kWarps * kStages * 2 * kTileBytes, "the join fits the ring");
+  static_assert((kWarps * (D + 2) + 2) * MT * 16 * 4 <= kWarps * kStages * 2 * kTileBytes, "the join fits the ring");
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, kvh = blockIdx.y % p.heads_kv, row0 = int(blockIdx.y / p.heads_kv) * (MT * 16);
@@ -163,10 +165,14 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
   const int drafted = p.k_draft ? rq.n : 0;
   const int cached_tiles = (rq.len + kKeys - 1) / kKeys;
   const int tiles = tiles_of(rq.len, drafted, kKeys);
-  const int first = int(blockIdx.x) * p.tiles_per_cta;
-  if (first >= tiles && blockIdx.x > 0) return;  // split 0 writes the rows of a request without keys
-  const int last = min(tiles, first + p.tiles_per_cta);
-  const bool whole = tiles <= p.tiles_per_cta;
+  int first = int(blockIdx.x) * p.tiles_per_cta, last = min(tiles, first + p.tiles_per_cta);
+  if (p.cluster) {  // even shares
+    first = int(int64_t(tiles) * blockIdx.x / p.splits);
+    last = int(int64_t(tiles) * (blockIdx.x + 1) / p.splits);
+  } else if (first >= tiles && blockIdx.x > 0) {
+    return;  // split 0 writes the rows of a request without keys
+  }
+  const bool whole = !p.cluster && tiles <= p.tiles_per_cta;
 
   const uint32_t q_smem = smem_u32(smem);
   const uint32_t ring = q_smem + MT * 16 * kRow + warp * (kStages * 2 * kTileBytes);
@@ -454,6 +460,19 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
             make_float2(o[m][j][2 * h], o[m][j][2 * h + 1]);
     }
   __syncthreads();
+  float *am = sl + kWarps * kRows, *al = am + kRows;  // of all warps, for the cluster's join
+  auto write = [&](int r, int c, const float(&acc)[8], float m_all, float l_all) {
+    const int token = rq.lo + (row0 + r) / p.group, head = kvh * p.group + (row0 + r) % p.group;
+    const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;  // no key seen: zeros
+    uint4 v;
+    v.x = pack2<T>(acc[0] * inv, acc[1] * inv);
+    v.y = pack2<T>(acc[2] * inv, acc[3] * inv);
+    v.z = pack2<T>(acc[4] * inv, acc[5] * inv);
+    v.w = pack2<T>(acc[6] * inv, acc[7] * inv);
+    *reinterpret_cast<uint4 *>(p.out + int64_t(token) * p.out_token + int64_t(head) * p.out_head + c * 2) = v;
+    if (p.lse && c == 0)
+      p.lse[int64_t(head) * p.batch.total + token] = l_all == 0.0f ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
+  };
   for (int i = threadIdx.x; i < rows * (D / 8); i += kWarps * 32) {  // 8 columns of a row each
     const int r = i / (D / 8), c = (i % (D / 8)) * 8;
     float m_all = -INFINITY;
@@ -469,25 +488,49 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
       acc[0] += f * x.x, acc[1] += f * x.y, acc[2] += f * x.z, acc[3] += f * x.w;
       acc[4] += f * y.x, acc[5] += f * y.y, acc[6] += f * y.z, acc[7] += f * y.w;
     }
-    const int token = rq.lo + (row0 + r) / p.group, head = kvh * p.group + (row0 + r) % p.group;
     if (whole) {
-      const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;  // no key seen: zeros
-      uint4 v;
-      v.x = pack2<T>(acc[0] * inv, acc[1] * inv);
-      v.y = pack2<T>(acc[2] * inv, acc[3] * inv);
-      v.z = pack2<T>(acc[4] * inv, acc[5] * inv);
-      v.w = pack2<T>(acc[6] * inv, acc[7] * inv);
-      *reinterpret_cast<uint4 *>(p.out + int64_t(token) * p.out_token + int64_t(head) * p.out_head + c * 2) = v;
-      if (p.lse && c == 0)
-        p.lse[int64_t(head) * p.batch.total + token] =
-            l_all == 0.0f ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
+      write(r, c, acc, m_all, l_all);
+      continue;
+    }
+    const float4 x = make_float4(acc[0], acc[1], acc[2], acc[3]), y = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    float4 *dst;
+    if (p.cluster) {  // over warp 0's part, which only this thread reads here
+      dst = reinterpret_cast<float4 *>(so + int64_t(r) * D + c);
+      if (c == 0) am[r] = m_all, al[r] = l_all;
     } else {
-      const int64_t at = (int64_t(blockIdx.x) * p.batch.total + token) * p.heads_q + head;
-      float4 *dst = reinterpret_cast<float4 *>(p.part_o + at * D + c);
-      dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      const int64_t at = (int64_t(blockIdx.x) * p.batch.total + rq.lo + (row0 + r) / p.group) * p.heads_q + kvh * p.group +
+                         (row0 + r) % p.group;
+      dst = reinterpret_cast<float4 *>(p.part_o + at * D + c);
       if (c == 0) p.part_ml[at] = make_float2(m_all, l_all);
     }
+    dst[0] = x;
+    dst[1] = y;
+  }
+  if (p.cluster) {
+    cluster_sync();
+    const int step = p.splits * kWarps * 32;
+    for (int i = int(blockIdx.x) * (kWarps * 32) + threadIdx.x; i < rows * (D / 8); i += step) {
+      const int r = i / (D / 8), c = (i % (D / 8)) * 8;
+      float m_all = -INFINITY, l_all = 0.0f, acc[8] = {};
+      float m[kMaxCluster];
+#pragma unroll
+      for (int x = 0; x < kMaxCluster; ++x) {
+        m[x] = x < p.splits ? ld_cluster1(smem_u32(am + r), uint32_t(x)) : -INFINITY;
+        m_all = fmaxf(m_all, m[x]);
+      }
+#pragma unroll
+      for (int x = 0; x < kMaxCluster; ++x) {
+        if (x >= p.splits) continue;
+        const float f = join_factor(m[x], m_all);
+        const uint32_t at = smem_u32(so + int64_t(r) * D + c);
+        const float4 u = ld_cluster4(at, uint32_t(x)), v = ld_cluster4(at + 16, uint32_t(x));
+        l_all += f * ld_cluster1(smem_u32(al + r), uint32_t(x));
+        acc[0] += f * u.x, acc[1] += f * u.y, acc[2] += f * u.z, acc[3] += f * u.w;
+        acc[4] += f * v.x, acc[5] += f * v.y, acc[6] += f * v.z, acc[7] += f * v.w;
+      }
+      write(r, c, acc, m_all, l_all);
+    }
+    cluster_sync();  // nobody leaves while its sums are read
   }
 }
 
@@ -990,6 +1033,7 @@ struct TreePlan {
   int key_tile;
   int row_ctas;       // CTAs for the rows of a request, all K/V heads
   int splits;
+  bool cluster;       // the splits are a cluster's CTAs, joined there: no workspace, one launch
   int64_t workspace;
 };
 
@@ -1029,22 +1073,39 @@ TreePlan tree_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head
   }
   t.tiles_per_cta = int(per);
   t.splits = int((max_tiles + per - 1) / per);
-  if (t.splits > 1) t.workspace = int64_t(t.splits) * in.total * heads_q * (head_dim + 2) * 4;
+  // Few CTAs: a cluster's join in shared memory saves the second launch and the partial rows' way through memory
+  // (counted as `fixed` tiles).
+  if (!t.tc && t.splits > 1) {
+    for (int x = 2; x <= kMaxCluster; ++x) {
+      const int64_t ctas = int64_t(t.row_ctas) * in.batch * x;
+      const int64_t cost = (ctas + slots - 1) / slots * ((max_tiles + x - 1) / x + fixed);
+      if (cost < best + fixed && (!t.cluster || cost < best)) {
+        best = cost;
+        t.cluster = true;
+        t.splits = x;
+      }
+    }
+    if (t.cluster) t.tiles_per_cta = int((max_tiles + t.splits - 1) / t.splits);
+  }
+  if (t.splits > 1 && !t.cluster) t.workspace = int64_t(t.splits) * in.total * heads_q * (head_dim + 2) * 4;
   return t;
 }
 
 template <auto kKernel, typename... Args>
-int launch(dim3 grid, int threads, int smem, cudaStream_t stream, const char *what, const Args &...args) {
+int launch(dim3 grid, int cluster, int threads, int smem, cudaStream_t stream, const char *what, const Args &...args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(unsigned(threads));
   cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   if (smem > 48 * 1024) {
     static std::atomic<bool> raised[64];  // per device
     int dev = 0;
@@ -1069,15 +1130,15 @@ int run_tree(const TreeParams &p, const TreePlan &t, const qe_draft_batch &in, c
     const uint64_t q_strides[2] = {uint64_t(p.q_head), uint64_t(p.q_token)};
     const uint32_t q_box[3] = {64, uint32_t(p.group), uint32_t(kTcTile / p.group)};
     if ((s = tensor_map_16bit("qe_tree_attention", &q, type, p.q, 3, q_dims, q_strides, q_box, "q"))) return s;
-    s = launch<tree_attention_tc_kernel<T, D>>(grid, kTcThreads, TSmem<D>::bytes, stream, "qe_tree_attention launch", q, p);
+    s = launch<tree_attention_tc_kernel<T, D>>(grid, 1, kTcThreads, TSmem<D>::bytes, stream, "qe_tree_attention launch", q, p);
   } else if (t.m_tiles == 1) {
-    s = launch<tree_attention_kernel<T, D, 1>>(grid, kWarps * 32, tree_smem_bytes<D, 1>(), stream, "qe_tree_attention launch", p);
+    s = launch<tree_attention_kernel<T, D, 1>>(grid, t.cluster ? t.splits : 1, kWarps * 32, tree_smem_bytes<D, 1>(), stream, "qe_tree_attention launch", p);
   } else {
-    s = launch<tree_attention_kernel<T, D, 2>>(grid, kWarps * 32, tree_smem_bytes<D, 2>(), stream, "qe_tree_attention launch", p);
+    s = launch<tree_attention_kernel<T, D, 2>>(grid, t.cluster ? t.splits : 1, kWarps * 32, tree_smem_bytes<D, 2>(), stream, "qe_tree_attention launch", p);
   }
-  if (s || t.splits == 1) return s;
+  if (s || t.splits == 1 || t.cluster) return s;
   const dim3 join(unsigned((in.max_nodes * p.heads_q + 7) / 8), unsigned(in.batch));
-  return launch<tree_join_kernel<T, D>>(join, 256, 0, stream, "qe_tree_attention join launch", p);
+  return launch<tree_join_kernel<T, D>>(join, 1, 256, 0, stream, "qe_tree_attention join launch", p);
 }
 
 bool al16(int64_t v) { return v % 16 == 0; }
@@ -1159,6 +1220,7 @@ extern "C" int qe_tree_attention(const qe_tree_attention_args *args, void *strea
   p.key_tile = t.key_tile;
   p.tiles_per_cta = t.tiles_per_cta;
   p.splits = t.splits;
+  p.cluster = t.cluster ? 1 : 0;
   p.scale_log2 = scale * kLog2e;
   p.part_o = static_cast<float *>(workspace);
   p.part_ml = reinterpret_cast<float2 *>(p.part_o + int64_t(t.splits) * batch.total * heads_q * head_dim);

@@ -99,7 +99,8 @@ def heaviest(weights: torch.Tensor, budget: int, lengths: torch.Tensor | None = 
     if lengths is not None:
         if lengths.device != weights.device or lengths.dtype != torch.int32:
             raise ValueError(f"lengths must be int32 on {weights.device}")
-        lengths = lengths.broadcast_to(lead).contiguous()
+        if lengths.shape != lead or not lengths.is_contiguous():
+            lengths = lengths.broadcast_to(lead).contiguous()
     n = [1] * (3 - len(lead)) + list(lead)
     s = [0] * (3 - len(lead)) + list(weights.stride()[:-1])
     keep = torch.empty(*lead, budget, dtype=torch.int32, device=weights.device)
