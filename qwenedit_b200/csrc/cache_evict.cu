@@ -11,9 +11,13 @@ namespace qe {
 namespace {
 
 // ---- heaviest ---------------------------------------------------------------------------------------------------
-
-constexpr int kThreads = 1024;
-constexpr int kWarps = kThreads / 32;
+//
+// Per row the key (an order-preserving integer) of the last position kept, by radix selection from the top bits, then
+// one ordered pass that writes the kept positions. A CTA per row. A row of up to 32,768 positions is read once, into
+// registers, all its loads in flight together; a longer one is read again in each pass (from L2), eight loads at a
+// time. Digits are 11, 11 and 10 bits: the first holds the sign, the exponent and two mantissa bits, so that weights
+// spread over some octaves meet in one counter a few at a time (with 8-bit digits and a re-read per pass, 1,792 rows of
+// 3,001 to 32,749 took 239 us).
 
 struct HeaviestParams {
   const float *weights;
@@ -28,15 +32,17 @@ struct HeaviestParams {
 __device__ __forceinline__ uint32_t order_key(float x) {
   x = x == x ? x + 0.0f : -INFINITY;
   const uint32_t u = __float_as_uint(x);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
 
-// One CTA per row: the key of the last position kept by radix selection (8 bits a pass, from the top), then one
-// ordered pass that writes the kept positions.
+// kItems > 0: up to kItems positions a thread, in registers (position lo + j * kThreads + thread); 0: any number.
+template <int kThreads, int kItems>
 __global__ void __launch_bounds__(kThreads) heaviest_kernel(const HeaviestParams p) {
-  __shared__ int hist[256];
+  constexpr int kWarps = kThreads / 32, kBins = 2048, kPer = kBins / kThreads;  // counters per thread
+  constexpr int kHeld = kItems > 0 ? kItems : 1;
+  __shared__ int hist[kBins];
+  __shared__ int warp_sum[kWarps];
   __shared__ int found[2];  // digit, positions above it
-  __shared__ int2 counts[kWarps];
   const int64_t row = blockIdx.x;
   const float *w = p.weights + row / (p.n1 * p.n2) * p.s0 + row / p.n2 % p.n1 * p.s1 + row % p.n2 * p.s2;
   int32_t *keep = p.keep + row * p.budget;
@@ -51,46 +57,30 @@ __global__ void __launch_bounds__(kThreads) heaviest_kernel(const HeaviestParams
     return;
   }
   const int lo = p.sinks, hi = n - p.recent;  // n > budget >= sinks + recent: lo < hi
-  int need = p.budget - p.sinks - p.recent;   // of the positions [lo, hi), fewer than there are
-  uint32_t prefix = 0;                        // the bits of the threshold key found so far
-  if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int i = lo + tid; i < hi; i += kThreads) {
-        const uint32_t k = order_key(w[i]);
-        if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
-      }
-      __syncthreads();
-      if (warp == 0) {  // the digit at which the count from the top reaches `need`: lane l holds digits 8 l .. 8 l + 7
-        int mine = 0;
-        for (int e = 0; e < 8; ++e) mine += hist[lane * 8 + e];
-        int above = mine;  // of this lane's digits and the higher lanes'
-        for (int x = 1; x < 32; x <<= 1) {
-          const int y = __shfl_down_sync(0xffffffffu, above, x);
-          if (lane + x < 32) above += y;
-        }
-        const int higher = above - mine;
-        if (higher < need && above >= need) {
-          int c = higher;
-          for (int e = 7; e >= 0; --e) {
-            const int h = hist[lane * 8 + e];
-            if (c + h >= need) {
-              found[0] = lane * 8 + e;
-              found[1] = c;
-              break;
-            }
-            c += h;
-          }
-        }
-      }
-      __syncthreads();
-      prefix = (prefix << 8) | uint32_t(found[0]);
-      need -= found[1];
-    }
+  const float *mid = w + lo;
+  const int count = hi - lo;
+  float held[kHeld];
+  if (kItems > 0) {
+#pragma unroll
+    for (int j = 0; j < kItems; ++j) held[j] = j * kThreads + tid < count ? __ldg(mid + j * kThreads + tid) : 0.0f;
   }
-  // `need` of the positions whose key equals the threshold are kept, the lowest ones
-  const bool any = p.budget > p.sinks + p.recent;
+  // calls f(j, position, weight) for this thread's positions, in rising order
+  auto each = [&](auto f) {
+    if (kItems > 0) {
+#pragma unroll
+      for (int j = 0; j < kItems; ++j)
+        if (j * kThreads + tid < count) f(held[j]);
+    } else {
+      for (int i0 = tid; i0 < count; i0 += 8 * kThreads) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = i0 + u * kThreads < count ? __ldg(mid + i0 + u * kThreads) : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (i0 + u * kThreads < count) f(x[u]);
+      }
+    }
+  };
   for (int i = tid; i < p.sinks; i += kThreads) {
     keep[i] = i;
     if (kept) kept[i] = w[i];
@@ -99,41 +89,126 @@ __global__ void __launch_bounds__(kThreads) heaviest_kernel(const HeaviestParams
     keep[p.budget - p.recent + i] = hi + i;
     if (kept) kept[p.budget - p.recent + i] = w[hi + i];
   }
-  if (!any) return;
-  // every warp takes a run of positions: count those above the threshold and those at it, add up over the warps
-  // before it, then write in order
-  const int per = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int from = lo + warp * per, to = min(hi, from + per);
-  int above = 0, equal = 0;
-  for (int i = from + lane; i < to; i += 32) {
-    const uint32_t k = order_key(w[i]);
-    above += k > prefix;
-    equal += k == prefix;
-  }
-  above = __reduce_add_sync(0xffffffffu, above);
-  equal = __reduce_add_sync(0xffffffffu, equal);
-  if (lane == 0) counts[warp] = make_int2(above, equal);
-  __syncthreads();
-  int above0 = 0, equal0 = 0;
-  for (int x = 0; x < warp; ++x) {
-    above0 += counts[x].x;
-    equal0 += counts[x].y;
-  }
-  for (int i0 = from; i0 < to; i0 += 32) {
-    const int i = i0 + lane;
-    const float x = i < to ? w[i] : 0.0f;
-    const uint32_t k = order_key(x);
-    const uint32_t up = __ballot_sync(0xffffffffu, i < to && k > prefix);
-    const uint32_t eq = __ballot_sync(0xffffffffu, i < to && k == prefix);
-    const uint32_t below = (1u << lane) - 1u;
-    const int a = above0 + __popc(up & below), e = equal0 + __popc(eq & below);
-    if (((up >> lane) & 1u) || (((eq >> lane) & 1u) && e < need)) {
-      const int at = p.sinks + a + min(e, need);
-      keep[at] = i;
-      if (kept) kept[at] = x;
+  int need = p.budget - p.sinks - p.recent;  // of the positions between, fewer than there are
+  if (need == 0) return;
+  uint32_t prefix = 0;  // the threshold key's bits found so far
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
+    const int shift = kShift[pass];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) hist[e * kThreads + tid] = 0;
+    __syncthreads();
+    each([&](float x) {
+      const uint32_t k = order_key(x);
+      if (pass == 0 || (k >> (shift + kBits[pass])) == prefix)
+        atomicAdd(&hist[(k >> shift) & ((1u << kBits[pass]) - 1u)], 1);
+    });
+    __syncthreads();
+    // the digit at which the count from the top reaches `need`: thread t sums counters kBins - 1 - kPer t and below
+    int c[kPer], mine = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) mine += c[e] = hist[kBins - 1 - (tid * kPer + e)];
+    int upto = mine;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, x);
+      if (lane >= x) upto += y;
     }
-    above0 += __popc(up);
-    equal0 += __popc(eq);
+    if (lane == 31) warp_sum[warp] = upto;
+    __syncthreads();
+    int before = upto - mine;
+    for (int x = 0; x < warp; ++x) before += warp_sum[x];
+    if (before < need && before + mine >= need) {
+      int e = 0;
+      while (before + c[e] < need) before += c[e++];
+      found[0] = kBins - 1 - (tid * kPer + e);
+      found[1] = before;
+    }
+    __syncthreads();
+    prefix = (prefix << kBits[pass]) | uint32_t(found[0]);
+    need -= found[1];
+  }
+  // Kept: the positions above the threshold, and the first `need` of those at it. Positions in rising order are
+  // (chunk of kThreads, warp, lane); a pair of 16-bit counts (above, at) per chunk and warp, added up in that order.
+  const int chunks = (count + kThreads - 1) / kThreads;
+  const uint32_t below = (1u << lane) - 1u;
+  int base = 0;        // kept before this round of chunks
+  int at_before = 0;   // at the threshold before it
+  constexpr int kRound = 32;  // chunks: at most 32,768 positions, so that neither 16-bit count runs over
+  static_assert(kRound * kWarps <= kBins && kRound * kThreads <= 32768 && kItems <= kRound, "a round's counts");
+  for (int j0 = 0; j0 < chunks; j0 += kRound) {
+    const int round = min(chunks - j0, kRound);
+    __syncthreads();
+    auto count_chunk = [&](int j, float x, bool there) {
+      const uint32_t k = order_key(x);
+      const uint32_t up = __ballot_sync(0xffffffffu, there && k > prefix);
+      const uint32_t eq = __ballot_sync(0xffffffffu, there && k == prefix);
+      if (lane == 0) hist[(j - j0) * kWarps + warp] = int((uint32_t(__popc(up)) << 16) | uint32_t(__popc(eq)));
+    };
+    if (kItems > 0) {
+#pragma unroll
+      for (int j = 0; j < kItems; ++j)
+        if (j < chunks) count_chunk(j, held[j], j * kThreads + tid < count);
+    } else {
+      for (int j = j0; j < j0 + round; ++j) {
+        const int i = j * kThreads + tid;
+        count_chunk(j, i < count ? __ldg(mid + i) : 0.0f, i < count);
+      }
+    }
+    __syncthreads();
+    // exclusive sums of the pairs (unsigned: `above` may take all 16 bits); a thread takes kPer neighbours
+    uint32_t c[kPer], mine = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      c[e] = tid * kPer + e < round * kWarps ? uint32_t(hist[tid * kPer + e]) : 0u;
+      mine += c[e];
+    }
+    uint32_t upto = mine;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, upto, x);
+      if (lane >= x) upto += y;
+    }
+    if (lane == 31) warp_sum[warp] = int(upto);
+    __syncthreads();
+    uint32_t before = upto - mine, all = 0;
+    for (int x = 0; x < kWarps; ++x) {
+      if (x < warp) before += uint32_t(warp_sum[x]);
+      all += uint32_t(warp_sum[x]);
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      if (tid * kPer + e < round * kWarps) hist[tid * kPer + e] = int(before);
+      before += c[e];
+    }
+    __syncthreads();
+    auto write_chunk = [&](int j, float x, bool there) {
+      const uint32_t k = order_key(x);
+      const uint32_t up = __ballot_sync(0xffffffffu, there && k > prefix);
+      const uint32_t eq = __ballot_sync(0xffffffffu, there && k == prefix);
+      const uint32_t pair = uint32_t(hist[(j - j0) * kWarps + warp]);
+      const int above = int(pair >> 16) + __popc(up & below);
+      const int at = at_before + int(pair & 0xffffu) + __popc(eq & below);
+      if (((up >> lane) & 1u) || (((eq >> lane) & 1u) && at < need)) {
+        const int to = p.sinks + base + above + min(at, need) - min(at_before, need);
+        keep[to] = lo + j * kThreads + tid;
+        if (kept) kept[to] = x;
+      }
+    };
+    if (kItems > 0) {
+#pragma unroll
+      for (int j = 0; j < kItems; ++j)
+        if (j < chunks) write_chunk(j, held[j], j * kThreads + tid < count);
+    } else {
+      for (int j = j0; j < j0 + round; ++j) {
+        const int i = j * kThreads + tid;
+        write_chunk(j, i < count ? __ldg(mid + i) : 0.0f, i < count);
+      }
+    }
+    const int at_all = at_before + int(all & 0xffffu);
+    base += int(all >> 16) + min(at_all, need) - min(at_before, need);
+    at_before = at_all;
   }
 }
 
@@ -221,7 +296,19 @@ extern "C" int qe_heaviest(const float *weights, int64_t n0, int64_t n1, int64_t
   if (rows == 0 || budget == 0) return ok();
   QE_CHECK_ARG((weights || width == 0) && keep, "qe_heaviest: null weights or keep");
   HeaviestParams p{weights, n1, n2, s0, s1, s2, lengths, keep, kept, int(width), int(budget), int(sinks), int(recent)};
-  heaviest_kernel<<<unsigned(rows), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  const unsigned n = unsigned(rows);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t mid = width - sinks - recent;  // at most
+  if (mid <= 2048)
+    heaviest_kernel<512, 4><<<n, 512, 0, st>>>(p);
+  else if (mid <= 8192)
+    heaviest_kernel<512, 16><<<n, 512, 0, st>>>(p);
+  else if (mid <= 16384)
+    heaviest_kernel<512, 32><<<n, 512, 0, st>>>(p);
+  else if (mid <= 32768)
+    heaviest_kernel<1024, 32><<<n, 1024, 0, st>>>(p);
+  else
+    heaviest_kernel<1024, 0><<<n, 1024, 0, st>>>(p);
   const int s = cuda_status(cudaGetLastError(), "qe_heaviest launch");
   return s ? s : ok();
 }
