@@ -13,11 +13,11 @@ namespace {
 // ---- heaviest ---------------------------------------------------------------------------------------------------
 //
 // Per row the key (an order-preserving integer) of the last position kept, by radix selection from the top bits, then
-// one ordered pass that writes the kept positions. A CTA per row. A row of up to 32,768 positions is read once, into
-// registers, all its loads in flight together; a longer one is read again in each pass (from L2), eight loads at a
-// time. Digits are 11, 11 and 10 bits: the first holds the sign, the exponent and two mantissa bits, so that weights
-// spread over some octaves meet in one counter a few at a time (with 8-bit digits and a re-read per pass, 1,792 rows of
-// 3,001 to 32,749 took 239 us).
+// one ordered pass that writes the kept positions. A CTA per row, each warp a run of neighbouring positions. The keys
+// of a row of up to 32,768 positions stay in registers, read once with all loads in flight together; a longer row is
+// read again in each pass (from L2), eight loads at a time. Digits are 11, 11 and 10 bits: the first holds the sign,
+// the exponent and two mantissa bits, so that weights spread over some octaves meet in one counter a few at a time.
+// What bounds it is the instructions per position (25 or so; forms with 128 took five times as long), not the memory.
 
 struct HeaviestParams {
   const float *weights;
@@ -28,21 +28,21 @@ struct HeaviestParams {
   int width, budget, sinks, recent;
 };
 
-// Order-preserving map of fp32 to uint32: NaN as -inf, -0 as +0, so that equal weights are equal keys.
+// Order-preserving map of fp32 to uint32: NaN as -inf, -0 as +0, so that equal weights are equal keys. Never 0, which
+// stands for no position.
 __device__ __forceinline__ uint32_t order_key(float x) {
   x = x == x ? x + 0.0f : -INFINITY;
   const uint32_t u = __float_as_uint(x);
   return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
 
-// kItems > 0: up to kItems positions a thread, in registers (position lo + j * kThreads + thread); 0: any number.
+// kItems > 0: up to kItems positions a thread, in registers; 0: any number.
 template <int kThreads, int kItems>
-__global__ void __launch_bounds__(kThreads) heaviest_kernel(const HeaviestParams p) {
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(const HeaviestParams p) {
   constexpr int kWarps = kThreads / 32, kBins = 2048, kPer = kBins / kThreads;  // counters per thread
-  constexpr int kHeld = kItems > 0 ? kItems : 1;
   __shared__ int hist[kBins];
-  __shared__ int warp_sum[kWarps];
-  __shared__ int found[2];  // digit, positions above it
+  __shared__ int warp_sum[kWarps], warp_at[kWarps];
+  __shared__ int found[3];  // digit, positions above it, positions at it
   const int64_t row = blockIdx.x;
   const float *w = p.weights + row / (p.n1 * p.n2) * p.s0 + row / p.n2 % p.n1 * p.s1 + row % p.n2 * p.s2;
   int32_t *keep = p.keep + row * p.budget;
@@ -59,25 +59,39 @@ __global__ void __launch_bounds__(kThreads) heaviest_kernel(const HeaviestParams
   const int lo = p.sinks, hi = n - p.recent;  // n > budget >= sinks + recent: lo < hi
   const float *mid = w + lo;
   const int count = hi - lo;
-  float held[kHeld];
+  // this warp's run [from, to) of the positions between, `steps` times 32
+  const int run = kItems > 0 ? kItems * 32 : ((count + kThreads - 1) / kThreads) * 32;
+  const int from = warp * run, to = min(count, from + run);
+  const int steps = to > from ? (to - from + 31) / 32 : 0;
+  uint32_t held[kItems > 0 ? kItems : 1];
   if (kItems > 0) {
 #pragma unroll
-    for (int j = 0; j < kItems; ++j) held[j] = j * kThreads + tid < count ? __ldg(mid + j * kThreads + tid) : 0.0f;
+    for (int j = 0; j < kItems; ++j) {
+      const int i = from + j * 32 + lane;
+      held[j] = i < to ? __float_as_uint(__ldg(mid + i)) : 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < kItems; ++j)
+      held[j] = from + j * 32 + lane < to ? order_key(__uint_as_float(held[j])) : 0u;
   }
-  // calls f(j, position, weight) for this thread's positions, in rising order
+  // calls f(key, position) for the warp's run, 32 neighbours at a time (key 0: no position there)
   auto each = [&](auto f) {
     if (kItems > 0) {
 #pragma unroll
-      for (int j = 0; j < kItems; ++j)
-        if (j * kThreads + tid < count) f(held[j]);
+      for (int j = 0; j < kItems; ++j) f(held[j], from + j * 32 + lane);
     } else {
-      for (int i0 = tid; i0 < count; i0 += 8 * kThreads) {
-        float x[8];
+      for (int j0 = 0; j0 < steps; j0 += 8) {
+        uint32_t k[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = i0 + u * kThreads < count ? __ldg(mid + i0 + u * kThreads) : 0.0f;
+        for (int u = 0; u < 8; ++u) {
+          const int i = from + (j0 + u) * 32 + lane;
+          k[u] = i < to ? __float_as_uint(__ldg(mid + i)) : 0u;
+        }
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (i0 + u * kThreads < count) f(x[u]);
+        for (int u = 0; u < 8; ++u) {
+          const int i = from + (j0 + u) * 32 + lane;
+          f(i < to ? order_key(__uint_as_float(k[u])) : 0u, i);
+        }
       }
     }
   };
@@ -92,6 +106,7 @@ __global__ void __launch_bounds__(kThreads) heaviest_kernel(const HeaviestParams
   int need = p.budget - p.sinks - p.recent;  // of the positions between, fewer than there are
   if (need == 0) return;
   uint32_t prefix = 0;  // the threshold key's bits found so far
+  int at_all = 0;       // positions whose key starts with them
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
@@ -99,9 +114,10 @@ __global__ void __launch_bounds__(kThreads) heaviest_kernel(const HeaviestParams
 #pragma unroll
     for (int e = 0; e < kPer; ++e) hist[e * kThreads + tid] = 0;
     __syncthreads();
-    each([&](float x) {
-      const uint32_t k = order_key(x);
-      if (pass == 0 || (k >> (shift + kBits[pass])) == prefix)
+    each([&](uint32_t k, int) {  // no position: a key below every real one, counted where no threshold can be
+      if (pass == 0)
+        atomicAdd(&hist[k >> 21], 1);
+      else if ((k >> (shift + kBits[pass])) == prefix)
         atomicAdd(&hist[(k >> shift) & ((1u << kBits[pass]) - 1u)], 1);
     });
     __syncthreads();
@@ -120,96 +136,57 @@ __global__ void __launch_bounds__(kThreads) heaviest_kernel(const HeaviestParams
     int before = upto - mine;
     for (int x = 0; x < warp; ++x) before += warp_sum[x];
     if (before < need && before + mine >= need) {
-      int e = 0;
-      while (before + c[e] < need) before += c[e++];
-      found[0] = kBins - 1 - (tid * kPer + e);
-      found[1] = before;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        if (before < need && before + c[e] >= need) {
+          found[0] = kBins - 1 - (tid * kPer + e);
+          found[1] = before;
+          found[2] = c[e];
+        }
+        before += c[e];
+      }
     }
     __syncthreads();
     prefix = (prefix << kBits[pass]) | uint32_t(found[0]);
     need -= found[1];
+    at_all = found[2];
   }
-  // Kept: the positions above the threshold, and the first `need` of those at it. Positions in rising order are
-  // (chunk of kThreads, warp, lane); a pair of 16-bit counts (above, at) per chunk and warp, added up in that order.
-  const int chunks = (count + kThreads - 1) / kThreads;
+  // Kept: the positions above the threshold and the first `need` of the at_all at it. Without ties to cut those are
+  // the keys of at least the threshold; else the positions at it are counted apart.
+  const bool cut = need < at_all;
+  int above = 0, at = 0;
+  each([&](uint32_t k, int) {
+    above += __popc(__ballot_sync(0xffffffffu, cut ? k > prefix : k >= prefix));
+    if (cut) at += __popc(__ballot_sync(0xffffffffu, k == prefix));
+  });
+  if (lane == 0) {
+    warp_sum[warp] = above;
+    warp_at[warp] = at;
+  }
+  __syncthreads();
+  above = at = 0;  // of the warps before
+  for (int x = 0; x < warp; ++x) {
+    above += warp_sum[x];
+    at += warp_at[x];
+  }
   const uint32_t below = (1u << lane) - 1u;
-  int base = 0;        // kept before this round of chunks
-  int at_before = 0;   // at the threshold before it
-  constexpr int kRound = 32;  // chunks: at most 32,768 positions, so that neither 16-bit count runs over
-  static_assert(kRound * kWarps <= kBins && kRound * kThreads <= 32768 && kItems <= kRound, "a round's counts");
-  for (int j0 = 0; j0 < chunks; j0 += kRound) {
-    const int round = min(chunks - j0, kRound);
-    __syncthreads();
-    auto count_chunk = [&](int j, float x, bool there) {
-      const uint32_t k = order_key(x);
-      const uint32_t up = __ballot_sync(0xffffffffu, there && k > prefix);
-      const uint32_t eq = __ballot_sync(0xffffffffu, there && k == prefix);
-      if (lane == 0) hist[(j - j0) * kWarps + warp] = int((uint32_t(__popc(up)) << 16) | uint32_t(__popc(eq)));
-    };
-    if (kItems > 0) {
-#pragma unroll
-      for (int j = 0; j < kItems; ++j)
-        if (j < chunks) count_chunk(j, held[j], j * kThreads + tid < count);
-    } else {
-      for (int j = j0; j < j0 + round; ++j) {
-        const int i = j * kThreads + tid;
-        count_chunk(j, i < count ? __ldg(mid + i) : 0.0f, i < count);
-      }
+  each([&](uint32_t k, int i) {
+    const uint32_t up = __ballot_sync(0xffffffffu, cut ? k > prefix : k >= prefix);
+    bool take = (up >> lane) & 1u;
+    int place = above + __popc(up & below);
+    above += __popc(up);
+    if (cut) {
+      const uint32_t eq = __ballot_sync(0xffffffffu, k == prefix);
+      const int mine = at + __popc(eq & below);
+      take = take || (((eq >> lane) & 1u) && mine < need);
+      place += min(mine, need);
+      at += __popc(eq);
     }
-    __syncthreads();
-    // exclusive sums of the pairs (unsigned: `above` may take all 16 bits); a thread takes kPer neighbours
-    uint32_t c[kPer], mine = 0;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      c[e] = tid * kPer + e < round * kWarps ? uint32_t(hist[tid * kPer + e]) : 0u;
-      mine += c[e];
+    if (take) {
+      keep[p.sinks + place] = lo + i;
+      if (kept) kept[p.sinks + place] = __ldg(mid + i);
     }
-    uint32_t upto = mine;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      const uint32_t y = __shfl_up_sync(0xffffffffu, upto, x);
-      if (lane >= x) upto += y;
-    }
-    if (lane == 31) warp_sum[warp] = int(upto);
-    __syncthreads();
-    uint32_t before = upto - mine, all = 0;
-    for (int x = 0; x < kWarps; ++x) {
-      if (x < warp) before += uint32_t(warp_sum[x]);
-      all += uint32_t(warp_sum[x]);
-    }
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      if (tid * kPer + e < round * kWarps) hist[tid * kPer + e] = int(before);
-      before += c[e];
-    }
-    __syncthreads();
-    auto write_chunk = [&](int j, float x, bool there) {
-      const uint32_t k = order_key(x);
-      const uint32_t up = __ballot_sync(0xffffffffu, there && k > prefix);
-      const uint32_t eq = __ballot_sync(0xffffffffu, there && k == prefix);
-      const uint32_t pair = uint32_t(hist[(j - j0) * kWarps + warp]);
-      const int above = int(pair >> 16) + __popc(up & below);
-      const int at = at_before + int(pair & 0xffffu) + __popc(eq & below);
-      if (((up >> lane) & 1u) || (((eq >> lane) & 1u) && at < need)) {
-        const int to = p.sinks + base + above + min(at, need) - min(at_before, need);
-        keep[to] = lo + j * kThreads + tid;
-        if (kept) kept[to] = x;
-      }
-    };
-    if (kItems > 0) {
-#pragma unroll
-      for (int j = 0; j < kItems; ++j)
-        if (j < chunks) write_chunk(j, held[j], j * kThreads + tid < count);
-    } else {
-      for (int j = j0; j < j0 + round; ++j) {
-        const int i = j * kThreads + tid;
-        write_chunk(j, i < count ? __ldg(mid + i) : 0.0f, i < count);
-      }
-    }
-    const int at_all = at_before + int(all & 0xffffu);
-    base += int(all >> 16) + min(at_all, need) - min(at_before, need);
-    at_before = at_all;
-  }
+  });
 }
 
 // ---- retain -----------------------------------------------------------------------------------------------------
