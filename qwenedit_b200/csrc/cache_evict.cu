@@ -14,8 +14,8 @@ namespace {
 //
 // Per row the key (an order-preserving integer) of the last position kept, by radix selection from the top bits, then
 // one ordered pass that writes the kept positions. A CTA per row, each warp a run of neighbouring positions. The keys
-// of a row of up to 32,768 positions stay in registers, read once with all loads in flight together; a longer row is
-// read again in each pass (from L2), eight loads at a time. Digits are 11, 11 and 10 bits: the first holds the sign,
+// of a row of up to 73,728 positions stay on the SM, in registers (to 32,768) and shared memory, read once with the
+// loads in flight together; a longer row is read again in each pass (from L2), eight loads at a time. Digits are 11, 11 and 10 bits: the first holds the sign,
 // the exponent and two mantissa bits, so that weights spread over some octaves meet in one counter a few at a time.
 // What bounds it is the instructions per position (25 or so; forms with 128 took five times as long), not the memory.
 
@@ -36,11 +36,12 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
 
-// kItems > 0: up to kItems positions a thread, in registers; 0: any number.
-template <int kThreads, int kItems>
+// kItems > 0: up to kItems positions a thread in registers, kStored more in shared memory; 0: any number.
+template <int kThreads, int kItems, int kStored>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(const HeaviestParams p) {
   constexpr int kWarps = kThreads / 32, kBins = 2048, kPer = kBins / kThreads;  // counters per thread
-  __shared__ int hist[kBins];
+  extern __shared__ uint32_t stored[];  // [kStored][kThreads]
+  __shared__ int hists[3][kBins];
   __shared__ int warp_sum[kWarps], warp_at[kWarps];
   __shared__ int found[3];  // digit, positions above it, positions at it
   const int64_t row = blockIdx.x;
@@ -60,25 +61,40 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
   const float *mid = w + lo;
   const int count = hi - lo;
   // this warp's run [from, to) of the positions between, `steps` times 32
-  const int run = kItems > 0 ? kItems * 32 : ((count + kThreads - 1) / kThreads) * 32;
+  const int run = (count + kThreads - 1) / kThreads * 32;
   const int from = warp * run, to = min(count, from + run);
   const int steps = to > from ? (to - from + 31) / 32 : 0;
   uint32_t held[kItems > 0 ? kItems : 1];
   if (kItems > 0) {
-#pragma unroll
-    for (int j = 0; j < kItems; ++j) {
+    auto bits_at = [&](int j) {
       const int i = from + j * 32 + lane;
-      held[j] = i < to ? __float_as_uint(__ldg(mid + i)) : 0u;
+      return i < to ? __float_as_uint(__ldg(mid + i)) : 0u;
+    };
+    auto key_at = [&](int j, uint32_t bits) { return from + j * 32 + lane < to ? order_key(__uint_as_float(bits)) : 0u; };
+#pragma unroll
+    for (int j = 0; j < kItems; ++j)
+      if (j < steps) held[j] = bits_at(j);
+    for (int j0 = 0; j0 < kStored; j0 += 8) {
+      if (kItems + j0 >= steps) break;
+      uint32_t x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = bits_at(kItems + j0 + u);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) stored[(j0 + u) * kThreads + tid] = key_at(kItems + j0 + u, x[u]);
     }
 #pragma unroll
     for (int j = 0; j < kItems; ++j)
-      held[j] = from + j * 32 + lane < to ? order_key(__uint_as_float(held[j])) : 0u;
+      if (j < steps) held[j] = key_at(j, held[j]);
   }
   // calls f(key, position) for the warp's run, 32 neighbours at a time (key 0: no position there)
   auto each = [&](auto f) {
     if (kItems > 0) {
 #pragma unroll
-      for (int j = 0; j < kItems; ++j) f(held[j], from + j * 32 + lane);
+      for (int j = 0; j < kItems; ++j)
+        if (j < steps) f(held[j], from + j * 32 + lane);
+      if (kStored > 0)
+#pragma unroll 8
+        for (int j = kItems; j < steps; ++j) f(stored[(j - kItems) * kThreads + tid], from + j * 32 + lane);
     } else {
       for (int j0 = 0; j0 < steps; j0 += 8) {
         uint32_t k[8];
@@ -95,6 +111,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
       }
     }
   };
+  // this warp's place in sums over the warps (every warp adds up all of them)
+  auto before_warp = [&](const int *sums) {
+    int x = lane < kWarps && lane < warp ? sums[lane] : 0;
+    return __reduce_add_sync(0xffffffffu, x);
+  };
+#pragma unroll
+  for (int e = 0; e < 3 * kPer; ++e) hists[0][e * kThreads + tid] = 0;
   for (int i = tid; i < p.sinks; i += kThreads) {
     keep[i] = i;
     if (kept) kept[i] = w[i];
@@ -111,9 +134,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
   for (int pass = 0; pass < 3; ++pass) {
     constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
     const int shift = kShift[pass];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) hist[e * kThreads + tid] = 0;
-    __syncthreads();
+    int *hist = hists[pass];
+    if (pass == 0) __syncthreads();
     each([&](uint32_t k, int) {  // no position: a key below every real one, counted where no threshold can be
       if (pass == 0)
         atomicAdd(&hist[k >> 21], 1);
@@ -133,8 +155,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
     }
     if (lane == 31) warp_sum[warp] = upto;
     __syncthreads();
-    int before = upto - mine;
-    for (int x = 0; x < warp; ++x) before += warp_sum[x];
+    int before = upto - mine + before_warp(warp_sum);
     if (before < need && before + mine >= need) {
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
@@ -164,11 +185,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
     warp_at[warp] = at;
   }
   __syncthreads();
-  above = at = 0;  // of the warps before
-  for (int x = 0; x < warp; ++x) {
-    above += warp_sum[x];
-    at += warp_at[x];
-  }
+  above = before_warp(warp_sum);
+  at = before_warp(warp_at);
   const uint32_t below = (1u << lane) - 1u;
   each([&](uint32_t k, int i) {
     const uint32_t up = __ballot_sync(0xffffffffu, cut ? k > prefix : k >= prefix);
@@ -276,16 +294,31 @@ extern "C" int qe_heaviest(const float *weights, int64_t n0, int64_t n1, int64_t
   const unsigned n = unsigned(rows);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t mid = width - sinks - recent;  // at most
-  if (mid <= 2048)
-    heaviest_kernel<512, 4><<<n, 512, 0, st>>>(p);
-  else if (mid <= 8192)
-    heaviest_kernel<512, 16><<<n, 512, 0, st>>>(p);
-  else if (mid <= 16384)
-    heaviest_kernel<512, 32><<<n, 512, 0, st>>>(p);
-  else if (mid <= 32768)
-    heaviest_kernel<1024, 32><<<n, 1024, 0, st>>>(p);
-  else
-    heaviest_kernel<1024, 0><<<n, 1024, 0, st>>>(p);
+  if (mid <= 1024) {
+    heaviest_kernel<256, 4, 0><<<n, 256, 0, st>>>(p);
+  } else if (mid <= 4096) {
+    heaviest_kernel<256, 16, 0><<<n, 256, 0, st>>>(p);
+  } else if (mid <= 8192) {
+    heaviest_kernel<512, 16, 0><<<n, 512, 0, st>>>(p);
+  } else if (mid <= 16384) {
+    heaviest_kernel<512, 32, 0><<<n, 512, 0, st>>>(p);
+  } else if (mid <= 32768) {
+    heaviest_kernel<1024, 32, 0><<<n, 1024, 0, st>>>(p);
+  } else if (mid <= 73728) {
+    constexpr int kStored = 48, kBytes = kStored * 1024 * 4;
+    auto kernel = heaviest_kernel<1024, 24, kStored>;
+    static std::atomic<bool> raised[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (!raised[dev].load(std::memory_order_relaxed)) {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+      if (e != cudaSuccess) return cuda_status(e, "qe_heaviest: smem attribute");
+      raised[dev].store(true, std::memory_order_relaxed);
+    }
+    kernel<<<n, 1024, kBytes, st>>>(p);
+  } else {
+    heaviest_kernel<1024, 0, 0><<<n, 1024, 0, st>>>(p);
+  }
   const int s = cuda_status(cudaGetLastError(), "qe_heaviest launch");
   return s ? s : ok();
 }
