@@ -2,10 +2,10 @@
 // group) of e^{scale q . K_j - lse_row}.
 //
 // With the rows' log-sum-exp at hand a key's weight needs its own K row and all query rows, nothing of the other
-// keys: the keys are split over warps, each warp keeps 16 keys' K as the A operand of S^T = K Q^T and runs over the
-// query rows, and the weights are sums over the columns of S^T. One pass over K, no joining of partial results.
+// keys: the keys are split over CTAs and warps, and nothing has to be joined.
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -16,9 +16,13 @@ namespace qe {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kKeys = 16;    // keys per warp and pass
-constexpr int kQRows = 128;  // query rows in shared memory at a time
-constexpr int kTcRows = 64;  // more query rows a K/V head than this: the tensor-memory kernel
+constexpr int kKeys = 16;    // keys per tile
+constexpr int kStages = 4;   // tiles of K in flight per warp
+constexpr int kQRows = 64;   // query rows in shared memory at a time
+#ifndef QE_W_TC
+#define QE_W_TC 64
+#endif
+constexpr int kTcRows = QE_W_TC;  // more query rows a K/V head than this: the tensor-memory kernel
 
 struct WeightParams {
   DecodeBatch batch;
@@ -38,14 +42,19 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
   return uint32_t(r * (D * 2) + ((c ^ (r & 7)) << 4));
 }
 
+// ---- few rows: every warp streams its own keys ------------------------------------------------------------------
+//
+// S^T = K Q^T with 16 keys as the A operand, the query rows (in shared memory) as B, eight at a time: a thread holds two
+// keys' scores against two of the eight rows. One pass over K per 64 query rows, four tiles of 16 keys in flight a warp.
+
 template <int D>
 constexpr int weights_smem() {
-  return kQRows * D * 2 + kWarps * kKeys * D * 2 + kQRows * 8;
+  return kQRows * D * 2 + kWarps * kStages * kKeys * D * 2 + kQRows * 8;
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kWarps * 32) attention_weights_kernel(const WeightParams p) {
-  constexpr int kChunks = D / 8, kSteps = D / 16, kCopies = kKeys * kChunks / 32;
+  constexpr int kChunks = D / 8, kSteps = D / 16, kCopies = kKeys * kChunks / 32, kTileBytes = kKeys * D * 2;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, kvh = blockIdx.y;
@@ -62,104 +71,118 @@ __global__ void __launch_bounds__(kWarps * 32) attention_weights_kernel(const We
       out[j] = 0.0f;
   if (first >= last) return;
 
-  const uint32_t qs = smem_u32(smem), ks = qs + kQRows * D * 2 + warp * kKeys * D * 2;
-  float *lse_s = reinterpret_cast<float *>(smem + kQRows * D * 2 + kWarps * kKeys * D * 2);  // log2 units
+  const uint32_t qs = smem_u32(smem), ring = qs + kQRows * D * 2 + warp * (kStages * kTileBytes);
+  float *lse_s = reinterpret_cast<float *>(smem + kQRows * D * 2 + kWarps * kStages * kTileBytes);  // log2 units
   int *node_s = reinterpret_cast<int *>(lse_s + kQRows);
-  const int passes = (last - first + kWarps - 1) / kWarps;
-  int q_at = -1;  // the query rows in shared memory
-  for (int pass = 0; pass < passes; ++pass) {
-    const int t = first + pass * kWarps + warp;
-    const bool there = t < last, draft_tile = t >= cached_tiles;
-    // this warp's 16 keys
-    int row = -1;
-    if (there && lane < kKeys) {
-      if (!draft_tile) {
-        const int key = t * kKeys + lane;
-        if (key < rq.len) row = pool_row(p.batch, b, key);
-      } else {
-        const int j = (t - cached_tiles) * kKeys + lane;
-        if (j < drafted) row = rq.lo + j;
-      }
-    }
-    const char *base = draft_tile ? p.k_draft + int64_t(kvh) * p.draft_head : p.k_pool + int64_t(kvh) * (D * 2);
-    const int64_t stride = draft_tile ? p.draft_token : p.pool_row;
-    __syncwarp();
+  // key `lane` of tile t: fetch reads its table entry, settle makes of it, a tile later, the pool row (or the drafted
+  // token; -1: nothing there), so that no one waits for the table
+  auto fetch = [&](int t) -> int {
+    const int key = t * kKeys + lane;
+    return t < last && t < cached_tiles && lane < kKeys && key < rq.len
+               ? __ldg(p.batch.tables + int64_t(b) * p.batch.table_width + page_index(p.batch, key))
+               : INT_MIN;
+  };
+  auto settle = [&](int t, int page) -> int {
+    if (t < cached_tiles) return page == INT_MIN ? -1 : row_in_page(p.batch, page, t * kKeys + lane);
+    const int j = (t - cached_tiles) * kKeys + lane;
+    return t < last && lane < kKeys && j < drafted ? rq.lo + j : -1;
+  };
+  for (int q0 = 0; q0 < rows || q0 == 0; q0 += kQRows) {
+    int t_load = first + warp;
+    int page = fetch(t_load);
+    auto copy_next = [&](int stage) {
+      const int row = settle(t_load, page);
+      page = fetch(t_load + kWarps);
+      if (t_load < last) {
+        const bool draft = t_load >= cached_tiles;
+        const char *base = draft ? p.k_draft + int64_t(kvh) * p.draft_head : p.k_pool + int64_t(kvh) * (D * 2);
+        const int64_t stride = draft ? p.draft_token : p.pool_row;
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int r = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
-      const int at = __shfl_sync(0xffffffffu, row, r);
-      cp_async16(ks + chunk_at<D>(r, c), at < 0 ? base : base + int64_t(at) * stride + c * 16, at < 0 || !there ? 0 : 16);
-    }
-    cp_async_commit();
-    cp_async_wait<0>();
-    __syncwarp();
-    uint32_t kf[kSteps][4];
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k)
-      ldmatrix4(kf[k], ks + chunk_at<D>(((lane >> 3) & 1) * 8 + (lane & 7), 2 * k + (lane >> 4)));
-    float sum[2] = {0.0f, 0.0f};  // keys lane / 4 and lane / 4 + 8, this lane's columns
-    for (int q0 = 0; q0 < rows; q0 += kQRows) {
-      if (q_at != q0) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < kQRows * kChunks; i += kWarps * 32) {
-          const int r = i / kChunks, c = i % kChunks;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (q0 + r < rows) {
-            const int node = (q0 + r) / p.group, g = (q0 + r) % p.group;
-            v = __ldg(reinterpret_cast<const uint4 *>(p.q + int64_t(rq.lo + node) * p.q_token +
-                                                      int64_t(kvh * p.group + g) * p.q_head + c * 16));
-          }
-          *reinterpret_cast<uint4 *>(smem + chunk_at<D>(r, c)) = v;
+        for (int i = 0; i < kCopies; ++i) {
+          const int r = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
+          const int at = __shfl_sync(0xffffffffu, row, r);
+          cp_async16(ring + stage * kTileBytes + chunk_at<D>(r, c), at < 0 ? base : base + int64_t(at) * stride + c * 16,
+                     at < 0 ? 0 : 16);
         }
-        for (int r = threadIdx.x; r < kQRows; r += kWarps * 32) {
-          float x = INFINITY;  // counts nothing
-          int node = 0;
-          if (q0 + r < rows) {
-            node = (q0 + r) / p.group;
-            x = p.lse[int64_t(kvh * p.group + (q0 + r) % p.group) * p.lse_head + rq.lo + node] * kLog2e;
-            if (x == -INFINITY) x = INFINITY;
-          }
-          lse_s[r] = x;
-          node_s[r] = node;
-        }
-        __syncthreads();
-        q_at = q0;
       }
-      const int blocks = min((rows - q0 + 7) / 8, kQRows / 8);
+      cp_async_commit();
+      t_load += kWarps;
+    };
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) copy_next(s);
+    // the query rows and their lse
+    if (q0 > 0) __syncthreads();
+    const int here = min(rows - q0, kQRows), blocks = (here + 7) / 8;
+    for (int i = threadIdx.x; i < blocks * 8 * kChunks; i += kWarps * 32) {
+      const int r = i / kChunks, c = i % kChunks;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < here) {
+        const int node = (q0 + r) / p.group, g = (q0 + r) % p.group;
+        v = __ldg(reinterpret_cast<const uint4 *>(p.q + int64_t(rq.lo + node) * p.q_token +
+                                                  int64_t(kvh * p.group + g) * p.q_head + c * 16));
+      }
+      *reinterpret_cast<uint4 *>(smem + chunk_at<D>(r, c)) = v;
+    }
+    for (int r = threadIdx.x; r < blocks * 8; r += kWarps * 32) {
+      float x = INFINITY;  // counts nothing
+      int node = 0;
+      if (r < here) {
+        node = (q0 + r) / p.group;
+        x = p.lse[int64_t(kvh * p.group + (q0 + r) % p.group) * p.lse_head + rq.lo + node] * kLog2e;
+        if (x == -INFINITY) x = INFINITY;
+      }
+      lse_s[r] = x;
+      node_s[r] = node;
+    }
+    __syncthreads();
+    int stage = 0;
+    for (int t = first + warp; t < last; t += kWarps) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();  // every lane's copies of this tile have landed, and the stage filled next is no longer read
+      copy_next((stage + kStages - 1) % kStages);
+      const uint32_t ks = ring + stage * kTileBytes;
+      uint32_t kf[kSteps][4];
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+        ldmatrix4(kf[k], ks + chunk_at<D>(((lane >> 3) & 1) * 8 + (lane & 7), 2 * k + (lane >> 4)));
+      const bool draft_tile = t >= cached_tiles;
+      float sum[2] = {0.0f, 0.0f};  // keys lane / 4 and lane / 4 + 8, this lane's columns
       for (int nb = 0; nb < blocks; ++nb) {
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float s[2][4] = {};  // even and odd k-steps, so that two products are under way
 #pragma unroll
         for (int k = 0; k < kSteps; k += 2) {
           uint32_t qb[4];
           ldmatrix4(qb, qs + chunk_at<D>(nb * 8 + (lane & 7), 2 * k + (lane >> 3)));
-          mma16816<T>(s, kf[k], qb[0], qb[1]);
-          mma16816<T>(s, kf[k + 1], qb[2], qb[3]);
+          mma16816<T>(s[0], kf[k], qb[0], qb[1]);
+          mma16816<T>(s[1], kf[k + 1], qb[2], qb[3]);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = nb * 8 + (lane & 3) * 2 + e;
           const float x = lse_s[r];
-          uint32_t bits = 0xffffu;
-          if (draft_tile) bits = draft_bits16(p.batch, rq, node_s[r], (t - cached_tiles) * kKeys);
-          const bool counts = x != INFINITY;
+          uint32_t bits = x != INFINITY ? 0xffffu : 0u;
+          if (draft_tile) bits &= draft_bits16(p.batch, rq, node_s[r], (t - cached_tiles) * kKeys);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float w = exp2_approx(fmaf(s[2 * h + e], p.scale_log2, -x));
-            if (counts && ((bits >> (lane / 4 + 8 * h)) & 1u)) sum[h] += w;
+            const float w = exp2_approx(fmaf(s[0][2 * h + e] + s[1][2 * h + e], p.scale_log2, -x));
+            if ((bits >> (lane / 4 + 8 * h)) & 1u) sum[h] += w;
           }
         }
       }
-    }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-      const int key = (draft_tile ? t - cached_tiles : t) * kKeys + lane / 4 + 8 * h;
-      if (there && (lane & 3) == 0 && key < (draft_tile ? drafted : rq.len)) {
-        float *dst = out + (draft_tile ? rq.len : 0) + key;
-        *dst = p.accumulate ? *dst + sum[h] : sum[h];
+      for (int h = 0; h < 2; ++h) {
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+        sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+        const int key = (draft_tile ? t - cached_tiles : t) * kKeys + lane / 4 + 8 * h;
+        if ((lane & 3) == 0 && key < (draft_tile ? drafted : rq.len)) {
+          float *dst = out + (draft_tile ? rq.len : 0) + key;
+          *dst = p.accumulate || q0 > 0 ? *dst + sum[h] : sum[h];
+        }
       }
+      stage = (stage + 1) % kStages;
     }
+    cp_async_wait<0>();
+    __syncwarp();
   }
 }
 
@@ -592,9 +615,20 @@ extern "C" int qe_attention_weights(const qe_attention_weights_args *args, void 
   p.scale_log2 = scale * kLog2e;
   const int nodes = k_draft ? batch.max_nodes : 0;
   const int max_tiles = std::max(1, (batch.max_length + kKeys - 1) / kKeys + (nodes + kKeys - 1) / kKeys);
+  // tiles a CTA: the count that ends first by waves x (tiles + a start's 12), half a CTA more per request
   const int64_t all = (batch.sum_length + kKeys - 1) / kKeys + int64_t(batch.batch) * ((nodes + kKeys - 1) / kKeys);
-  int64_t per = (all * heads_kv + 4 * sm_count() - 1) / (4 * sm_count());
-  per = std::min<int64_t>(std::max<int64_t>((per + kWarps - 1) / kWarps * kWarps, kWarps), 1 << 20);
+  const int64_t slots = 2 * int64_t(sm_count());
+  int64_t per = max_tiles, best = INT64_MAX;
+  for (int64_t x = kWarps;; x = std::max(x + kWarps, x * 9 / 8 / kWarps * kWarps)) {
+    x = std::min<int64_t>(x, max_tiles);
+    const int64_t ctas = heads_kv * ((all + x - 1) / x + (x < max_tiles && batch.batch > 1 ? batch.batch / 2 : 0));
+    const int64_t cost = (ctas + slots - 1) / slots * (x + 12);
+    if (cost < best) {
+      best = cost;
+      per = x;
+    }
+    if (x == max_tiles) break;
+  }
   p.tiles_per_cta = int(per);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (int64_t(batch.max_nodes) * p.group > kTcRows && p.group <= kTile) {
