@@ -17,12 +17,8 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kKeys = 16;    // keys per tile
-constexpr int kStages = 4;   // tiles of K in flight per warp
-constexpr int kQRows = 64;   // query rows in shared memory at a time
-#ifndef QE_W_TC
-#define QE_W_TC 64
-#endif
-constexpr int kTcRows = QE_W_TC;  // more query rows a K/V head than this: the tensor-memory kernel
+constexpr int kQRows = 224;   // query rows in shared memory at a time, at most
+constexpr int kTcRows = 224;  // more query rows a K/V head than this: the tensor-memory kernel
 
 struct WeightParams {
   DecodeBatch batch;
@@ -33,7 +29,7 @@ struct WeightParams {
   float *weights;
   int64_t weights_batch, weights_head, width;
   int heads_q, heads_kv, group, accumulate;
-  int tiles_per_cta;
+  int tiles_per_cta, q_rows;  // q_rows: query rows in shared memory at a time
   float scale_log2;
 };
 
@@ -45,14 +41,17 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 // ---- few rows: every warp streams its own keys ------------------------------------------------------------------
 //
 // S^T = K Q^T with 16 keys as the A operand, the query rows (in shared memory) as B, eight at a time: a thread holds two
-// keys' scores against two of the eight rows. One pass over K per 64 query rows, four tiles of 16 keys in flight a warp.
+// keys' scores against two of the eight rows. One pass over K per 224 query rows.
 
-template <int D>
-constexpr int weights_smem() {
-  return kQRows * D * 2 + kWarps * kStages * kKeys * D * 2 + kQRows * 8;
+// tiles of K per warp in the ring: three where the bytes bound the call (32 requests of 257 to 8,191 tokens, 7 rows a
+// K/V head: 41.5 us with four, 29.1 with three, 35.1 with two), two where the rows do and CTAs an SM count for more
+// (56 rows: 90 / 67 / 58 us)
+inline int stages_for(int q_rows) { return q_rows <= 16 ? 3 : 2; }
+inline int weights_smem(int d, int q_rows) {
+  return q_rows * d * 2 + kWarps * stages_for(q_rows) * kKeys * d * 2 + q_rows * 8;
 }
 
-template <typename T, int D>
+template <typename T, int D, int kStages>
 __global__ void __launch_bounds__(kWarps * 32) attention_weights_kernel(const WeightParams p) {
   constexpr int kChunks = D / 8, kSteps = D / 16, kCopies = kKeys * kChunks / 32, kTileBytes = kKeys * D * 2;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -71,9 +70,10 @@ __global__ void __launch_bounds__(kWarps * 32) attention_weights_kernel(const We
       out[j] = 0.0f;
   if (first >= last) return;
 
-  const uint32_t qs = smem_u32(smem), ring = qs + kQRows * D * 2 + warp * (kStages * kTileBytes);
-  float *lse_s = reinterpret_cast<float *>(smem + kQRows * D * 2 + kWarps * kStages * kTileBytes);  // log2 units
-  int *node_s = reinterpret_cast<int *>(lse_s + kQRows);
+  const int q_rows = p.q_rows;
+  const uint32_t qs = smem_u32(smem), ring = qs + q_rows * D * 2 + warp * (kStages * kTileBytes);
+  float *lse_s = reinterpret_cast<float *>(smem + q_rows * D * 2 + kWarps * kStages * kTileBytes);  // log2 units
+  int *node_s = reinterpret_cast<int *>(lse_s + q_rows);
   // key `lane` of tile t: fetch reads its table entry, settle makes of it, a tile later, the pool row (or the drafted
   // token; -1: nothing there), so that no one waits for the table
   auto fetch = [&](int t) -> int {
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_weights_kernel(const We
     const int j = (t - cached_tiles) * kKeys + lane;
     return t < last && lane < kKeys && j < drafted ? rq.lo + j : -1;
   };
-  for (int q0 = 0; q0 < rows || q0 == 0; q0 += kQRows) {
+  for (int q0 = 0; q0 < rows || q0 == 0; q0 += q_rows) {
     int t_load = first + warp;
     int page = fetch(t_load);
     auto copy_next = [&](int stage) {
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_weights_kernel(const We
     for (int s = 0; s < kStages - 1; ++s) copy_next(s);
     // the query rows and their lse
     if (q0 > 0) __syncthreads();
-    const int here = min(rows - q0, kQRows), blocks = (here + 7) / 8;
+    const int here = min(rows - q0, q_rows), blocks = (here + 7) / 8;
     for (int i = threadIdx.x; i < blocks * 8 * kChunks; i += kWarps * 32) {
       const int r = i / kChunks, c = i % kChunks;
       uint4 v = make_uint4(0, 0, 0, 0);
@@ -494,15 +494,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (splits > 1) cluster_sync();  // nobody leaves while its sums are read
 }
 
-template <typename T, int D>
-int run_weights(const WeightParams &p, const qe_draft_batch &in, int64_t sum_keys, int max_tiles, cudaStream_t stream) {
-  auto kernel = attention_weights_kernel<T, D>;
-  constexpr int smem = weights_smem<D>();
+template <typename T, int D, int kStages>
+int run_weights(const WeightParams &p, const qe_draft_batch &in, int max_tiles, cudaStream_t stream) {
+  auto kernel = attention_weights_kernel<T, D, kStages>;
+  const int smem = weights_smem(D, p.q_rows);
   static std::atomic<bool> raised[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
   if (smem > 48 * 1024 && !raised[dev].load(std::memory_order_relaxed)) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         std::max(weights_smem(D, 16), weights_smem(D, kQRows)));
     if (e != cudaSuccess) return cuda_status(e, "qe_attention_weights: smem attribute");
     raised[dev].store(true, std::memory_order_relaxed);
   }
@@ -617,7 +618,8 @@ extern "C" int qe_attention_weights(const qe_attention_weights_args *args, void 
   const int max_tiles = std::max(1, (batch.max_length + kKeys - 1) / kKeys + (nodes + kKeys - 1) / kKeys);
   // tiles a CTA: the count that ends first by waves x (tiles + a start's 12), half a CTA more per request
   const int64_t all = (batch.sum_length + kKeys - 1) / kKeys + int64_t(batch.batch) * ((nodes + kKeys - 1) / kKeys);
-  const int64_t slots = 2 * int64_t(sm_count());
+  p.q_rows = int(std::min<int64_t>((int64_t(batch.max_nodes) * p.group + 7) / 8 * 8, kQRows));
+  const int64_t slots = int64_t(sm_count()) * std::min(8, 227 * 1024 / (weights_smem(head_dim, p.q_rows) + 1024));
   int64_t per = max_tiles, best = INT64_MAX;
   for (int64_t x = kWarps;; x = std::max(x + kWarps, x * 9 / 8 / kWarps * kWarps)) {
     x = std::min<int64_t>(x, max_tiles);
@@ -642,11 +644,17 @@ extern "C" int qe_attention_weights(const qe_attention_weights_args *args, void 
                           : run_weights_tc<__half, 64>(p, batch, nodes, st);
     return s ? s : ok();
   }
+  auto run = [&](auto t, auto d) {
+    using T = decltype(t);
+    constexpr int kD = decltype(d)::value;
+    return stages_for(p.q_rows) == 3 ? run_weights<T, kD, 3>(p, args->batch, max_tiles, st)
+                                     : run_weights<T, kD, 2>(p, args->batch, max_tiles, st);
+  };
+  using D64 = std::integral_constant<int, 64>;
+  using D128 = std::integral_constant<int, 128>;
   if (dtype == 1)
-    s = head_dim == 128 ? run_weights<__nv_bfloat16, 128>(p, batch, all, max_tiles, st)
-                        : run_weights<__nv_bfloat16, 64>(p, batch, all, max_tiles, st);
+    s = head_dim == 128 ? run(__nv_bfloat16{}, D128{}) : run(__nv_bfloat16{}, D64{});
   else
-    s = head_dim == 128 ? run_weights<__half, 128>(p, batch, all, max_tiles, st)
-                        : run_weights<__half, 64>(p, batch, all, max_tiles, st);
+    s = head_dim == 128 ? run(__half{}, D128{}) : run(__half{}, D64{});
   return s ? s : ok();
 }

@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
   constexpr int kSteps = D / 16;         // k-steps of Q K^T
   constexpr int kTileBytes = kKeys * kRow;
   constexpr int kCopies = kKeys * kChunks / 32;  // per lane and tile, K or V
-  static_assert((kWarps * (D + 2) + 2) * MT * 16 * 4 <= kWarps * kStages * 2 * kTileBytes, "the join fits the ring");
+  static_assert(MT * 16 * 4 * (kWarps * (D + 2) + 2) <= kWarps * kStages * 2 * kTileBytes, "the join fits the ring");
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, kvh = blockIdx.y % p.heads_kv, row0 = int(blockIdx.y / p.heads_kv) * (MT * 16);
@@ -963,65 +963,91 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
 }
 
-// Joins the splits of the requests that have more than one: a warp per (node, head) row. The lanes hold the splits'
-// factors, 32 at a time; the partial rows are read eight at a time (one after the other, 37 splits took 9 us).
-template <typename T, int D>
-__global__ void __launch_bounds__(256) tree_join_kernel(const TreeParams p) {
-  const int lane = threadIdx.x & 31;
+// Joins the splits of the requests that have more than one. kShare warps share a (node, head) row, its splits dealt out
+// to them in turn; a warp has eight splits' partial rows in flight. (One warp a row with 47 splits took 28 us from cold
+// caches, more than the attention itself.)
+constexpr int kJoinWarps = 8;
+
+template <typename T, int D, int kShare>
+__global__ void __launch_bounds__(kJoinWarps * 32) tree_join_kernel(const TreeParams p) {
+  constexpr int kPer = D / 32, kRows = kJoinWarps / kShare;  // columns per lane, rows per CTA
+  __shared__ float2 ml_s[kJoinWarps];
+  __shared__ float acc_s[kShare > 1 ? kJoinWarps : 1][D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % kShare;
   const int b = blockIdx.y;
-  const int at = int(blockIdx.x) * 8 + int(threadIdx.x >> 5);
+  const int at = int(blockIdx.x) * kRows + warp / kShare;
   grid_dep_wait();
   grid_dep_launch();
   const Request rq = request_of(p.batch, b);
-  if (at >= rq.n * p.heads_q) return;
   const int tiles = tiles_of(rq.len, p.k_draft ? rq.n : 0, p.key_tile);
   if (tiles <= p.tiles_per_cta) return;
   const int splits = min((tiles + p.tiles_per_cta - 1) / p.tiles_per_cta, p.splits);
+  const bool there = at < rq.n * p.heads_q;
   const int token = rq.lo + at / p.heads_q, head = at % p.heads_q;
   const int64_t row = int64_t(token) * p.heads_q + head, step = int64_t(p.batch.total) * p.heads_q;
-  const float2 none = make_float2(-INFINITY, 0.0f);
-  float2 ml = lane < splits ? p.part_ml[lane * step + row] : none;
-  float m_all = ml.x;
-  for (int s = 32 + lane; s < splits; s += 32) m_all = fmaxf(m_all, p.part_ml[s * step + row].x);
+  // this warp's splits: a running maximum and sums, as in the attention
+  float m = -INFINITY, l = 0.0f, acc[kPer] = {};
+  for (int s0 = share; there && s0 < splits; s0 += 8 * kShare) {
+    float2 ml[8], v[8][kPer / 2];
 #pragma unroll
-  for (int x = 16; x; x >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, x));
-  constexpr int kPer = D / 32;  // columns per lane
-  float acc[kPer] = {}, l_all = 0.0f;
-  for (int s0 = 0; s0 < splits; s0 += 32) {
-    if (s0 > 0) ml = s0 + lane < splits ? p.part_ml[(s0 + lane) * step + row] : none;
-    const float f = s0 + lane < splits ? join_factor(ml.x, m_all) : 0.0f;
-    l_all += f * ml.y;
-    const int here = min(splits - s0, 32);
-    for (int u0 = 0; u0 < here; u0 += 8) {
-      float2 v[8][kPer / 2];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float *src = p.part_o + ((s0 + min(u0 + u, here - 1)) * step + row) * D + lane * kPer;
+    for (int u = 0; u < 8; ++u) {
+      const int s = s0 + u * kShare;
+      ml[u] = make_float2(-INFINITY, 0.0f);
+      if (s < splits) {
+        ml[u] = p.part_ml[s * step + row];
+        const float *src = p.part_o + (s * step + row) * D + lane * kPer;
 #pragma unroll
         for (int e = 0; e < kPer / 2; ++e) v[u][e] = *reinterpret_cast<const float2 *>(src + 2 * e);
       }
+    }
+    float top = m;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float fu = __shfl_sync(0xffffffffu, f, (u0 + u) & 31);
-        if (u0 + u < here) {
+    for (int u = 0; u < 8; ++u) top = fmaxf(top, ml[u].x);
+    const float old = join_factor(m, top);
+    m = top;
+    l *= old;
 #pragma unroll
-          for (int e = 0; e < kPer / 2; ++e) {
-            acc[2 * e] += fu * v[u][e].x;
-            acc[2 * e + 1] += fu * v[u][e].y;
-          }
-        }
+    for (int e = 0; e < kPer; ++e) acc[e] *= old;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (s0 + u * kShare >= splits) continue;
+      const float f = join_factor(ml[u].x, m);
+      l += f * ml[u].y;
+#pragma unroll
+      for (int e = 0; e < kPer / 2; ++e) {
+        acc[2 * e] += f * v[u][e].x;
+        acc[2 * e + 1] += f * v[u][e].y;
       }
     }
   }
+  if (kShare > 1) {
+    if (lane == 0) ml_s[warp] = make_float2(m, l);
 #pragma unroll
-  for (int x = 16; x; x >>= 1) l_all += __shfl_xor_sync(0xffffffffu, l_all, x);
-  const float inv = l_all == 0.0f ? 0.0f : 1.0f / l_all;
+    for (int e = 0; e < kPer; ++e) acc_s[warp][lane * kPer + e] = acc[e];
+    __syncthreads();
+    if (share != 0) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kShare; ++w) m = fmaxf(m, ml_s[warp + w].x);
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kShare; ++w) {
+      const float f = join_factor(ml_s[warp + w].x, m);
+      l += f * ml_s[warp + w].y;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] += f * acc_s[warp + w][lane * kPer + e];
+    }
+  }
+  if (!there) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint32_t *dst = reinterpret_cast<uint32_t *>(p.out + int64_t(token) * p.out_token + int64_t(head) * p.out_head) +
                   lane * (kPer / 2);
 #pragma unroll
   for (int e = 0; e < kPer; e += 2) dst[e / 2] = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
   if (p.lse && lane == 0)
-    p.lse[int64_t(head) * p.batch.total + token] = l_all == 0.0f ? -INFINITY : (m_all + log2f(l_all)) * kLn2;
+    p.lse[int64_t(head) * p.batch.total + token] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------
@@ -1038,6 +1064,9 @@ struct TreePlan {
 };
 
 // More rows a K/V head than this take the tensor-memory kernel, whose row tile is 128 (the groups must fit it).
+#ifndef QE_TC_FIX
+#define QE_TC_FIX 4
+#endif
 #ifndef QE_TREE_TC_ROWS
 #define QE_TREE_TC_ROWS 32
 #endif
@@ -1058,7 +1087,7 @@ TreePlan tree_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head
   // half a CTA more per request for the last, shorter one. One wave for all took 64 requests of 313 to 8,191 tokens
   // from N to M us.
   const int64_t all = (in.sum_length + t.key_tile - 1) / t.key_tile + int64_t(in.batch) * tiles_of(0, in.max_nodes, t.key_tile);
-  const int64_t slots = (t.tc ? 1 : 2) * sm_count(), step = t.tc ? 1 : kWarps, fixed = t.tc ? 4 : 8;
+  const int64_t slots = (t.tc ? 1 : 2) * sm_count(), step = t.tc ? 1 : kWarps, fixed = t.tc ? QE_TC_FIX : 16;
   const int64_t ragged = in.batch > 1 ? in.batch / 2 : 0;
   int64_t per = max_tiles, best = INT64_MAX;
   for (int64_t x = step;; x = std::max(x + step, x * 9 / 8 / step * step)) {
@@ -1137,8 +1166,13 @@ int run_tree(const TreeParams &p, const TreePlan &t, const qe_draft_batch &in, c
     s = launch<tree_attention_kernel<T, D, 2>>(grid, t.cluster ? t.splits : 1, kWarps * 32, tree_smem_bytes<D, 2>(), stream, "qe_tree_attention launch", p);
   }
   if (s || t.splits == 1 || t.cluster) return s;
-  const dim3 join(unsigned((in.max_nodes * p.heads_q + 7) / 8), unsigned(in.batch));
-  return launch<tree_join_kernel<T, D>>(join, 1, 256, 0, stream, "qe_tree_attention join launch", p);
+  // as many warps a row as have eight splits each
+  const int share = t.splits > 32 ? 8 : t.splits > 8 ? 4 : 1, rows_cta = kJoinWarps / share;
+  const dim3 join(unsigned((in.max_nodes * p.heads_q + rows_cta - 1) / rows_cta), unsigned(in.batch));
+  const char *what = "qe_tree_attention join launch";
+  if (share == 8) return launch<tree_join_kernel<T, D, 8>>(join, 1, kJoinWarps * 32, 0, stream, what, p);
+  if (share == 4) return launch<tree_join_kernel<T, D, 4>>(join, 1, kJoinWarps * 32, 0, stream, what, p);
+  return launch<tree_join_kernel<T, D, 1>>(join, 1, kJoinWarps * 32, 0, stream, what, p);
 }
 
 bool al16(int64_t v) { return v % 16 == 0; }
