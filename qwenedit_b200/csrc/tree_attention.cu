@@ -539,10 +539,11 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
 // A CTA takes up to two tiles of 128 rows (the G heads of as many whole nodes as fit) of one K/V head and runs over
 // its share of the keys, 128 at a time: S = Q K^T, softmax in registers, O += P V with P from tensor memory.
 //   warps 0-7   softmax, one warpgroup per row tile, a thread per row (tensor-memory lane)
-//   warps 8-10  K and V tiles into two-stage rings: cached keys by cp.async through the block table (any page size;
-//               keys past the length or in bad pages read zeros; a TMA gather of four rows a lane took 10 us a tile),
-//               drafted keys through registers, because values that are not finite are taken out of V (0 x inf would
-//               reach the rows that do not see them) and put back at the end, for the rows that do
+//   warps 8-10  K and V tiles into two-stage rings. Full tiles of a pool whose pages are 8 to 128 rows (or whole
+//               multiples of 128) by TMA, a lane a page and 64 dims; other cached tiles by cp.async (any page size;
+//               keys past the length or in bad pages read zeros); drafted keys through registers, because values that
+//               are not finite are taken out of V (0 x inf would reach the rows that do not see them) and put back at
+//               the end, for the rows that do. (A TMA gather of four rows a lane took 10 us a tile.)
 //   warp 11     Q by TMA, tcgen05.mma (one thread), and the tensor memory: S0 | O0 | S1 | O1, P_t over S_t
 // The products of one thread execute in issue order, so P_t V(j) reads P_t(j) before Q_t K^T(j + 1) rewrites S_t, and
 // S_t(j + 1) being there means that O_t holds every product up to tile j.
@@ -580,7 +581,8 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const TreeParams p) {
+    tree_attention_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                             const __grid_constant__ CUtensorMap tm_v, const int page_boxes, const TreeParams p) {
   using S = TSmem<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -702,6 +704,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                      : "memory");
       }
     };
+    // Boxes of a tile: pages of box_rows rows, 64 dims each; a lane of warp 8 copies one (its table entry a tile ahead).
+    constexpr int kHalves = D / 64;
+    const int box_rows = min(p.batch.page_size, kTcTile), boxes = page_boxes ? kTcTile / box_rows * kHalves : 0;
+    const int box_page = lane / kHalves, box_half = lane % kHalves;
+    auto fetch_box = [&](int t) {
+      return me == 0 && lane < boxes && (t + 1) * kTcTile <= rq.len
+                 ? __ldg(p.batch.tables + int64_t(b) * p.batch.table_width +
+                         page_index(p.batch, t * kTcTile + box_page * box_rows))
+                 : 0;
+    };
+    int box = fetch_box(first), box_next = 0;
     // K 0, V 0, K 1, V 1, ...: a slot's barrier counts a thread when its copies have landed, nobody waits for them here
     fetch(first);
     for (int n = 0; n < 2 * n_tiles; ++n) {
@@ -710,6 +723,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (!v) {
         settle(t);
         fetch(t + 1);
+        box_next = fetch_box(t + 1);
+        if (me == 0 && lane < boxes && (box < 0 || box >= p.batch.pool_pages)) {
+          if (p.batch.err) atomicOr(p.batch.err, 1);
+          box = p.batch.pool_pages;  // outside the map: zeros
+        }
       }
       const bool ok = mbar_wait(bar((v ? tVEmpty : tKEmpty) + s), ((i >> 1) & 1) ^ 1, abort, p.batch.err);
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -717,10 +735,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (t >= cached_tiles) {
         copy_draft(v ? p.v_draft : p.k_draft, dst, (t - cached_tiles) * kTcTile, v);
         mbar_arrive(full);
+      } else if (boxes && (t + 1) * kTcTile <= rq.len) {
+        if (me == 0 && lane == 0)
+          mbar_expect_tx(full, S::tile);
+        else
+          mbar_arrive(full);
+        __syncwarp();
+        if (me == 0 && lane < boxes)
+          tma_load_4d(dst + box_half * S::half + box_page * box_rows * 128, v ? &tm_v : &tm_k, box_half * 64, kvh,
+                      t * kTcTile % p.batch.page_size, box, full);
       } else {
         copy_cached(v ? p.v_pool : p.k_pool, dst);
         cp_async_arrive(full);
       }
+      if (v) box = box_next;
     }
     cp_async_wait<0>();
   } else if (warp == 8 + kCopyWarps) {
@@ -1159,7 +1187,19 @@ int run_tree(const TreeParams &p, const TreePlan &t, const qe_draft_batch &in, c
     const uint64_t q_strides[2] = {uint64_t(p.q_head), uint64_t(p.q_token)};
     const uint32_t q_box[3] = {64, uint32_t(p.group), uint32_t(kTcTile / p.group)};
     if ((s = tensor_map_16bit("qe_tree_attention", &q, type, p.q, 3, q_dims, q_strides, q_box, "q"))) return s;
-    s = launch<tree_attention_tc_kernel<T, D>>(grid, 1, kTcThreads, TSmem<D>::bytes, stream, "qe_tree_attention launch", q, p);
+    CUtensorMap kv[2];
+    std::memset(kv, 0, sizeof(kv));
+    const int P = in.page_size;
+    const bool page_boxes = p.batch.table_width > 0 && in.max_length >= kTcTile && P >= 8 && (kTcTile % P == 0 || P % kTcTile == 0);
+    if (page_boxes) {
+      const uint64_t dims[4] = {uint64_t(D), uint64_t(p.heads_kv), uint64_t(P), uint64_t(p.batch.pool_pages)};
+      const uint64_t strides[3] = {uint64_t(D) * 2, uint64_t(p.pool_row), uint64_t(p.pool_row) * uint64_t(P)};
+      const uint32_t box[4] = {64, 1, uint32_t(std::min(P, kTcTile)), 1};
+      if ((s = tensor_map_16bit("qe_tree_attention", &kv[0], type, p.k_pool, 4, dims, strides, box, "the K plane"))) return s;
+      if ((s = tensor_map_16bit("qe_tree_attention", &kv[1], type, p.v_pool, 4, dims, strides, box, "the V plane"))) return s;
+    }
+    s = launch<tree_attention_tc_kernel<T, D>>(grid, 1, kTcThreads, TSmem<D>::bytes, stream, "qe_tree_attention launch", q, kv[0],
+                                               kv[1], int(page_boxes), p);
   } else if (t.m_tiles == 1) {
     s = launch<tree_attention_kernel<T, D, 1>>(grid, t.cluster ? t.splits : 1, kWarps * 32, tree_smem_bytes<D, 1>(), stream, "qe_tree_attention launch", p);
   } else {

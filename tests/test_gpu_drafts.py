@@ -128,6 +128,30 @@ def test_hidden_drafts_with_nan_and_infinities_do_not_show(bad, d, dtype, n):
         assert torch.isnan(out[i, 3:]).all() and torch.isnan(lse[3:, i]).all()
 
 
+@pytest.mark.parametrize("page", [2, 8, 32, 96, 128, 256])
+@pytest.mark.parametrize("n", [2, 50])
+def test_page_sizes(page, n):
+    """Pages inside a key tile, as long as one, over several, and sizes that fit none."""
+    lens = [1000, 255, 128, 5]
+    pool, slots, q, kn, vn = _case(lens, [n] * 4, 8, 2, 128, torch.bfloat16, page, page + n, layers=1)
+    out, lse = tree_attention(q, PagedBatch(pool, slots), DraftTree([n] * 4), 0, kn, vn, return_lse=True)
+    _compare(pool, slots, lens, [n] * 4, [R.chain(n)] * 4, q, kn, vn, out, lse, 0)
+    assert pool.device_errors() == 0
+
+
+def test_pages_outside_the_pool_with_many_rows():
+    lens, n = [700], 30
+    pool, slots, q, kn, vn = _case(lens, [n], 8, 2, 128, torch.bfloat16, 64, 3, layers=1)
+    cache = PagedBatch(pool, slots)
+    cache.tables[0, 1] = pool.rows // 64
+    cache.tables[0, 10] = -7
+    out, lse = tree_attention(q, cache, DraftTree([n]), 0, kn, vn, return_lse=True)
+    assert pool.device_errors() == 1
+    pool.kv[:, :, slots[0][64:128]] = 0
+    pool.kv[:, :, slots[0][640:]] = 0
+    _compare(pool, slots, lens, [n], [R.chain(n)], q, kn, vn, out, lse, 0)
+
+
 def test_scores_far_apart():
     """Maxima that grow by hundreds along the keys, and scores that vanish beside them."""
     pool, slots, q, kn, vn = _case([2000], [3], 8, 2, 64, torch.bfloat16, 16, 11)
