@@ -4,6 +4,7 @@
 // With the rows' log-sum-exp at hand a key's weight needs its own K row and all query rows, nothing of the other
 // keys: the keys are split over CTAs and warps, and nothing has to be joined.
 #include <algorithm>
+#include <array>
 #include <atomic>
 #include <climits>
 #include <cmath>
@@ -619,17 +620,24 @@ extern "C" int qe_attention_weights(const qe_attention_weights_args *args, void 
   // tiles a CTA: the count that ends first by waves x (tiles + a start's 12), half a CTA more per request
   const int64_t all = (batch.sum_length + kKeys - 1) / kKeys + int64_t(batch.batch) * ((nodes + kKeys - 1) / kKeys);
   p.q_rows = int(std::min<int64_t>((int64_t(batch.max_nodes) * p.group + 7) / 8 * 8, kQRows));
+  // (kept for the sizes asked for last on this thread: a model's layers ask for the same ones)
+  thread_local std::array<int64_t, 6> last{-1};
+  thread_local int64_t per = 0;
   const int64_t slots = int64_t(sm_count()) * std::min(8, 227 * 1024 / (weights_smem(head_dim, p.q_rows) + 1024));
-  int64_t per = max_tiles, best = INT64_MAX;
-  for (int64_t x = kWarps;; x = std::max(x + kWarps, x * 9 / 8 / kWarps * kWarps)) {
-    x = std::min<int64_t>(x, max_tiles);
-    const int64_t ctas = heads_kv * ((all + x - 1) / x + (x < max_tiles && batch.batch > 1 ? batch.batch / 2 : 0));
-    const int64_t cost = (ctas + slots - 1) / slots * (x + 12);
-    if (cost < best) {
-      best = cost;
-      per = x;
+  const std::array<int64_t, 6> now{all, max_tiles, heads_kv, batch.batch, slots, kWarps};
+  if (now != last) {
+    int64_t best = INT64_MAX;
+    for (int64_t x = kWarps;; x = std::max(x + kWarps, x * 9 / 8 / kWarps * kWarps)) {
+      x = std::min<int64_t>(x, max_tiles);
+      const int64_t ctas = heads_kv * ((all + x - 1) / x + (x < max_tiles && batch.batch > 1 ? batch.batch / 2 : 0));
+      const int64_t cost = (ctas + slots - 1) / slots * (x + 12);
+      if (cost < best) {
+        best = cost;
+        per = x;
+      }
+      if (x == max_tiles) break;
     }
-    if (x == max_tiles) break;
+    last = now;
   }
   p.tiles_per_cta = int(per);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -7,6 +7,7 @@
 // the keys; the keys are split over CTAs and warps, each with its own running maximum and sum, and joined at the end
 // by out = sum_w e^{m_w - m} O_w / sum_w e^{m_w - m} l_w.
 #include <algorithm>
+#include <array>
 #include <atomic>
 #include <climits>
 #include <cmath>
@@ -1100,7 +1101,7 @@ struct TreePlan {
 #endif
 constexpr int kTcRows = QE_TREE_TC_ROWS;
 
-TreePlan tree_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head_dim) {
+TreePlan make_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head_dim) {
   TreePlan t{};
   const int group = heads_q / heads_kv;
   const int64_t rows = int64_t(in.max_nodes) * group;
@@ -1146,6 +1147,20 @@ TreePlan tree_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head
   }
   if (t.splits > 1 && !t.cluster) t.workspace = int64_t(t.splits) * in.total * heads_q * (head_dim + 2) * 4;
   return t;
+}
+
+// The plan of the sizes asked for last on this thread (a model's layers ask for the same ones; the search takes a
+// microsecond).
+TreePlan tree_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head_dim) {
+  thread_local std::array<int64_t, 9> last{-1};
+  thread_local TreePlan plan;
+  const std::array<int64_t, 9> now{in.batch, in.total, in.max_nodes, in.max_length, in.sum_length,
+                                   heads_q,  heads_kv, head_dim,     sm_count()};
+  if (now != last) {
+    plan = make_plan(in, heads_q, heads_kv, head_dim);
+    last = now;
+  }
+  return plan;
 }
 
 template <auto kKernel, typename... Args>

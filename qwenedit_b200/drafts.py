@@ -58,10 +58,20 @@ class PagedBatch:
         table = np.full((self.batch, self.table_width), -1, np.int32)
         for i, (pages, _) in enumerate(tables):
             table[i, : len(pages)] = pages
-        self.tables = _to_device(table, pool.device)
+        self._tables = _to_device(table, pool.device)
         pool.h2d_bytes += table.nbytes
-        self.lengths = torch.zeros(self.batch, dtype=torch.int32, device=pool.device)
+        self._lengths = torch.zeros(self.batch, dtype=torch.int32, device=pool.device)
         self.set_lengths(self.room if lengths is None else lengths)
+
+    @property
+    def tables(self) -> torch.Tensor:
+        """[batch, table_width] int32 page ids on the device (in place only: the kernels keep reading this memory)."""
+        return self._tables
+
+    @property
+    def lengths(self) -> torch.Tensor:
+        """[batch] int32 cached tokens on the device (in place only; what a device-side loop may add to)."""
+        return self._lengths
 
     def set_lengths(self, lengths) -> None:
         """The cached tokens of each request from now on (on the current stream), at most its slots."""
@@ -100,17 +110,27 @@ class DraftTree:
             raise ValueError("too many nodes")
         self._host_starts = starts
         self.total, self.max_nodes = int(starts[-1]), max(self.counts, default=0)
-        self.starts = _to_device(starts.astype(np.int32), self.device)
-        self.mode, self.masks, self.words = (self.FULL if full else self.CHAIN), None, 0
+        self._starts = _to_device(starts.astype(np.int32), self.device)
+        self.mode, self._masks, self.words = (self.FULL if full else self.CHAIN), None, 0
         self._err = None
         self._view = None
         if parents is not None or visible is not None:
             self.mode, self.words = self.MASKS, max(1, -(-self.max_nodes // 32))
-            self.masks = torch.zeros(self.total, self.words, dtype=torch.int32, device=self.device)
+            self._masks = torch.zeros(self.total, self.words, dtype=torch.int32, device=self.device)
         if parents is not None:
             self.set_parents(parents)
         if visible is not None:
             self._set_visible(visible)
+
+    @property
+    def starts(self) -> torch.Tensor:
+        """[batch + 1] int32: the first node of each request, on the device (in place only)."""
+        return self._starts
+
+    @property
+    def masks(self) -> torch.Tensor | None:
+        """[total, words] int32 bit masks on the device (in place only); None for a chain or `full`."""
+        return self._masks
 
     def set_parents(self, parents) -> None:
         """Another tree of the same counts: rebuilds the masks in place, one launch on the current stream (with a
@@ -164,22 +184,19 @@ class DraftTree:
 
 
 class _View:
-    """The C view of a cache and a tree (``qe_draft_batch`` as bytes), the workspace sizes asked of it, and the tensor
-    layouts that its calls have checked."""
+    """The C view of a cache and a tree (``qe_draft_batch`` as bytes), and what the calls made with them have checked and
+    worked out, by the layouts of their tensors."""
 
-    __slots__ = ("cache", "batch", "workspace", "checked")
+    __slots__ = ("cache", "batch", "plans")
 
     def __init__(self, cache, batch):
-        self.cache, self.batch, self.workspace, self.checked = cache, batch, {}, {}
+        self.cache, self.batch, self.plans = cache, batch, {}
 
-    def check(self, name: str, t: torch.Tensor, n: int, heads: int, head_dim: int, dtype, device) -> tuple:
-        """The strides of a [tokens, heads, head_dim] tensor, after checks that equal layouts pass without repeating."""
-        stride = t.stride()
-        layout = (t.shape, stride, t.dtype, t.device, heads)
-        if self.checked.get(name) != layout:
-            _check_rows(name, t, n, heads, head_dim, dtype, device)
-            self.checked[name] = layout
-        return stride
+    def keep(self, key, plan):
+        if len(self.plans) >= 1024:  # a program whose layouts never repeat
+            self.plans.clear()
+        self.plans[key] = plan
+        return plan
 
 
 def _view(cache: PagedBatch, tree: DraftTree) -> _View:
@@ -229,44 +246,62 @@ def tree_attention(q: torch.Tensor, cache: PagedBatch, tree: DraftTree, layer: i
     [T, Hq, D], and with `return_lse` the log-sum-exp [Hq, tree.total] fp32 of the scaled scores, which
     ``evict.attention_weights`` takes. A token that sees nothing gets zeros and -inf; rows of `out` past the tree's
     are left as they were (zeros where the call makes `out`). Runs on the current stream, without synchronising."""
-    pool = _check_pool(cache, layer)
-    kv, device, heads_kv, d = pool.kv, pool.device, pool.heads, pool.head_dim
-    dtype = kv.dtype
-    if q.dim() != 3 or q.shape[1] % heads_kv or q.shape[1] == 0:
-        raise ValueError(f"q must be [tokens, heads, {d}], its heads a multiple of the pool's {heads_kv}")
-    if (k_draft is None) != (v_draft is None):
-        raise ValueError("k_draft and v_draft go together")
-    view, total, heads_q = _view(cache, tree), tree.total, q.shape[1]
-    qs = view.check("q", q, total, heads_q, d, dtype, device)
-    draft = (0, 0, 0, 0)
-    if k_draft is not None:
-        ks = view.check("k_draft", k_draft, total, heads_kv, d, dtype, device)
-        if view.check("v_draft", v_draft, total, heads_kv, d, dtype, device) != ks:
-            raise ValueError("k_draft and v_draft must have the same strides")
-        draft = (k_draft.data_ptr(), v_draft.data_ptr(), 2 * ks[0], 2 * ks[1])
+    view = tree._view
+    if view is None or view.cache is not cache:
+        view = _view(cache, tree)
+    key = (layer, scale, q.shape, q.stride(), q.dtype, q.device,
+           None if k_draft is None else (k_draft.shape, k_draft.stride(), k_draft.dtype, k_draft.device),
+           None if v_draft is None else (v_draft.shape, v_draft.stride(), v_draft.dtype, v_draft.device),
+           None if out is None else (out.shape, out.stride(), out.dtype, out.device))
+    plan = view.plans.get(key)
+    if plan is None:
+        plan = view.keep(key, _TreePlan(view, tree, layer, q, k_draft, v_draft, scale, out))
     if out is None:
-        make = torch.empty if q.shape[0] == total else torch.zeros
-        out = make(q.shape, dtype=dtype, device=device)
-    os = view.check("out", out, total, heads_q, d, dtype, device)
-    lse = torch.empty((heads_q, total), dtype=torch.float32, device=device) if return_lse else None
-    if scale is None:
-        scale = 1.0 / math.sqrt(d)
-    plane = kv.data_ptr() + 2 * layer * kv.stride(0)
+        out = (torch.empty_like if plan.exact else torch.zeros_like)(q, memory_format=torch.contiguous_format)
+    device, plane = plan.device, cache.pool.kv.data_ptr() + plan.plane
+    lse = torch.empty_strided(plan.lse, plan.lse_strides, dtype=torch.float32, device=device) if return_lse else None
     with _lib.on_device(device):
-        size = view.workspace.get((heads_q, heads_kv, d))
-        if size is None:
-            size = view.workspace[heads_q, heads_kv, d] = _workspace_bytes(view, heads_q, heads_kv, d)
-        work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        args = view.batch + _lib.TREE_ATTENTION.pack(
-            q.data_ptr(), 2 * qs[0], 2 * qs[1], plane, plane + 2 * kv.stride(1), pool.rows, *draft, out.data_ptr(),
-            2 * os[0], 2 * os[1], 0 if lse is None else lse.data_ptr(), 0 if work is None else work.data_ptr(), size,
-            pool._err.data_ptr(), heads_q, heads_kv, d, DTYPES[dtype], scale)
+        work = torch.empty(plan.work, dtype=torch.uint8, device=device) if plan.work else None
+        args = plan.head + _TREE.pack(
+            q.data_ptr(), *plan.q, plane, plane + plan.to_v, plan.rows, 0 if k_draft is None else k_draft.data_ptr(),
+            0 if v_draft is None else v_draft.data_ptr(), *plan.draft, out.data_ptr(), *plan.out,
+            0 if lse is None else lse.data_ptr(), 0 if work is None else work.data_ptr(), *plan.tail)
         _lib.call("qe_tree_attention", args, _lib.stream_of(device))
     return (out, lse) if return_lse else out
 
 
-def _workspace_bytes(view: _View, heads_q: int, heads_kv: int, d: int) -> int:
-    out = ctypes.c_int64()
-    args = view.batch + _lib.TREE_ATTENTION.pack(*[0] * 17, heads_q, heads_kv, d, 1, 1.0)
-    _lib.call("qe_tree_attention_workspace", args, ctypes.byref(out))
-    return out.value
+_TREE = _lib.TREE_ATTENTION
+
+
+class _TreePlan:
+    """The checked layouts of a ``tree_attention`` call as the numbers its C arguments need."""
+
+    def __init__(self, view, tree, layer, q, k_draft, v_draft, scale, out):
+        pool = _check_pool(view.cache, layer)
+        kv, device, heads_kv, d = pool.kv, pool.device, pool.heads, pool.head_dim
+        if q.dim() != 3 or q.shape[1] % heads_kv or q.shape[1] == 0:
+            raise ValueError(f"q must be [tokens, heads, {d}], its heads a multiple of the pool's {heads_kv}")
+        if (k_draft is None) != (v_draft is None):
+            raise ValueError("k_draft and v_draft go together")
+        total, heads_q = tree.total, q.shape[1]
+        _check_rows("q", q, total, heads_q, d, kv.dtype, device)
+        self.draft = (0, 0)
+        if k_draft is not None:
+            _check_rows("k_draft", k_draft, total, heads_kv, d, kv.dtype, device)
+            _check_rows("v_draft", v_draft, total, heads_kv, d, kv.dtype, device)
+            if k_draft.stride() != v_draft.stride():
+                raise ValueError("k_draft and v_draft must have the same strides")
+            self.draft = (2 * k_draft.stride(0), 2 * k_draft.stride(1))
+        if out is not None:
+            _check_rows("out", out, total, heads_q, d, kv.dtype, device)
+        self.device, self.exact, self.head = device, q.shape[0] == total, view.batch
+        self.q, self.rows = (2 * q.stride(0), 2 * q.stride(1)), pool.rows
+        self.plane, self.to_v = 2 * layer * kv.stride(0), 2 * kv.stride(1)
+        self.out = (2 * heads_q * d, 2 * d) if out is None else (2 * out.stride(0), 2 * out.stride(1))
+        self.lse, self.lse_strides = (heads_q, total), (total, 1)
+        heads = (heads_q, heads_kv, d, DTYPES[kv.dtype])
+        size = ctypes.c_int64()
+        with _lib.on_device(device):
+            _lib.call("qe_tree_attention_workspace", view.batch + _TREE.pack(*[0] * 17, *heads, 1.0), ctypes.byref(size))
+        self.work = size.value
+        self.tail = (size.value, pool._err.data_ptr(), *heads, 1.0 / math.sqrt(d) if scale is None else float(scale))

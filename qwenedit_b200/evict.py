@@ -19,7 +19,7 @@ import math
 import torch
 
 from qwenedit_b200 import _lib
-from qwenedit_b200.drafts import DTYPES, DraftTree, PagedBatch, _check_pool, _view
+from qwenedit_b200.drafts import DTYPES, DraftTree, PagedBatch, _check_pool, _check_rows, _view
 
 
 def attention_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedBatch, tree: DraftTree, layer: int = 0,
@@ -36,45 +36,64 @@ def attention_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedBatch, tre
     Returns `out` [B, Hkv, W] fp32, by default as wide as the longest request needs: its slots, and with `k_draft` the
     tree's largest count. With `accumulate` the weights are added to what `out` holds (positions past a request's
     keys stay); else those positions get 0. The same inputs give the same bits. One launch on the current stream."""
-    pool = _check_pool(cache, layer)
-    kv, device, heads_kv, d = pool.kv, pool.device, pool.heads, pool.head_dim
-    dtype = kv.dtype
-    if q.dim() != 3 or q.shape[1] % heads_kv or q.shape[1] == 0:
-        raise ValueError(f"q must be [tokens, heads, {d}], its heads a multiple of the pool's {heads_kv}")
-    view, total, heads_q = _view(cache, tree), tree.total, q.shape[1]
-    qs = view.check("q", q, total, heads_q, d, dtype, device)
-    draft = (0, 0, 0)
-    width = cache.max_length
-    if k_draft is not None:
-        ks = view.check("k_draft", k_draft, total, heads_kv, d, dtype, device)
-        draft = (k_draft.data_ptr(), 2 * ks[0], 2 * ks[1])
-        width += tree.max_nodes
-    if lse.device != device or lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[0] != heads_q or \
-            lse.shape[1] < total or (lse.shape[1] > 1 and lse.stride(1) != 1):
-        raise ValueError(f"lse must be [{heads_q}, at least {total}] float32 on {device} with contiguous rows")
+    view = tree._view
+    if view is None or view.cache is not cache:
+        view = _view(cache, tree)
+    key = (layer, scale, accumulate, q.shape, q.stride(), q.dtype, q.device, lse.shape, lse.stride(), lse.dtype, lse.device,
+           None if k_draft is None else (k_draft.shape, k_draft.stride(), k_draft.dtype, k_draft.device),
+           None if out is None else (out.shape, out.stride(), out.dtype, out.device))
+    plan = view.plans.get(key)
+    if plan is None:
+        plan = view.keep(key, _WeightsPlan(view, tree, layer, q, lse, k_draft, scale, out, accumulate))
+    device = plan.device
     if out is None:
-        if accumulate:
-            raise ValueError("accumulate needs `out`")
-        out = torch.empty((cache.batch, heads_kv, width), dtype=torch.float32, device=device)
-        os = (heads_kv * width, width)
-    else:
-        os = out.stride()
-        if out.device != device or out.dtype != torch.float32 or out.dim() != 3 or out.shape[0] != cache.batch or \
-                out.shape[1] != heads_kv or out.shape[2] < width or (out.shape[2] > 1 and os[2] != 1):
-            raise ValueError(f"out must be [{cache.batch}, {heads_kv}, at least {width}] float32 on {device} with "
-                             "contiguous rows")
-        width = out.shape[2]
-        if (cache.batch > 1 and abs(os[0]) < width) or (heads_kv > 1 and abs(os[1]) < width):
-            raise ValueError("out must not have rows that overlap")
-    if scale is None:
-        scale = 1.0 / math.sqrt(d)
+        out = torch.empty(plan.shape, dtype=torch.float32, device=device)
     with _lib.on_device(device):
-        args = view.batch + _lib.ATTENTION_WEIGHTS.pack(
-            q.data_ptr(), 2 * qs[0], 2 * qs[1], kv.data_ptr() + 2 * layer * kv.stride(0), pool.rows, *draft,
-            lse.data_ptr(), lse.stride(0), out.data_ptr(), os[0], os[1], width, pool._err.data_ptr(), heads_q, heads_kv,
-            d, DTYPES[dtype], 1 if accumulate else 0, scale)
+        args = plan.head + _WEIGHTS.pack(q.data_ptr(), *plan.q, cache.pool.kv.data_ptr() + plan.plane, plan.rows,
+                                         0 if k_draft is None else k_draft.data_ptr(), *plan.draft, lse.data_ptr(), plan.lse, out.data_ptr(), *plan.tail)
         _lib.call("qe_attention_weights", args, _lib.stream_of(device))
     return out
+
+
+_WEIGHTS = _lib.ATTENTION_WEIGHTS
+
+
+class _WeightsPlan:
+    """The checked layouts of an ``attention_weights`` call as the numbers its C arguments need."""
+
+    def __init__(self, view, tree, layer, q, lse, k_draft, scale, out, accumulate):
+        cache = view.cache
+        pool = _check_pool(cache, layer)
+        kv, device, heads_kv, d = pool.kv, pool.device, pool.heads, pool.head_dim
+        if q.dim() != 3 or q.shape[1] % heads_kv or q.shape[1] == 0:
+            raise ValueError(f"q must be [tokens, heads, {d}], its heads a multiple of the pool's {heads_kv}")
+        total, heads_q, width = tree.total, q.shape[1], cache.max_length
+        _check_rows("q", q, total, heads_q, d, kv.dtype, device)
+        self.draft = (0, 0)
+        if k_draft is not None:
+            _check_rows("k_draft", k_draft, total, heads_kv, d, kv.dtype, device)
+            self.draft = (2 * k_draft.stride(0), 2 * k_draft.stride(1))
+            width += tree.max_nodes
+        if lse.device != device or lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[0] != heads_q or \
+                lse.shape[1] < total or (lse.shape[1] > 1 and lse.stride(1) != 1):
+            raise ValueError(f"lse must be [{heads_q}, at least {total}] float32 on {device} with contiguous rows")
+        if out is None:
+            if accumulate:
+                raise ValueError("accumulate needs `out`")
+            strides = (heads_kv * width, width)
+        else:
+            strides = out.stride()
+            if out.device != device or out.dtype != torch.float32 or out.dim() != 3 or out.shape[0] != cache.batch or \
+                    out.shape[1] != heads_kv or out.shape[2] < width or (out.shape[2] > 1 and strides[2] != 1):
+                raise ValueError(f"out must be [{cache.batch}, {heads_kv}, at least {width}] float32 on {device} with "
+                                 "contiguous rows")
+            width = out.shape[2]
+            if (cache.batch > 1 and abs(strides[0]) < width) or (heads_kv > 1 and abs(strides[1]) < width):
+                raise ValueError("out must not have rows that overlap")
+        self.device, self.head, self.shape, self.lse = device, view.batch, (cache.batch, heads_kv, width), lse.stride(0)
+        self.q, self.plane, self.rows = (2 * q.stride(0), 2 * q.stride(1)), 2 * layer * kv.stride(0), pool.rows
+        self.tail = (strides[0], strides[1], width, pool._err.data_ptr(), heads_q, heads_kv, d, DTYPES[kv.dtype],
+                     1 if accumulate else 0, 1.0 / math.sqrt(d) if scale is None else float(scale))
 
 
 def heaviest(weights: torch.Tensor, budget: int, lengths: torch.Tensor | None = None, sinks: int = 0,
@@ -103,8 +122,8 @@ def heaviest(weights: torch.Tensor, budget: int, lengths: torch.Tensor | None = 
             lengths = lengths.broadcast_to(lead).contiguous()
     n = [1] * (3 - len(lead)) + list(lead)
     s = [0] * (3 - len(lead)) + list(weights.stride()[:-1])
-    keep = torch.empty(*lead, budget, dtype=torch.int32, device=weights.device)
-    kept = torch.empty(*lead, budget, dtype=torch.float32, device=weights.device)
+    keep = torch.empty((*lead, budget), dtype=torch.int32, device=weights.device)
+    kept = torch.empty_like(keep, dtype=torch.float32)
     with _lib.on_device(weights.device):
         _lib.call("qe_heaviest", weights.data_ptr(), *n, *s, weights.shape[-1],
                   None if lengths is None else lengths.data_ptr(), budget, sinks, recent, keep.data_ptr(),
