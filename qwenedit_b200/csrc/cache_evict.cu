@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
   if (need == 0) return;
   uint32_t prefix = 0;  // the threshold key's bits found so far
   int at_all = 0;       // positions whose key starts with them
+  int low = 0;          // bits below them
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
@@ -137,10 +138,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
     int *hist = hists[pass];
     if (pass == 0) __syncthreads();
     each([&](uint32_t k, int) {  // no position: a key below every real one, counted where no threshold can be
-      if (pass == 0)
-        atomicAdd(&hist[k >> 21], 1);
-      else if ((k >> (shift + kBits[pass])) == prefix)
-        atomicAdd(&hist[(k >> shift) & ((1u << kBits[pass]) - 1u)], 1);
+      // every lane adds, those of other prefixes nothing: no branch, and low digits seldom meet
+      atomicAdd(&hist[(k >> shift) & ((1u << kBits[pass]) - 1u)],
+                pass == 0 || (k >> (shift + kBits[pass])) == prefix ? 1 : 0);
     });
     __syncthreads();
     // the digit at which the count from the top reaches `need`: thread t sums counters kBins - 1 - kPer t and below
@@ -171,15 +171,23 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
     prefix = (prefix << kBits[pass]) | uint32_t(found[0]);
     need -= found[1];
     at_all = found[2];
+    low = shift;
+    if (need == at_all) break;  // all of this digit: the lower bits do not matter
   }
   // Kept: the positions above the threshold and the first `need` of the at_all at it. Without ties to cut those are
   // the keys of at least the threshold; else the positions at it are counted apart.
   const bool cut = need < at_all;
+  const uint32_t threshold = prefix << low, least = cut ? threshold + 1 : threshold;  // a cut threshold is a whole key
   int above = 0, at = 0;
-  each([&](uint32_t k, int) {
-    above += __popc(__ballot_sync(0xffffffffu, cut ? k > prefix : k >= prefix));
-    if (cut) at += __popc(__ballot_sync(0xffffffffu, k == prefix));
-  });
+  if (cut)
+    each([&](uint32_t k, int) {
+      above += k >= least;
+      at += k == threshold;
+    });
+  else
+    each([&](uint32_t k, int) { above += k >= least; });
+  above = __reduce_add_sync(0xffffffffu, above);
+  at = __reduce_add_sync(0xffffffffu, at);
   if (lane == 0) {
     warp_sum[warp] = above;
     warp_at[warp] = at;
@@ -189,14 +197,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
   at = before_warp(warp_at);
   const uint32_t below = (1u << lane) - 1u;
   each([&](uint32_t k, int i) {
-    const uint32_t up = __ballot_sync(0xffffffffu, cut ? k > prefix : k >= prefix);
-    bool take = (up >> lane) & 1u;
+    bool take = k >= least;
+    const uint32_t up = __ballot_sync(0xffffffffu, take);
     int place = above + __popc(up & below);
     above += __popc(up);
     if (cut) {
-      const uint32_t eq = __ballot_sync(0xffffffffu, k == prefix);
+      const uint32_t eq = __ballot_sync(0xffffffffu, k == threshold);
       const int mine = at + __popc(eq & below);
-      take = take || (((eq >> lane) & 1u) && mine < need);
+      take = take || (k == threshold && mine < need);
       place += min(mine, need);
       at += __popc(eq);
     }
