@@ -846,9 +846,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     };
     float m_use = -INFINITY, l = 0.0f;
     bool ok = true;
+    const bool idle = !__any_sync(0xffffffffu, mine);  // no row of the warp is used: what P holds there reaches no other
     for (int i = 0; i < n_tiles; ++i) {
       ok = __all_sync(0xffffffffu, mbar_wait(bar(tSFull + t), i & 1, abort, p.batch.err));
       if (!ok) break;
+      if (idle) {
+        if (lane == 0) mbar_arrive(bar(tPReady + t));
+        continue;
+      }
       tc_fence_after();
       const int at = first + i;
       const bool masked = at >= cached_tiles || (at + 1) * kTcTile > rq.len;  // the same for the whole CTA
@@ -858,6 +863,43 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int c = 0; c < 4; ++c) bits[c] = bits32(at, c);
       }
       uint32_t buf[2][32];
+      // One pass where every row has a reference maximum already: p = 2^(s scale - m_use) without looking for the
+      // tile's maximum. If a row's 128 weights then sum to more than 128 x 2^8 its maximum has grown past 2^8: nothing
+      // has been stored yet, and the tile goes through the two passes below (p stays below 2^15 otherwise).
+      if (__all_sync(0xffffffffu, m_use != -INFINITY || !mine)) {
+        const f32x2 scale2 = pk2(p.scale_log2, p.scale_log2), base2 = pk2(mine ? -m_use : 0.0f, mine ? -m_use : 0.0f);
+        f32x2 sum[2] = {pk2(0.0f, 0.0f), pk2(0.0f, 0.0f)};
+        uint32_t w[4][16];
+        tmem_ld32_async(s_col, buf[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_ld_wait(buf[c & 1]);
+          if (c + 1 < 4) tmem_ld32_async(s_col + 32 * (c + 1), buf[(c + 1) & 1]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 x = up2(fma2(pk2(__uint_as_float(buf[c & 1][2 * e]), __uint_as_float(buf[c & 1][2 * e + 1])), scale2, base2));
+            float y0 = ex2(x.x), y1 = ex2(x.y);
+            if (masked) {
+              y0 = (bits[c] >> (2 * e)) & 1u ? y0 : 0.0f;
+              y1 = (bits[c] >> (2 * e + 1)) & 1u ? y1 : 0.0f;
+            }
+            sum[e & 1] = add2(sum[e & 1], pk2(y0, y1));
+            w[c][e] = pack2<T>(y0, y1);
+          }
+        }
+        const float2 a = up2(add2(sum[0], sum[1]));
+        const float add = a.x + a.y;
+        if (!__any_sync(0xffffffffu, mine && add > 128.0f * 256.0f)) {
+          l += add;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_st16(s_col + 16 * c, w[c]);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(tPReady + t));
+          continue;
+        }
+      }
       // the row's maximum over the visible keys; the columns are read again for the exponentials
       float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       tmem_ld32_async(s_col, buf[0]);
@@ -937,6 +979,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int token = rq.lo + node, head = kvh * p.group + r - dn * p.group;
       const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
       const bool put_back = drafts && *odd;
+      float *turn = reinterpret_cast<float *>(smem + S::k) + warp * 32 * 33;  // the K tiles are done with
       char *dst = p.out + int64_t(token) * p.out_token + int64_t(head) * p.out_head;
       const int64_t part = (int64_t(blockIdx.x) * p.batch.total + token) * p.heads_q + head;
 #pragma unroll
@@ -945,35 +988,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
         tmem_ld32_async(o_col + 32 * c, w);
         tmem_ld_wait(w);
-        if (!mine) continue;
-        float o[32];
+        if (mine) {
+          float o[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : __uint_as_float(w[e]);  // no key seen: O may be unwritten
-        if (put_back) {
-          for (int j = max(first - cached_tiles, 0) * kTcTile; j < min(rq.n, (first + n_tiles - cached_tiles) * kTcTile); ++j) {
-            if (!((bits32(cached_tiles + j / kTcTile, j % kTcTile / 32) >> (j & 31)) & 1u)) continue;
-            const T *v = reinterpret_cast<const T *>(p.v_draft + int64_t(rq.lo + j) * p.draft_token + int64_t(kvh) * p.draft_head) + 32 * c;
+          for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : __uint_as_float(w[e]);  // no key seen: O may be unwritten
+          if (put_back) {
+            for (int j = max(first - cached_tiles, 0) * kTcTile; j < min(rq.n, (first + n_tiles - cached_tiles) * kTcTile); ++j) {
+              if (!((bits32(cached_tiles + j / kTcTile, j % kTcTile / 32) >> (j & 31)) & 1u)) continue;
+              const T *v = reinterpret_cast<const T *>(p.v_draft + int64_t(rq.lo + j) * p.draft_token + int64_t(kvh) * p.draft_head) + 32 * c;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float x = to_float(v[e]);
-              if (!(fabsf(x) < INFINITY)) o[e] += x;
+              for (int e = 0; e < 32; ++e) {
+                const float x = to_float(v[e]);
+                if (!(fabsf(x) < INFINITY)) o[e] += x;
+              }
             }
           }
-        }
-        if (whole) {
+          if (whole) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint4 x;
-            x.x = pack2<T>(o[e] * inv, o[e + 1] * inv);
-            x.y = pack2<T>(o[e + 2] * inv, o[e + 3] * inv);
-            x.z = pack2<T>(o[e + 4] * inv, o[e + 5] * inv);
-            x.w = pack2<T>(o[e + 6] * inv, o[e + 7] * inv);
-            *reinterpret_cast<uint4 *>(dst + (32 * c + e) * 2) = x;
+            for (int e = 0; e < 32; e += 8) {
+              uint4 x;
+              x.x = pack2<T>(o[e] * inv, o[e + 1] * inv);
+              x.y = pack2<T>(o[e + 2] * inv, o[e + 3] * inv);
+              x.z = pack2<T>(o[e + 4] * inv, o[e + 5] * inv);
+              x.w = pack2<T>(o[e + 6] * inv, o[e + 7] * inv);
+              *reinterpret_cast<uint4 *>(dst + (32 * c + e) * 2) = x;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) turn[lane * 33 + e] = o[e];
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4 *>(p.part_o + part * D + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+        if (!whole) {  // by rows: a warp writes 32 columns of one at a time (a lane its own row: 3.8 us for two tiles)
+          __syncwarp();
+          const uint32_t rows_used = __ballot_sync(0xffffffffu, mine);
+#pragma unroll 8
+          for (int x = 0; x < 32; ++x) {
+            const int64_t to = __shfl_sync(0xffffffffu, part, x);
+            if ((rows_used >> x) & 1u) p.part_o[to * D + 32 * c + lane] = turn[x * 33 + lane];
+          }
+          __syncwarp();
         }
       }
       if (mine) {
@@ -1178,15 +1231,14 @@ int launch(dim3 grid, int cluster, int threads, int smem, cudaStream_t stream, c
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  if (smem > 48 * 1024) {
-    static std::atomic<bool> raised[64];  // per device
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    if (!raised[dev].load(std::memory_order_relaxed)) {
-      cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      if (e != cudaSuccess) return cuda_status(e, what);
-      raised[dev].store(true, std::memory_order_relaxed);
-    }
+  static std::atomic<bool> raised[64];  // per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  if (!raised[dev].load(std::memory_order_relaxed)) {
+    cudaError_t e = cudaSuccess;
+    if (smem > 48 * 1024) e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_status(e, what);
+    raised[dev].store(true, std::memory_order_relaxed);
   }
   return cuda_status(cudaLaunchKernelEx(&cfg, kKernel, args...), what);
 }
