@@ -863,8 +863,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int c = 0; c < 4; ++c) bits[c] = bits32(at, c);
       }
       uint32_t buf[2][32];
-      // One pass where every row has a reference maximum already: p = 2^(s scale - m_use) without looking for the
-      // tile's maximum. If a row's 128 weights then sum to more than 128 x 2^8 its maximum has grown past 2^8: nothing
+      // A row without a reference maximum yet takes that of the tile's first 32 keys.
+      if (__any_sync(0xffffffffu, mine && m_use == -INFINITY)) {
+        const uint32_t see = bits[0];
+        tmem_ld32_async(s_col, buf[0]);
+        tmem_ld_wait(buf[0]);
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 32; ++e) top[e & 1] = (see >> e) & 1u ? fmaxf(top[e & 1], __uint_as_float(buf[0][e])) : top[e & 1];
+        if (m_use == -INFINITY) m_use = fmaxf(top[0], top[1]) * p.scale_log2;  // its O and l are still 0
+      }
+      // One pass where every row has a reference maximum: p = 2^(s scale - m_use) without looking for the tile's
+      // maximum. If a row's 128 weights then sum to more than 128 x 2^8 its maximum has grown past 2^8: nothing
       // has been stored yet, and the tile goes through the two passes below (p stays below 2^15 otherwise).
       if (__all_sync(0xffffffffu, m_use != -INFINITY || !mine)) {
         const f32x2 scale2 = pk2(p.scale_log2, p.scale_log2), base2 = pk2(mine ? -m_use : 0.0f, mine ? -m_use : 0.0f);
@@ -979,7 +989,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int token = rq.lo + node, head = kvh * p.group + r - dn * p.group;
       const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
       const bool put_back = drafts && *odd;
-      float *turn = reinterpret_cast<float *>(smem + S::k) + warp * 32 * 33;  // the K tiles are done with
+      float *turn = reinterpret_cast<float *>(smem + S::k) + warp * 32 * 36;  // the K tiles are done with
       char *dst = p.out + int64_t(token) * p.out_token + int64_t(head) * p.out_head;
       const int64_t part = (int64_t(blockIdx.x) * p.batch.total + token) * p.heads_q + head;
 #pragma unroll
@@ -1015,16 +1025,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) turn[lane * 33 + e] = o[e];
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4 *>(turn + lane * 36 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
-        if (!whole) {  // by rows: a warp writes 32 columns of one at a time (a lane its own row: 3.8 us for two tiles)
+        if (!whole) {  // four rows' 128 bytes at a time (a lane its own row: 3.8 us for two row tiles)
           __syncwarp();
-          const uint32_t rows_used = __ballot_sync(0xffffffffu, mine);
-#pragma unroll 8
-          for (int x = 0; x < 32; ++x) {
-            const int64_t to = __shfl_sync(0xffffffffu, part, x);
-            if ((rows_used >> x) & 1u) p.part_o[to * D + 32 * c + lane] = turn[x * 33 + lane];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const int from = x * 4 + lane / 8;
+            const int64_t to = __shfl_sync(0xffffffffu, mine ? part : int64_t(-1), from);
+            const float4 v = *reinterpret_cast<const float4 *>(turn + from * 36 + (lane & 7) * 4);
+            if (to >= 0) *reinterpret_cast<float4 *>(p.part_o + to * D + 32 * c + (lane & 7) * 4) = v;
           }
           __syncwarp();
         }
