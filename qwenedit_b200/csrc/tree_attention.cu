@@ -547,13 +547,15 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
 //               the end, for the rows that do. (A TMA gather of four rows a lane took 10 us a tile.)
 //   warp 11     Q by TMA, tcgen05.mma (one thread), and the tensor memory: S0 | O0 | S1 | O1, P_t over S_t
 // The products of one thread execute in issue order, so P_t V(j) reads P_t(j) before Q_t K^T(j + 1) rewrites S_t, and
-// S_t(j + 1) being there means that O_t holds every product up to tile j.
+// S_t(j + 1) being there means that O_t holds every product up to tile j. A single row tile has both S buffers: the next
+// key tile's Q K^T runs under the softmax of this one (8 requests of 5 nodes over 701 to 6,007: 27.0 -> 26.6 us), and a barrier of its own says when P V
+// has landed, for the rare rescaling of O.
 
 constexpr int kTcTile = 128;
 constexpr int kCopyWarps = 3;
 constexpr int kTcThreads = (8 + kCopyWarps + 1) * 32;
 enum TBar { tQFull = 0, tKFull = 1, tKEmpty = 3, tVFull = 5, tVEmpty = 7, tSFull = 9, tPReady = 11, tOFinal = 13,
-            tDrain = 14, tBars = 15 };
+            tDrain = 14, tODone = 15, tBars = 16 };
 
 template <int D>
 struct TSmem {
@@ -621,6 +623,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     mbar_init(bar(tOFinal), 1);
     mbar_init(bar(tDrain), 1);
+    mbar_init(bar(tODone), 1);
     *abort = 0;
     *odd = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -761,28 +764,52 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tma_load_3d(base + S::q + t * S::tile + h * S::half, &tm_q, h * 64, kvh * p.group, rq.lo + node0 + t * nodes,
                       bar(tQFull));
       constexpr uint32_t idesc_qk = idesc_of<T>(kTcTile, false), idesc_pv = idesc_of<T>(D, true);
-      auto qk = [&](int t, int s) {
+      auto qk = [&](int t, int s, int to) {
         const uint64_t a = sw128_desc(base + S::q + t * S::tile, 16, 1024), k = sw128_desc(base + S::k + s * S::tile, 16, 1024);
 #pragma unroll
         for (int x = 0; x < D / 16; ++x) {
           const uint64_t off = uint64_t((x >> 2) * S::half + (x & 3) * 32) >> 4;
-          mma_ss(tmem + t * 256, a + off, k + off, idesc_qk, x > 0);
+          mma_ss(tmem + to * 256, a + off, k + off, idesc_qk, x > 0);
         }
       };
-      auto pv = [&](int t, int s, bool acc) {
+      auto pv = [&](int t, int s, int from, bool acc) {
         const uint64_t v = sw128_desc(base + S::v + s * S::tile, S::half, 1024);
 #pragma unroll
         for (int x = 0; x < kTcTile / 16; ++x)
-          mma_ts(tmem + t * 256 + 128, tmem + t * 256 + 8 * x, v + uint64_t(x * 2048 >> 4), idesc_pv, acc || x > 0);
+          mma_ts(tmem + t * 256 + 128, tmem + from * 256 + 8 * x, v + uint64_t(x * 2048 >> 4), idesc_pv, acc || x > 0);
       };
       bool ok = mbar_wait(bar(tQFull), 0, abort, p.batch.err);
-      if (ok && n_tiles > 0) {
+      if (q_tiles == 1) {
+        auto scores = [&](int i) {  // Q K^T of key tile i into S buffer i % 2
+          const int s = i & 1;
+          if (!mbar_wait(bar(tKFull + s), (i >> 1) & 1, abort, p.batch.err)) return false;
+          fence_async_smem();  // the copying threads' writes, which the barrier showed, before the products' reads
+          tc_fence_after();
+          qk(0, s, s);
+          mma_commit(bar(tSFull + s));
+          mma_commit(bar(tKEmpty + s));
+          return true;
+        };
+        for (int i = 0; i < 2 && i < n_tiles && ok; ++i) ok = scores(i);
+        for (int i = 0; i < n_tiles && ok; ++i) {
+          const int s = i & 1;
+          ok = mbar_wait(bar(tVFull + s), (i >> 1) & 1, abort, p.batch.err) &&
+               mbar_wait(bar(tPReady + s), (i >> 1) & 1, abort, p.batch.err);
+          if (!ok) break;
+          fence_async_smem();
+          tc_fence_after();
+          pv(0, s, s, i > 0);
+          mma_commit(bar(tVEmpty + s));
+          mma_commit(bar(tODone));
+          if (i + 2 < n_tiles) ok = scores(i + 2);
+        }
+      } else if (ok && n_tiles > 0) {
         ok = mbar_wait(bar(tKFull), 0, abort, p.batch.err);
         if (ok) {
           fence_async_smem();  // the copying threads' writes, which the barrier showed, before the products' reads
           tc_fence_after();
           for (int t = 0; t < q_tiles; ++t) {
-            qk(t, 0);
+            qk(t, 0, t);
             mma_commit(bar(tSFull + t));
           }
           mma_commit(bar(tKEmpty));
@@ -795,7 +822,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             ok = mbar_wait(bar(tPReady + t), i & 1, abort, p.batch.err);
             if (!ok) break;
             tc_fence_after();
-            pv(t, s, i > 0);
+            pv(t, s, t, i > 0);
             if (i + 1 < n_tiles) {
               if (t == 0) {
                 ok = mbar_wait(bar(tKFull + s1), ((i + 1) >> 1) & 1, abort, p.batch.err);
@@ -803,7 +830,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 fence_async_smem();
                 tc_fence_after();
               }
-              qk(t, s1);
+              qk(t, s1, t);
               mma_commit(bar(tSFull + t));
             }
           }
@@ -826,7 +853,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int dn = r / p.group, node = node0 + t * nodes + dn;
     const bool mine = r < filled && node < rq.n;
     const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
-    const uint32_t s_col = lanes + t * 256, o_col = s_col + 128;
+    const uint32_t o_col = lanes + t * 256 + 128;
+    const bool single = q_tiles == 1;  // S buffers and their barriers alternate
     // keys 32 c .. 32 c + 31 of tile `at` that the row sees, a bit each
     auto bits32 = [&](int at, int c) -> uint32_t {
       int seen;
@@ -848,10 +876,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     bool ok = true;
     const bool idle = !__any_sync(0xffffffffu, mine);  // no row of the warp is used: what P holds there reaches no other
     for (int i = 0; i < n_tiles; ++i) {
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(tSFull + t), i & 1, abort, p.batch.err));
+      const int sb = single ? i & 1 : t;
+      const uint32_t s_col = lanes + sb * 256;
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(tSFull + sb), single ? (i >> 1) & 1 : i & 1, abort, p.batch.err));
       if (!ok) break;
       if (idle) {
-        if (lane == 0) mbar_arrive(bar(tPReady + t));
+        if (lane == 0) mbar_arrive(bar(tPReady + sb));
         continue;
       }
       tc_fence_after();
@@ -906,7 +936,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(tPReady + t));
+          if (lane == 0) mbar_arrive(bar(tPReady + sb));
           continue;
         }
       }
@@ -936,6 +966,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (__any_sync(0xffffffffu, grow)) {
         const float f = grow && m_use != -INFINITY ? join_factor(m_use, mx) : 1.0f;
         if (i > 0) {
+          if (single) {  // S being there does not say that P V of the tile before has landed
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(tODone), (i - 1) & 1, abort, p.batch.err));
+            if (!ok) break;
+            tc_fence_after();
+          }
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t w[32];
@@ -978,7 +1013,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(tPReady + t));
+      if (lane == 0) mbar_arrive(bar(tPReady + sb));
     }
     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(tOFinal), 0, abort, p.batch.err));
     const bool drafts = first + n_tiles > cached_tiles;
@@ -1157,14 +1192,10 @@ struct TreePlan {
   int64_t workspace;
 };
 
-// More rows a K/V head than this take the tensor-memory kernel, whose row tile is 128 (the groups must fit it).
-#ifndef QE_TC_FIX
-#define QE_TC_FIX 4
-#endif
-#ifndef QE_TREE_TC_ROWS
-#define QE_TREE_TC_ROWS 32
-#endif
-constexpr int kTcRows = QE_TREE_TC_ROWS;
+// More rows a K/V head than this take the tensor-memory kernel, whose row tile is 128 (the groups must fit it). 8 requests
+// of 701 to 6,007 tokens, 7 rows a node: 14 rows 18.6 us with the kernel of 16-row tiles against 26.4, 21 rows 26.3 (32
+// rows a CTA) against 26.6, 35 rows 33 against 27, 105 rows 59 against 28.
+constexpr int kTcRows = 32;
 
 TreePlan make_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head_dim) {
   TreePlan t{};
@@ -1178,10 +1209,10 @@ TreePlan make_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head
   const int64_t max_tiles = std::max(1, tiles_of(in.max_length, in.max_nodes, t.key_tile));
   // Tiles a CTA: of the whole batch's tiles, over the CTAs that the SMs hold (two, or one with all of the tensor
   // memory), the count that ends first. The model: waves x (tiles + `fixed`, what a CTA's start and end cost in tiles),
-  // half a CTA more per request for the last, shorter one. One wave for all took 64 requests of 313 to 8,191 tokens
-  // from N to M us.
+  // half a CTA more per request for the last, shorter one. With one wave for all, 64
+  // requests of 313 to 8,191 tokens took 119 us instead of 102.
   const int64_t all = (in.sum_length + t.key_tile - 1) / t.key_tile + int64_t(in.batch) * tiles_of(0, in.max_nodes, t.key_tile);
-  const int64_t slots = (t.tc ? 1 : 2) * sm_count(), step = t.tc ? 1 : kWarps, fixed = t.tc ? QE_TC_FIX : 16;
+  const int64_t slots = (t.tc ? 1 : 2) * sm_count(), step = t.tc ? 1 : kWarps, fixed = t.tc ? 4 : 16;
   const int64_t ragged = in.batch > 1 ? in.batch / 2 : 0;
   int64_t per = max_tiles, best = INT64_MAX;
   for (int64_t x = step;; x = std::max(x + step, x * 9 / 8 / step * step)) {
