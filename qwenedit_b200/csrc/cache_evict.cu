@@ -352,15 +352,24 @@ extern "C" int qe_retain(qe_planes pool, int64_t pool_rows, int32_t layers, int3
                    pool.inner_stride % 16 == 0,
                "qe_retain: pool planes must be 16-byte aligned [layers, 2]");
   try {
-    std::vector<uint8_t> taken(static_cast<size_t>(pool_rows), 0);
-    for (int64_t i = 0; i < n_src; ++i) {
+    for (int64_t i = 0; i < n_src; ++i)
       QE_CHECK_ARG(src_host[i] >= 0 && src_host[i] < pool_rows, "qe_retain: source slots outside the pool");
-      taken[size_t(src_host[i])] = 1;
-    }
-    for (int64_t i = 0; i < n_keep; ++i) {
+    for (int64_t i = 0; i < n_keep; ++i)
       QE_CHECK_ARG(dst_host[i] >= 0 && dst_host[i] < pool_rows, "qe_retain: destination slots outside the pool");
-      QE_CHECK_ARG(!taken[size_t(dst_host[i])], "qe_retain: a destination slot twice, or among the sources");
-      taken[size_t(dst_host[i])] = 1;
+    const char *twice = "qe_retain: a destination slot twice, or among the sources";
+    if (pool_rows <= 16 * (n_src + n_keep)) {  // a mark per row of the pool, or, in a large pool, the sorted slots
+      std::vector<uint8_t> taken(static_cast<size_t>(pool_rows), 0);
+      for (int64_t i = 0; i < n_src; ++i) taken[size_t(src_host[i])] = 1;
+      for (int64_t i = 0; i < n_keep; ++i) {
+        QE_CHECK_ARG(!taken[size_t(dst_host[i])], "%s", twice);
+        taken[size_t(dst_host[i])] = 1;
+      }
+    } else {
+      std::vector<int64_t> to(dst_host, dst_host + n_keep);
+      std::sort(to.begin(), to.end());
+      QE_CHECK_ARG(std::adjacent_find(to.begin(), to.end()) == to.end(), "%s", twice);
+      for (int64_t i = 0; i < n_src; ++i)
+        QE_CHECK_ARG(!std::binary_search(to.begin(), to.end(), src_host[i]), "%s", twice);
     }
   } catch (const std::bad_alloc &) {
     return fail(QE_ERR_NOMEM, "qe_retain: out of host memory");

@@ -1379,9 +1379,8 @@ extern "C" int qe_tree_attention(const qe_tree_attention_args *args, void *strea
                    (!k_draft || (draft_head_stride >= row && draft_token_stride >= row)),
                "qe_tree_attention: strides must hold a row of head_dim");
   QE_CHECK_ARG(std::isfinite(scale) && scale > 0.0f, "qe_tree_attention: scale must be positive and finite");
-  QE_CHECK_ARG((int64_t(batch.max_nodes) * (heads_q / heads_kv) + 15) / 16 * heads_kv <= 65535,
-               "qe_tree_attention: too many rows (max_nodes x heads_q / 16 passes 65535)");
   const TreePlan t = tree_plan(batch, heads_q, heads_kv, head_dim);
+  QE_CHECK_ARG(t.row_ctas <= 65535, "qe_tree_attention: too many rows (%d CTAs for one request)", t.row_ctas);
   QE_CHECK_ARG(t.workspace == 0 || (workspace && aligned16(workspace) && workspace_bytes >= t.workspace),
                "qe_tree_attention: needs %lld bytes of 16-byte aligned workspace", (long long)t.workspace);
   p.q = static_cast<const char *>(q);

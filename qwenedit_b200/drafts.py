@@ -28,7 +28,12 @@ HEAD_DIMS = (64, 128)
 
 def _to_device(host: np.ndarray, device: torch.device) -> torch.Tensor:
     t = torch.from_numpy(host)
-    return t.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else t.to(device)
+    if device.type != "cuda":
+        return t.to(device)
+    if torch.cuda.is_current_stream_capturing():
+        # the copy would be replayed from host memory that is no longer these values
+        raise RuntimeError("values from the host cannot go into a captured graph: set them outside of it")
+    return t.pin_memory().to(device, non_blocking=True)
 
 
 class PagedBatch:

@@ -176,9 +176,10 @@ def test_c_entry_points_reject_and_accept_nothing():
         retain(dst, head=24)
     with pytest.raises(ValueError, match=r"\[layers, 2\]"):
         retain(dst, inner=1)
-    for bad in ([5, 5], [5, 3]):
-        with pytest.raises(ValueError, match="twice, or among"):
-            retain(np.array(bad, np.int64))
+    for rows in (8, 100_000):  # marks, and sorted slots
+        for bad in ([5, 5], [5, 3]):
+            with pytest.raises(ValueError, match="twice, or among"):
+                retain(np.array(bad, np.int64), rows=rows)
     for bad in ([5, 8], [-1, 5]):
         with pytest.raises(ValueError, match="destination slots outside"):
             retain(np.array(bad, np.int64))

@@ -152,6 +152,24 @@ def test_pages_outside_the_pool_with_many_rows():
     _compare(pool, slots, lens, [n], [R.chain(n)], q, kn, vn, out, lse, 0)
 
 
+@pytest.mark.parametrize("counts,hq,hkv", [([1500], 4, 2), ([3, 2], 132, 1), ([2], 260, 2), ([1, 40], 128, 1), ([20], 127, 1)])
+def test_long_drafts_and_large_groups(counts, hq, hkv):
+    lens = [700, 63][: len(counts)]
+    pool, slots, q, kn, vn = _case(lens, counts, hq, hkv, 64, torch.bfloat16, 16, 12, layers=1)
+    out, lse = tree_attention(q, PagedBatch(pool, slots), DraftTree(counts), 0, kn, vn, return_lse=True)
+    _compare(pool, slots, lens, counts, [R.chain(n) for n in counts], q, kn, vn, out, lse, 0)
+
+
+@pytest.mark.parametrize("n", [1, 30])
+def test_scores_that_pass_the_reference_maximum_late(n):
+    """Keys whose scores jump by hundreds at the end of a tile, in its middle and tiles later."""
+    pool, slots, q, kn, vn = _case([1000], [n], 8, 2, 64, torch.float16, 16, 11, layers=1)
+    for at, f in ((40, 30.0), (127, 60.0), (130, 100.0), (515, 200.0), (998, 300.0)):
+        pool.kv[0, 0, slots[0][at]] = (pool.kv[0, 0, slots[0][at]].float() * f).half()
+    out, lse = tree_attention(q, PagedBatch(pool, slots), DraftTree([n]), 0, kn, vn, return_lse=True)
+    _compare(pool, slots, [1000], [n], [R.chain(n)], q, kn, vn, out, lse, 0)
+
+
 def test_scores_far_apart():
     """Maxima that grow by hundreds along the keys, and scores that vanish beside them."""
     pool, slots, q, kn, vn = _case([2000], [3], 8, 2, 64, torch.bfloat16, 16, 11)
@@ -266,6 +284,39 @@ def test_graphs_replay_with_new_lengths_and_keep_apart():
         for layer in (0, 1):
             out, lse = results[layer]
             _compare(pool, slots, lengths, counts, [R.chain(1)] * 2, q, kn, vn, out, lse, layer)
+
+
+def test_host_values_are_refused_in_a_captured_graph():
+    pool, slots, *_ = _case([20], [2], 4, 2, 64, torch.bfloat16, 16, 4)
+    cache, tree = PagedBatch(pool, slots), DraftTree([2], [-1, 0])
+    parents = torch.tensor([-1, -1], dtype=torch.int32, device=DEV)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for call in (lambda: cache.set_lengths([3]), lambda: tree.set_parents([-1, -1]), lambda: DraftTree([1])):
+            with pytest.raises(RuntimeError, match="captured graph"):
+                call()
+        tree.set_parents(parents)  # a device tensor is fine
+        cache.lengths.sub_(1)
+    g.replay()
+    assert cache.lengths.tolist() == [19] and tree.masks.flatten().tolist() == [1, 2]
+
+
+def test_overlapping_calls_on_two_streams():
+    """Calls of one cache and tree on two streams at once: each has its own workspace."""
+    pool, slots, q, kn, vn = _case([30011], [3], 28, 4, 128, torch.bfloat16, 64, 6)
+    cache, tree = PagedBatch(pool, slots), DraftTree([3])
+    want = [tree_attention(q, cache, tree, layer, kn, vn) for layer in (0, 1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for layer, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[layer].append(tree_attention(q, cache, tree, layer, kn, vn))
+    torch.cuda.synchronize()
+    for layer in (0, 1):
+        for out in got[layer]:
+            assert torch.equal(out, want[layer])
 
 
 def test_rows_past_32_bit_offsets():

@@ -92,6 +92,18 @@ def test_weights_of_a_prompt(n, length, d, dtype):
     _run([length], [n], 4, 2, d, dtype, 16, seed=n)
 
 
+@pytest.mark.parametrize("counts,hq,hkv", [([3, 2], 132, 1), ([2], 260, 1), ([3, 40], 100, 1), ([2], 128, 1)])
+def test_weights_of_large_groups(counts, hq, hkv):
+    _run([300, 17][: len(counts)], counts, hq, hkv, 64, torch.bfloat16, 16, seed=hq)
+
+
+@pytest.mark.parametrize("kind", ["chain", "tree"])
+@pytest.mark.parametrize("n", [33, 60])
+def test_weights_either_side_of_the_kernels_border(kind, n):
+    """Rows a K/V head (7 a node) around the count from which the tensor-memory kernel takes over."""
+    _run([900, 0, 129], [n, 3, n - 1], 28, 4, 128, torch.bfloat16, 64, kind, seed=n)
+
+
 def test_weights_accumulate_into_a_wider_buffer():
     lens, counts, rooms = [130, 40], [2, 1], [200, 64]
     pool, slots, q, kn = _case(lens, counts, 28, 4, 128, torch.bfloat16, 64, 3, rooms=rooms)
