@@ -7,6 +7,11 @@ Drop-in modules (same API as the reference's):
   qwenedit_b200.fp4     <- multi_turn.fibo.fp4      (Quantized, norm_scale_fp4, silu_mul_fp4)
   qwenedit_b200.hooks   <- the pool call sites of multi_turn.pipeline.hooks / multi_turn.cache.encoder
 
+Additions without a counterpart in the reference:
+  qwenedit_b200.attention  attention over the pool pages (PagedPrefix, paged_attention, encoder tail, prefill)
+  qwenedit_b200.drafts     decoding over the pools: PagedBatch, DraftTree, tree_attention
+  qwenedit_b200.evict      attention_weights and heaviest; with PagedKVPool.retain, a cache cut by attention weight
+
 All device work runs in libqeb200.so (hand-written sm_100a kernels behind the C ABI in include/qeb200.h).
 """
 

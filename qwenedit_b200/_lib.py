@@ -197,5 +197,5 @@ def ptr64(array) -> "ctypes._Pointer":
     return array.ctypes.data_as(_P64)
 
 
-__all__ = ["LIB_PATH", "ATTENTION_WEIGHTS", "DRAFT_BATCH", "QEError", "Planes", "SIGNATURES", "TREE_ATTENTION", "call", "lib", "on_device", "planes", "ptr64",
-           "stream_of", "version", "c_uint8"]
+__all__ = ["ATTENTION_WEIGHTS", "DRAFT_BATCH", "LIB_PATH", "QEError", "Planes", "SIGNATURES", "TREE_ATTENTION", "call",
+           "lib", "on_device", "planes", "ptr64", "stream_of", "version", "c_uint8"]

@@ -41,8 +41,8 @@ __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
 
 // ---- few rows: every warp streams its own keys ------------------------------------------------------------------
 //
-// S^T = K Q^T with 16 keys as the A operand, the query rows (in shared memory) as B, eight at a time: a thread holds two
-// keys' scores against two of the eight rows. One pass over K per 224 query rows.
+// S^T = K Q^T with 16 keys as the A operand, the query rows (in shared memory) as B, eight at a time: a thread holds
+// two keys' scores against two of the eight rows. One pass over K per 224 query rows.
 
 // tiles of K per warp in the ring: three where the bytes bound the call (32 requests of 257 to 8,191 tokens, 7 rows a
 // K/V head: 41.5 us with four, 29.1 with three, 35.1 with two), two where the rows do and CTAs an SM count for more
@@ -102,8 +102,8 @@ __global__ void __launch_bounds__(kWarps * 32) attention_weights_kernel(const We
         for (int i = 0; i < kCopies; ++i) {
           const int r = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
           const int at = __shfl_sync(0xffffffffu, row, r);
-          cp_async16(ring + stage * kTileBytes + chunk_at<D>(r, c), at < 0 ? base : base + int64_t(at) * stride + c * 16,
-                     at < 0 ? 0 : 16);
+          cp_async16(ring + stage * kTileBytes + chunk_at<D>(r, c),
+                     at < 0 ? base : base + int64_t(at) * stride + c * 16, at < 0 ? 0 : 16);
         }
       }
       cp_async_commit();
@@ -317,8 +317,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!mbar_wait(bar(wQEmpty + s), ((asked / kTcStages) & 1) ^ 1, abort, p.batch.err)) break;
         mbar_expect_tx(bar(wQFull + s), uint32_t(filled) * (D * 2));
         for (int h = 0; h < D / 64; ++h)
-          tma_load_3d(base + S::q + s * S::tile + h * S::half, &tm_q, h * 64, kvh * p.group, rq.lo + (qa + asked) * nodes,
-                      bar(wQFull + s));
+          tma_load_3d(base + S::q + s * S::tile + h * S::half, &tm_q, h * 64, kvh * p.group,
+                      rq.lo + (qa + asked) * nodes, bar(wQFull + s));
       }
       if (asked < n_q) {  // a wait gave up: time for the copies in flight before the shared memory is given back
         const uint64_t since = globaltimer();
@@ -434,7 +434,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             leave();
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float2 x = up2(fma2(pk2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), scale2, nl2));
+            const f32x2 raw = pk2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1]));
+            const float2 x = up2(fma2(raw, scale2, nl2));
             if (kPlain) {
               acc[c * 8 + e] = add2(acc[c * 8 + e], pk2(ex2(x.x), ex2(x.y)));
             } else {
@@ -486,7 +487,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     float w = 0.0f;
     for (int x = 0; x < splits; ++x)
       for (int u = 0; u < 4; ++u)
-        w += x == 0 ? part[u * kTile + threadIdx.x] : ld_cluster1(base + S::part + 4 * (u * kTile + threadIdx.x), uint32_t(x));
+        w += x == 0 ? part[u * kTile + threadIdx.x]
+                    : ld_cluster1(base + S::part + 4 * (u * kTile + threadIdx.x), uint32_t(x));
     if (key < (draft ? drafted : rq.len)) {
       float *dst = out + (draft ? rq.len : 0) + key;
       *dst = p.accumulate ? *dst + w : w;

@@ -15,9 +15,11 @@ namespace {
 // Per row the key (an order-preserving integer) of the last position kept, by radix selection from the top bits, then
 // one ordered pass that writes the kept positions. A CTA per row, each warp a run of neighbouring positions. The keys
 // of a row of up to 73,728 positions stay on the SM, in registers (to 32,768) and shared memory, read once with the
-// loads in flight together; a longer row is read again in each pass (from L2), eight loads at a time. Digits are 11, 11 and 10 bits: the first holds the sign,
-// the exponent and two mantissa bits, so that weights spread over some octaves meet in one counter a few at a time.
-// What bounds it is the instructions per position (25 or so; forms with 128 took five times as long), not the memory.
+// loads in flight together; a longer row is read again in each pass (from L2), eight loads at a time. Digits are 11, 11
+// and 10 bits: the first holds the sign, the exponent and two mantissa bits, so that weights spread over some octaves
+// meet in one counter a few at a time; a pass whose digit is kept whole ends the search. What bounds it is instructions,
+// about 90 a warp per 32 positions over all the passes, at 0.6 of the issue rate (1,792 rows of 3,001 to 32,749: 187 us,
+// 0.13 of the copy rate).
 
 struct HeaviestParams {
   const float *weights;
@@ -70,7 +72,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
       const int i = from + j * 32 + lane;
       return i < to ? __float_as_uint(__ldg(mid + i)) : 0u;
     };
-    auto key_at = [&](int j, uint32_t bits) { return from + j * 32 + lane < to ? order_key(__uint_as_float(bits)) : 0u; };
+    auto key_at = [&](int j, uint32_t bits) {
+      return from + j * 32 + lane < to ? order_key(__uint_as_float(bits)) : 0u;
+    };
 #pragma unroll
     for (int j = 0; j < kItems; ++j)
       if (j < steps) held[j] = bits_at(j);
@@ -219,10 +223,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
 
 __device__ __forceinline__ uint4 load_vec(const uint4 *p) {
   uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
   return v;
 }
-__device__ __forceinline__ void store_vec(uint4 *p, const uint4 &v) { st_stream(reinterpret_cast<int4 *>(p), *reinterpret_cast<const int4 *>(&v)); }
+__device__ __forceinline__ void store_vec(uint4 *p, const uint4 &v) {
+  st_stream(reinterpret_cast<int4 *>(p), make_int4(int(v.x), int(v.y), int(v.z), int(v.w)));
+}
 struct RetainParams {
   char *base;
   int64_t outer, inner;  // bytes between layers, between K and V
@@ -276,7 +284,8 @@ __global__ void __launch_bounds__(256) retain_kernel(const RetainParams p) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         const int c = c0 + u * 32, r = c / chunks;
-        const int fr = __shfl_sync(0xffffffffu, f, r & (kRows - 1)), to_row = __shfl_sync(0xffffffffu, t, r & (kRows - 1));
+        const int fr = __shfl_sync(0xffffffffu, f, r & (kRows - 1));
+        const int to_row = __shfl_sync(0xffffffffu, t, r & (kRows - 1));
         if (c < total && fr >= 0) {
           char *dst = plane + int64_t(to_row) * p.row_bytes + (c - r * chunks) * 16;
           store_vec(reinterpret_cast<uint4 *>(dst), v[0][u]);
@@ -388,8 +397,8 @@ extern "C" int qe_retain(qe_planes pool, int64_t pool_rows, int32_t layers, int3
   p.n_keep = n_keep;
   p.heads = heads;
   p.err = err_flag;
-  // 32 positions a warp, or 16 while that leaves warps without work (28 layers x 4 heads, 251 of 1,024 kept: 9.2 against
-  // 7.3 us; 8,192 of 32,768: 162 against 170, 0.90 of the copy rate)
+  // 32 positions a warp, or 16 while that leaves warps without work (28 layers x 4 heads, 251 of 1,024 kept: 9.2
+  // against 7.3 us; 8,192 of 32,768: 162 against 170, 0.90 of the copy rate)
   const int64_t heads_all = int64_t(layers) * heads;
   const bool few = heads_all * ((n_keep + 31) / 32) <= int64_t(sm_count()) * 16;
   const int rows = few ? 16 : 32;

@@ -100,6 +100,14 @@ __global__ void tree_masks_kernel(const int32_t *parents, const int32_t *starts,
 }
 
 // ---- few rows: every warp on its own keys ---------------------------------------------------------------------
+//
+// Up to 32 rows a K/V head (one token a request: its G heads). Each warp streams 16-key tiles of K and V through its
+// own ring (cp.async, three tiles), keeps its own maximum, sum and O for all the rows, and waits for no other warp
+// until the end: a tile is 16 + 16 matrix instructions of 16 rows (mma.sync: its rate is far above what the bytes need,
+// and P goes from accumulator to operand in registers). HBM is the bound: 64 requests of 313 to 8,191 tokens, 558 MB,
+// in 102.5 us = 5.45 TB/s, 0.84 of the measured copy rate; what is missing is each CTA's start (three dependent loads
+// before the first K row) and end, about a sixth of a CTA's time at the chosen split. One request over 1,024 tokens is
+// that chain alone: 10 us.
 
 constexpr int kWarps = 4;    // per CTA; two CTAs an SM
 constexpr int kStages = 3;   // 16-key tiles (K and V) in flight per warp
@@ -145,7 +153,9 @@ __host__ __device__ constexpr int tree_smem_bytes() {
 }
 
 // joins (m, l) pairs: the factor that brings sums at reference m to reference m_all
-__device__ __forceinline__ float join_factor(float m, float m_all) { return m == m_all ? 1.0f : exp2_approx(m - m_all); }
+__device__ __forceinline__ float join_factor(float m, float m_all) {
+  return m == m_all ? 1.0f : exp2_approx(m - m_all);
+}
 
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeParams p) {
@@ -499,8 +509,8 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
       dst = reinterpret_cast<float4 *>(so + int64_t(r) * D + c);
       if (c == 0) am[r] = m_all, al[r] = l_all;
     } else {
-      const int64_t at = (int64_t(blockIdx.x) * p.batch.total + rq.lo + (row0 + r) / p.group) * p.heads_q + kvh * p.group +
-                         (row0 + r) % p.group;
+      const int token = rq.lo + (row0 + r) / p.group, head = kvh * p.group + (row0 + r) % p.group;
+      const int64_t at = (int64_t(blockIdx.x) * p.batch.total + token) * p.heads_q + head;
       dst = reinterpret_cast<float4 *>(p.part_o + at * D + c);
       if (c == 0) p.part_ml[at] = make_float2(m_all, l_all);
     }
@@ -537,6 +547,9 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
 
 // ---- many rows: both products on the fifth-generation tensor cores -----------------------------------------------
 //
+// More rows than that: the products bound it (61 drafted nodes x 7 heads are 427 rows against 512 bytes of K and V a
+// key), and 128-row tiles of tcgen05.mma carry them.
+//
 // A CTA takes up to two tiles of 128 rows (the G heads of as many whole nodes as fit) of one K/V head and runs over
 // its share of the keys, 128 at a time: S = Q K^T, softmax in registers, O += P V with P from tensor memory.
 //   warps 0-7   softmax, one warpgroup per row tile, a thread per row (tensor-memory lane)
@@ -547,9 +560,11 @@ __global__ void __launch_bounds__(kWarps * 32) tree_attention_kernel(const TreeP
 //               the end, for the rows that do. (A TMA gather of four rows a lane took 10 us a tile.)
 //   warp 11     Q by TMA, tcgen05.mma (one thread), and the tensor memory: S0 | O0 | S1 | O1, P_t over S_t
 // The products of one thread execute in issue order, so P_t V(j) reads P_t(j) before Q_t K^T(j + 1) rewrites S_t, and
-// S_t(j + 1) being there means that O_t holds every product up to tile j. A single row tile has both S buffers: the next
-// key tile's Q K^T runs under the softmax of this one (8 requests of 5 nodes over 701 to 6,007: 27.0 -> 26.6 us), and a barrier of its own says when P V
-// has landed, for the rare rescaling of O.
+// S_t(j + 1) being there means that O_t holds every product up to tile j. Measured on 24 nodes (168 rows) over 65,521
+// tokens: 2.6 us per key tile of 256 rows (softmax 1.1, of that 1.08 the exponential unit's; a row tile's own products
+// 0.54, the rest handing over), 4 us before the first softmax and 3 us after the last product: 55 us in all. A single
+// row tile has both S buffers: the next key tile's Q K^T runs under the softmax of this one (8 requests of 5 nodes over
+// 701 to 6,007: 27.0 -> 26.6 us), and a barrier of its own says when P V has landed, for the rare rescaling of O.
 
 constexpr int kTcTile = 128;
 constexpr int kCopyWarps = 3;
@@ -670,7 +685,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     };
     auto settle = [&](int t) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) row[e] = page[e] == INT_MIN ? -1 : row_in_page(p.batch, page[e], t * kTcTile + row_of(e * 32 + lane));
+      for (int e = 0; e < 2; ++e)
+        row[e] = page[e] == INT_MIN ? -1 : row_in_page(p.batch, page[e], t * kTcTile + row_of(e * 32 + lane));
     };
     const uint32_t place0 = uint32_t(c >> 3) * S::half;
     auto copy_cached = [&](const char *src, uint32_t dst) {
@@ -708,7 +724,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                      : "memory");
       }
     };
-    // Boxes of a tile: pages of box_rows rows, 64 dims each; a lane of warp 8 copies one (its table entry a tile ahead).
+    // Boxes of a tile: pages of box_rows rows, 64 dims each; a lane of warp 8 copies one (its table entry a tile
+    // ahead).
     constexpr int kHalves = D / 64;
     const int box_rows = min(p.batch.page_size, kTcTile), boxes = page_boxes ? kTcTile / box_rows * kHalves : 0;
     const int box_page = lane / kHalves, box_half = lane % kHalves;
@@ -765,7 +782,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                       bar(tQFull));
       constexpr uint32_t idesc_qk = idesc_of<T>(kTcTile, false), idesc_pv = idesc_of<T>(D, true);
       auto qk = [&](int t, int s, int to) {
-        const uint64_t a = sw128_desc(base + S::q + t * S::tile, 16, 1024), k = sw128_desc(base + S::k + s * S::tile, 16, 1024);
+        const uint64_t a = sw128_desc(base + S::q + t * S::tile, 16, 1024);
+        const uint64_t k = sw128_desc(base + S::k + s * S::tile, 16, 1024);
 #pragma unroll
         for (int x = 0; x < D / 16; ++x) {
           const uint64_t off = uint64_t((x >> 2) * S::half + (x & 3) * 32) >> 4;
@@ -874,7 +892,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     };
     float m_use = -INFINITY, l = 0.0f;
     bool ok = true;
-    const bool idle = !__any_sync(0xffffffffu, mine);  // no row of the warp is used: what P holds there reaches no other
+    // no row of the warp is used: what P holds there reaches no other row
+    const bool idle = !__any_sync(0xffffffffu, mine);
     for (int i = 0; i < n_tiles; ++i) {
       const int sb = single ? i & 1 : t;
       const uint32_t s_col = lanes + sb * 256;
@@ -900,7 +919,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         tmem_ld_wait(buf[0]);
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < 32; ++e) top[e & 1] = (see >> e) & 1u ? fmaxf(top[e & 1], __uint_as_float(buf[0][e])) : top[e & 1];
+        for (int e = 0; e < 32; ++e)
+          if ((see >> e) & 1u) top[e & 1] = fmaxf(top[e & 1], __uint_as_float(buf[0][e]));
         if (m_use == -INFINITY) m_use = fmaxf(top[0], top[1]) * p.scale_log2;  // its O and l are still 0
       }
       // One pass where every row has a reference maximum: p = 2^(s scale - m_use) without looking for the tile's
@@ -917,7 +937,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (c + 1 < 4) tmem_ld32_async(s_col + 32 * (c + 1), buf[(c + 1) & 1]);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float2 x = up2(fma2(pk2(__uint_as_float(buf[c & 1][2 * e]), __uint_as_float(buf[c & 1][2 * e + 1])), scale2, base2));
+            const f32x2 raw = pk2(__uint_as_float(buf[c & 1][2 * e]), __uint_as_float(buf[c & 1][2 * e + 1]));
+            const float2 x = up2(fma2(raw, scale2, base2));
             float y0 = ex2(x.x), y1 = ex2(x.y);
             if (masked) {
               y0 = (bits[c] >> (2 * e)) & 1u ? y0 : 0.0f;
@@ -949,7 +970,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (c + 1 < 4) tmem_ld32_async(s_col + 32 * (c + 1), buf[(c + 1) & 1]);
         if (masked) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) m4[e & 3] = (bits[c] >> e) & 1u ? fmaxf(m4[e & 3], __uint_as_float(buf[c & 1][e])) : m4[e & 3];
+          for (int e = 0; e < 32; ++e)
+            if ((bits[c] >> e) & 1u) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(buf[c & 1][e]));
         } else {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
@@ -997,7 +1019,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float2 x = up2(fma2(pk2(__uint_as_float(buf[c & 1][2 * e]), __uint_as_float(buf[c & 1][2 * e + 1])), scale2, nbase2));
+          const f32x2 raw = pk2(__uint_as_float(buf[c & 1][2 * e]), __uint_as_float(buf[c & 1][2 * e + 1]));
+          const float2 x = up2(fma2(raw, scale2, nbase2));
           float y0 = ex2(x.x), y1 = ex2(x.y);
           if (masked) {
             y0 = (bits[c] >> (2 * e)) & 1u ? y0 : 0.0f;
@@ -1018,7 +1041,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(tOFinal), 0, abort, p.batch.err));
     const bool drafts = first + n_tiles > cached_tiles;
     if (ok && drafts)  // what the copying warps found in V
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(tVFull + ((n_tiles - 1) & 1)), ((n_tiles - 1) >> 1) & 1, abort, p.batch.err));
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(tVFull + ((n_tiles - 1) & 1)), ((n_tiles - 1) >> 1) & 1, abort,
+                                             p.batch.err));
     if (ok) {
       tc_fence_after();
       const int token = rq.lo + node, head = kvh * p.group + r - dn * p.group;
@@ -1036,11 +1060,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (mine) {
           float o[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = l == 0.0f ? 0.0f : __uint_as_float(w[e]);  // no key seen: O may be unwritten
+          for (int e = 0; e < 32; ++e)
+            o[e] = l == 0.0f ? 0.0f : __uint_as_float(w[e]);  // no key seen: O may be unwritten
           if (put_back) {
-            for (int j = max(first - cached_tiles, 0) * kTcTile; j < min(rq.n, (first + n_tiles - cached_tiles) * kTcTile); ++j) {
+            const int j_end = min(rq.n, (first + n_tiles - cached_tiles) * kTcTile);
+            for (int j = max(first - cached_tiles, 0) * kTcTile; j < j_end; ++j) {
               if (!((bits32(cached_tiles + j / kTcTile, j % kTcTile / 32) >> (j & 31)) & 1u)) continue;
-              const T *v = reinterpret_cast<const T *>(p.v_draft + int64_t(rq.lo + j) * p.draft_token + int64_t(kvh) * p.draft_head) + 32 * c;
+              const T *v = reinterpret_cast<const T *>(p.v_draft + int64_t(rq.lo + j) * p.draft_token +
+                                                       int64_t(kvh) * p.draft_head) +
+                           32 * c;
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
                 const float x = to_float(v[e]);
@@ -1192,9 +1220,9 @@ struct TreePlan {
   int64_t workspace;
 };
 
-// More rows a K/V head than this take the tensor-memory kernel, whose row tile is 128 (the groups must fit it). 8 requests
-// of 701 to 6,007 tokens, 7 rows a node: 14 rows 18.6 us with the kernel of 16-row tiles against 26.4, 21 rows 26.3 (32
-// rows a CTA) against 26.6, 35 rows 33 against 27, 105 rows 59 against 28.
+// More rows a K/V head than this take the tensor-memory kernel, whose row tile is 128 (the groups must fit it). 8
+// requests of 701 to 6,007 tokens, 7 rows a node: 14 rows 18.6 us with the kernel of 16-row tiles against 26.4, 21 rows
+// 26.3 (32 rows a CTA) against 26.6, 35 rows 33 against 27, 105 rows 59 against 28.
 constexpr int kTcRows = 32;
 
 TreePlan make_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head_dim) {
@@ -1211,7 +1239,8 @@ TreePlan make_plan(const qe_draft_batch &in, int heads_q, int heads_kv, int head
   // memory), the count that ends first. The model: waves x (tiles + `fixed`, what a CTA's start and end cost in tiles),
   // half a CTA more per request for the last, shorter one. With one wave for all, 64
   // requests of 313 to 8,191 tokens took 119 us instead of 102.
-  const int64_t all = (in.sum_length + t.key_tile - 1) / t.key_tile + int64_t(in.batch) * tiles_of(0, in.max_nodes, t.key_tile);
+  const int64_t all = (in.sum_length + t.key_tile - 1) / t.key_tile +
+                      int64_t(in.batch) * tiles_of(0, in.max_nodes, t.key_tile);
   const int64_t slots = (t.tc ? 1 : 2) * sm_count(), step = t.tc ? 1 : kWarps, fixed = t.tc ? 4 : 16;
   const int64_t ragged = in.batch > 1 ? in.batch / 2 : 0;
   int64_t per = max_tiles, best = INT64_MAX;
@@ -1291,7 +1320,8 @@ int run_tree(const TreeParams &p, const TreePlan &t, const qe_draft_batch &in, c
   const dim3 grid(unsigned(t.splits), unsigned(t.row_ctas), unsigned(in.batch));
   int s;
   if (t.tc) {
-    const CUtensorMapDataType type = exponent_bits<T>() == 0x7f80u ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUtensorMapDataType type =
+        exponent_bits<T>() == 0x7f80u ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap q;
     const uint64_t q_dims[3] = {uint64_t(D), uint64_t(p.heads_q), uint64_t(in.total)};
     const uint64_t q_strides[2] = {uint64_t(p.q_head), uint64_t(p.q_token)};
@@ -1300,20 +1330,24 @@ int run_tree(const TreeParams &p, const TreePlan &t, const qe_draft_batch &in, c
     CUtensorMap kv[2];
     std::memset(kv, 0, sizeof(kv));
     const int P = in.page_size;
-    const bool page_boxes = p.batch.table_width > 0 && in.max_length >= kTcTile && P >= 8 && (kTcTile % P == 0 || P % kTcTile == 0);
+    const bool page_boxes = p.batch.table_width > 0 && in.max_length >= kTcTile && P >= 8 &&
+                            (kTcTile % P == 0 || P % kTcTile == 0);
     if (page_boxes) {
       const uint64_t dims[4] = {uint64_t(D), uint64_t(p.heads_kv), uint64_t(P), uint64_t(p.batch.pool_pages)};
       const uint64_t strides[3] = {uint64_t(D) * 2, uint64_t(p.pool_row), uint64_t(p.pool_row) * uint64_t(P)};
       const uint32_t box[4] = {64, 1, uint32_t(std::min(P, kTcTile)), 1};
-      if ((s = tensor_map_16bit("qe_tree_attention", &kv[0], type, p.k_pool, 4, dims, strides, box, "the K plane"))) return s;
-      if ((s = tensor_map_16bit("qe_tree_attention", &kv[1], type, p.v_pool, 4, dims, strides, box, "the V plane"))) return s;
+      const char *who = "qe_tree_attention";
+      if ((s = tensor_map_16bit(who, &kv[0], type, p.k_pool, 4, dims, strides, box, "the K plane"))) return s;
+      if ((s = tensor_map_16bit(who, &kv[1], type, p.v_pool, 4, dims, strides, box, "the V plane"))) return s;
     }
-    s = launch<tree_attention_tc_kernel<T, D>>(grid, 1, kTcThreads, TSmem<D>::bytes, stream, "qe_tree_attention launch", q, kv[0],
-                                               kv[1], int(page_boxes), p);
+    s = launch<tree_attention_tc_kernel<T, D>>(grid, 1, kTcThreads, TSmem<D>::bytes, stream,
+                                               "qe_tree_attention launch", q, kv[0], kv[1], int(page_boxes), p);
   } else if (t.m_tiles == 1) {
-    s = launch<tree_attention_kernel<T, D, 1>>(grid, t.cluster ? t.splits : 1, kWarps * 32, tree_smem_bytes<D, 1>(), stream, "qe_tree_attention launch", p);
+    s = launch<tree_attention_kernel<T, D, 1>>(grid, t.cluster ? t.splits : 1, kWarps * 32, tree_smem_bytes<D, 1>(),
+                                               stream, "qe_tree_attention launch", p);
   } else {
-    s = launch<tree_attention_kernel<T, D, 2>>(grid, t.cluster ? t.splits : 1, kWarps * 32, tree_smem_bytes<D, 2>(), stream, "qe_tree_attention launch", p);
+    s = launch<tree_attention_kernel<T, D, 2>>(grid, t.cluster ? t.splits : 1, kWarps * 32, tree_smem_bytes<D, 2>(),
+                                               stream, "qe_tree_attention launch", p);
   }
   if (s || t.splits == 1 || t.cluster) return s;
   // as many warps a row as have eight splits each

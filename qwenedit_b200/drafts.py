@@ -189,8 +189,8 @@ class DraftTree:
 
 
 class _View:
-    """The C view of a cache and a tree (``qe_draft_batch`` as bytes), and what the calls made with them have checked and
-    worked out, by the layouts of their tensors."""
+    """The C view of a cache and a tree (``qe_draft_batch`` as bytes), and what the calls made with them have checked
+    and worked out, by the layouts of their tensors."""
 
     __slots__ = ("cache", "batch", "plans")
 
@@ -307,6 +307,7 @@ class _TreePlan:
         heads = (heads_q, heads_kv, d, DTYPES[kv.dtype])
         size = ctypes.c_int64()
         with _lib.on_device(device):
-            _lib.call("qe_tree_attention_workspace", view.batch + _TREE.pack(*[0] * 17, *heads, 1.0), ctypes.byref(size))
+            _lib.call("qe_tree_attention_workspace", view.batch + _TREE.pack(*[0] * 17, *heads, 1.0),
+                      ctypes.byref(size))
         self.work = size.value
         self.tail = (size.value, pool._err.data_ptr(), *heads, 1.0 / math.sqrt(d) if scale is None else float(scale))

@@ -30,8 +30,9 @@ def attention_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedBatch, tre
 
     The arguments of the attention call that made `lse` [Hq, T] fp32 (``drafts.tree_attention`` with the same cache
     and tree; or ``attention.paged_attention``, whose block of n queries is ``DraftTree([n])`` over a ``PagedBatch`` of
-    one request, `full` where that call was not causal). Keys are the request's cached tokens, then, with `k_draft`, its new ones. A
-    token whose lse is +inf counts nothing (write it there to leave a rejected draft out), nor does one of -inf.
+    one request, `full` where that call was not causal). Keys are the request's cached tokens, then, with `k_draft`,
+    its new ones (in the tree's order). A token whose lse is +inf counts nothing (write it there to leave a rejected
+    draft out), nor does one of -inf.
 
     Returns `out` [B, Hkv, W] fp32, by default as wide as the longest request needs: its slots, and with `k_draft` the
     tree's largest count. With `accumulate` the weights are added to what `out` holds (positions past a request's
@@ -39,7 +40,8 @@ def attention_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedBatch, tre
     view = tree._view
     if view is None or view.cache is not cache:
         view = _view(cache, tree)
-    key = (layer, scale, accumulate, q.shape, q.stride(), q.dtype, q.device, lse.shape, lse.stride(), lse.dtype, lse.device,
+    key = (layer, scale, accumulate, q.shape, q.stride(), q.dtype, q.device,
+           lse.shape, lse.stride(), lse.dtype, lse.device,
            None if k_draft is None else (k_draft.shape, k_draft.stride(), k_draft.dtype, k_draft.device),
            None if out is None else (out.shape, out.stride(), out.dtype, out.device))
     plan = view.plans.get(key)
@@ -50,7 +52,8 @@ def attention_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedBatch, tre
         out = torch.empty(plan.shape, dtype=torch.float32, device=device)
     with _lib.on_device(device):
         args = plan.head + _WEIGHTS.pack(q.data_ptr(), *plan.q, cache.pool.kv.data_ptr() + plan.plane, plan.rows,
-                                         0 if k_draft is None else k_draft.data_ptr(), *plan.draft, lse.data_ptr(), plan.lse, out.data_ptr(), *plan.tail)
+                                         0 if k_draft is None else k_draft.data_ptr(), *plan.draft, lse.data_ptr(),
+                                         plan.lse, out.data_ptr(), *plan.tail)
         _lib.call("qe_attention_weights", args, _lib.stream_of(device))
     return out
 
