@@ -19,7 +19,11 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kKeys = 16;    // keys per tile
 constexpr int kQRows = 224;   // query rows in shared memory at a time, at most
-constexpr int kTcRows = 224;  // more query rows a K/V head than this: the tensor-memory kernel
+// More query rows a K/V head than this take the tensor-memory kernel. Its CTAs do one key tile each, so a large batch of
+// few rows pays for many starts (32 requests of 257 to 8,191 tokens: 112 rows 94 us here, 210 there; 210 rows 173, 237).
+// Where all the key tiles find an SM at once it is the faster one from fewer rows on (2,000 keys: 35 rows 5.6 us here,
+// 6.8 there; 63 rows 7.2, 6.7; 112 rows 10.1, 6.7; 12,000 keys, more than one tile an SM: 112 rows 15.4, 17.6).
+constexpr int kTcRows = 224, kTcRowsFewKeys = 56;
 
 struct WeightParams {
   DecodeBatch batch;
@@ -148,28 +152,43 @@ __global__ void __launch_bounds__(kWarps * 32) attention_weights_kernel(const We
         ldmatrix4(kf[k], ks + chunk_at<D>(((lane >> 3) & 1) * 8 + (lane & 7), 2 * k + (lane >> 4)));
       const bool draft_tile = t >= cached_tiles;
       float sum[2] = {0.0f, 0.0f};  // keys lane / 4 and lane / 4 + 8, this lane's columns
-      for (int nb = 0; nb < blocks; ++nb) {
-        float s[2][4] = {};  // even and odd k-steps, so that two products are under way
+      // kN blocks of eight rows at once: the products of a block are two chains, and chains are what a warp waits for
+      auto rows8 = [&](auto count, int nb) {
+        constexpr int kN = decltype(count)::value;
+        float s[kN][2][4] = {};  // even and odd k-steps
 #pragma unroll
         for (int k = 0; k < kSteps; k += 2) {
-          uint32_t qb[4];
-          ldmatrix4(qb, qs + chunk_at<D>(nb * 8 + (lane & 7), 2 * k + (lane >> 3)));
-          mma16816<T>(s[0], kf[k], qb[0], qb[1]);
-          mma16816<T>(s[1], kf[k + 1], qb[2], qb[3]);
-        }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = nb * 8 + (lane & 3) * 2 + e;
-          const float x = lse_s[r];
-          uint32_t bits = x != INFINITY ? 0xffffu : 0u;
-          if (draft_tile) bits &= draft_bits16(p.batch, rq, node_s[r], (t - cached_tiles) * kKeys);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float w = exp2_approx(fmaf(s[0][2 * h + e] + s[1][2 * h + e], p.scale_log2, -x));
-            if ((bits >> (lane / 4 + 8 * h)) & 1u) sum[h] += w;
+          for (int n = 0; n < kN; ++n) {
+            uint32_t qb[4];
+            ldmatrix4(qb, qs + chunk_at<D>((nb + n) * 8 + (lane & 7), 2 * k + (lane >> 3)));
+            mma16816<T>(s[n][0], kf[k], qb[0], qb[1]);
+            mma16816<T>(s[n][1], kf[k + 1], qb[2], qb[3]);
           }
         }
-      }
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          const int r = (nb + n) * 8 + (lane & 3) * 2;
+          const float2 x = *reinterpret_cast<const float2 *>(lse_s + r);
+          uint32_t bits[2] = {x.x != INFINITY ? 0xffffu : 0u, x.y != INFINITY ? 0xffffu : 0u};
+          if (draft_tile) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              bits[e] &= draft_bits16(p.batch, rq, node_s[r + e], (t - cached_tiles) * kKeys);
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float raw = s[n][0][2 * h + e] + s[n][1][2 * h + e];
+              const float w = exp2_approx(fmaf(raw, p.scale_log2, e ? -x.y : -x.x));
+              sum[h] += (bits[e] >> (lane / 4 + 8 * h)) & 1u ? w : 0.0f;
+            }
+        }
+      };
+      int nb = 0;  // three at once: 210 rows 206 -> 174 us, and four cost registers
+      for (; nb + 3 <= blocks; nb += 3) rows8(std::integral_constant<int, 3>{}, nb);
+      for (; nb < blocks; ++nb) rows8(std::integral_constant<int, 1>{}, nb);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
@@ -643,7 +662,8 @@ extern "C" int qe_attention_weights(const qe_attention_weights_args *args, void 
   }
   p.tiles_per_cta = int(per);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int64_t(batch.max_nodes) * p.group > kTcRows && p.group <= kTile) {
+  const bool few_keys = all * heads_kv <= int64_t(sm_count()) * (kTile / kKeys);
+  if (int64_t(batch.max_nodes) * p.group > (few_keys ? kTcRowsFewKeys : kTcRows) && p.group <= kTile) {
     QE_CHECK_ARG(int64_t(heads_kv) * batch.batch <= 65535 && (max_tiles + 7) / 8 < 65535,
                  "qe_attention_weights: too many requests x heads_kv, or keys, for one launch");
     if (dtype == 1)

@@ -104,6 +104,14 @@ def test_weights_either_side_of_the_kernels_border(kind, n):
     _run([900, 0, 129], [n, 3, n - 1], 28, 4, 128, torch.bfloat16, 64, kind, seed=n)
 
 
+@pytest.mark.parametrize("kind", ["chain", "tree"])
+@pytest.mark.parametrize("n", [8, 9, 16, 31, 32, 33])
+def test_weights_of_middle_rows_over_few_and_many_keys(kind, n):
+    """The border moves with the keys: few of them (every tile finds an SM) and many, at the same rows."""
+    _run([900, 0, 129], [n, 3, n - 1], 28, 4, 128, torch.float16, 64, kind, seed=n)
+    _run([4100, 0, 129, 1203], [n, 3, n - 1, n], 28, 4, 128, torch.bfloat16, 16, kind, seed=n)
+
+
 def test_weights_accumulate_into_a_wider_buffer():
     lens, counts, rooms = [130, 40], [2, 1], [200, 64]
     pool, slots, q, kn = _case(lens, counts, 28, 4, 128, torch.bfloat16, 64, 3, rooms=rooms)
