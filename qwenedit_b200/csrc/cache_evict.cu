@@ -17,9 +17,9 @@ namespace {
 // of a row of up to 73,728 positions stay on the SM, in registers (to 32,768) and shared memory, read once with the
 // loads in flight together; a longer row is read again in each pass (from L2), eight loads at a time. Digits are 11, 11
 // and 10 bits: the first holds the sign, the exponent and two mantissa bits, so that weights spread over some octaves
-// meet in one counter a few at a time; a pass whose digit is kept whole ends the search. What bounds it is instructions,
-// about 90 a warp per 32 positions over all the passes, at 0.6 of the issue rate (1,792 rows of 3,001 to 32,749: 187 us,
-// 0.13 of the copy rate).
+// meet in one counter a few at a time; a pass whose digit is kept whole ends the search. What bounds it is instructions
+// over all the passes and, with one row an SM, the waits of its start and barriers (1,792 rows of 3,001 to 32,749: 144
+// us, 0.17 of the copy rate).
 
 struct HeaviestParams {
   const float *weights;
@@ -38,10 +38,21 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
 }
 
+// The weight a key stands for; false where that is more than one (NaN and -inf, the zeros).
+__device__ __forceinline__ bool weight_of(uint32_t key, float *x) {
+  *x = __uint_as_float(key >> 31 ? key ^ 0x80000000u : ~key);
+  return key != 0x80000000u && key != 0x007fffffu;
+}
+
 // kItems > 0: up to kItems positions a thread in registers, kStored more in shared memory; 0: any number.
 template <int kThreads, int kItems, int kStored>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(const HeaviestParams p) {
   constexpr int kWarps = kThreads / 32, kBins = 2048, kPer = kBins / kThreads;  // counters per thread
+  // positions a lane handles without a branch between: one 187 us, two and four 156, eight 171 (1,792 rows)
+  constexpr int kGroup = kItems > 0 ? 4 : 8;
+  // Lower digits of many positions: only those of the prefix reach a counter (156 -> 144 us; 100 rows of 60,000: 33 ->
+  // 26). Of few, all lanes add, the others nothing, without a branch (112 rows of 4,096: 7.4 us, 7.7 with it).
+  constexpr bool kSkip = kItems == 0 || kItems > 16;
   extern __shared__ uint32_t stored[];  // [kStored][kThreads]
   __shared__ int hists[3][kBins];
   __shared__ int warp_sum[kWarps], warp_at[kWarps];
@@ -77,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
     };
 #pragma unroll
     for (int j = 0; j < kItems; ++j)
-      if (j < steps) held[j] = bits_at(j);
+      if (j / kGroup * kGroup < steps) held[j] = bits_at(j);
     for (int j0 = 0; j0 < kStored; j0 += 8) {
       if (kItems + j0 >= steps) break;
       uint32_t x[8];
@@ -88,32 +99,44 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
     }
 #pragma unroll
     for (int j = 0; j < kItems; ++j)
-      if (j < steps) held[j] = key_at(j, held[j]);
+      if (j / kGroup * kGroup < steps) held[j] = key_at(j, held[j]);
   }
-  // calls f(key, position) for the warp's run, 32 neighbours at a time (key 0: no position there)
-  auto each = [&](auto f) {
+  // calls f(keys, position of the first) for the warp's run, kGroup times 32 neighbours at a time (key 0: no position)
+  auto groups = [&](auto f) {
+    uint32_t k[kGroup];
     if (kItems > 0) {
 #pragma unroll
-      for (int j = 0; j < kItems; ++j)
-        if (j < steps) f(held[j], from + j * 32 + lane);
-      if (kStored > 0)
-#pragma unroll 8
-        for (int j = kItems; j < steps; ++j) f(stored[(j - kItems) * kThreads + tid], from + j * 32 + lane);
-    } else {
-      for (int j0 = 0; j0 < steps; j0 += 8) {
-        uint32_t k[8];
+      for (int j = 0; j < kItems; j += kGroup)
+        if (j < steps) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int i = from + (j0 + u) * 32 + lane;
+          for (int u = 0; u < kGroup; ++u) k[u] = held[j + u];
+          f(k, from + j * 32 + lane);
+        }
+      if (kStored > 0)
+        for (int j = kItems; j < steps; j += kGroup) {
+#pragma unroll
+          for (int u = 0; u < kGroup; ++u) k[u] = stored[(j - kItems + u) * kThreads + tid];
+          f(k, from + j * 32 + lane);
+        }
+    } else {
+      for (int j = 0; j < steps; j += kGroup) {
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {
+          const int i = from + (j + u) * 32 + lane;
           k[u] = i < to ? __float_as_uint(__ldg(mid + i)) : 0u;
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int i = from + (j0 + u) * 32 + lane;
-          f(i < to ? order_key(__uint_as_float(k[u])) : 0u, i);
-        }
+        for (int u = 0; u < kGroup; ++u)
+          k[u] = from + (j + u) * 32 + lane < to ? order_key(__uint_as_float(k[u])) : 0u;
+        f(k, from + j * 32 + lane);
       }
     }
+  };
+  auto each = [&](auto f) {
+    groups([&](const uint32_t(&k)[kGroup], int) {
+#pragma unroll
+      for (int u = 0; u < kGroup; ++u) f(k[u]);
+    });
   };
   // this warp's place in sums over the warps (every warp adds up all of them)
   auto before_warp = [&](const int *sums) {
@@ -141,10 +164,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
     const int shift = kShift[pass];
     int *hist = hists[pass];
     if (pass == 0) __syncthreads();
-    each([&](uint32_t k, int) {  // no position: a key below every real one, counted where no threshold can be
-      // every lane adds, those of other prefixes nothing: no branch, and low digits seldom meet
-      atomicAdd(&hist[(k >> shift) & ((1u << kBits[pass]) - 1u)],
-                pass == 0 || (k >> (shift + kBits[pass])) == prefix ? 1 : 0);
+    each([&](uint32_t k) {  // no position: a key below every real one, counted where no threshold can be
+      int *counter = &hist[(k >> shift) & ((1u << kBits[pass]) - 1u)];
+      const bool counts = pass == 0 || (k >> (shift + kBits[pass])) == prefix;
+      if (!kSkip) atomicAdd(counter, counts ? 1 : 0);
+      else if (counts) atomicAdd(counter, 1);
     });
     __syncthreads();
     // the digit at which the count from the top reaches `need`: thread t sums counters kBins - 1 - kPer t and below
@@ -184,12 +208,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
   const uint32_t threshold = prefix << low, least = cut ? threshold + 1 : threshold;  // a cut threshold is a whole key
   int above = 0, at = 0;
   if (cut)
-    each([&](uint32_t k, int) {
+    each([&](uint32_t k) {
       above += k >= least;
       at += k == threshold;
     });
   else
-    each([&](uint32_t k, int) { above += k >= least; });
+    each([&](uint32_t k) { above += k >= least; });
   above = __reduce_add_sync(0xffffffffu, above);
   at = __reduce_add_sync(0xffffffffu, at);
   if (lane == 0) {
@@ -200,21 +224,34 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
   above = before_warp(warp_sum);
   at = before_warp(warp_at);
   const uint32_t below = (1u << lane) - 1u;
-  each([&](uint32_t k, int i) {
-    bool take = k >= least;
-    const uint32_t up = __ballot_sync(0xffffffffu, take);
-    int place = above + __popc(up & below);
-    above += __popc(up);
-    if (cut) {
-      const uint32_t eq = __ballot_sync(0xffffffffu, k == threshold);
-      const int mine = at + __popc(eq & below);
-      take = take || (k == threshold && mine < need);
-      place += min(mine, need);
-      at += __popc(eq);
+  auto put = [&](uint32_t k, int place, int i) {
+    keep[p.sinks + place] = lo + i;
+    if (kept) {
+      float x;
+      kept[p.sinks + place] = weight_of(k, &x) ? x : __ldg(mid + i);
     }
-    if (take) {
-      keep[p.sinks + place] = lo + i;
-      if (kept) kept[p.sinks + place] = __ldg(mid + i);
+  };
+  groups([&](const uint32_t(&k)[kGroup], int i) {
+    int place[kGroup];
+#pragma unroll
+    for (int u = 0; u < kGroup; ++u) {
+      const uint32_t up = __ballot_sync(0xffffffffu, k[u] >= least);
+      place[u] = above + __popc(up & below);
+      above += __popc(up);
+    }
+    if (cut) {
+#pragma unroll
+      for (int u = 0; u < kGroup; ++u) {
+        const uint32_t eq = __ballot_sync(0xffffffffu, k[u] == threshold);
+        const int mine = at + __popc(eq & below);
+        at += __popc(eq);
+        place[u] += min(mine, need);
+        if (k[u] >= least || (k[u] == threshold && mine < need)) put(k[u], place[u], i + u * 32);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kGroup; ++u)
+        if (k[u] >= least) put(k[u], place[u], i + u * 32);
     }
   });
 }
