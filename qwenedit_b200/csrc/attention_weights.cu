@@ -19,10 +19,10 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kKeys = 16;    // keys per tile
 constexpr int kQRows = 224;   // query rows in shared memory at a time, at most
-// More query rows a K/V head than this take the tensor-memory kernel. Its CTAs do one key tile each, so a large batch of
-// few rows pays for many starts (32 requests of 257 to 8,191 tokens: 112 rows 94 us here, 210 there; 210 rows 173, 237).
-// Where all the key tiles find an SM at once it is the faster one from fewer rows on (2,000 keys: 35 rows 5.6 us here,
-// 6.8 there; 63 rows 7.2, 6.7; 112 rows 10.1, 6.7; 12,000 keys, more than one tile an SM: 112 rows 15.4, 17.6).
+// More query rows a K/V head than this take the tensor-memory kernel. Its CTAs do one key tile each, so a large batch
+// of few rows pays for many starts (32 requests of 257 to 8,191 tokens: 112 rows 94 us here, 210 there; 210 rows 173,
+// 237). Where all the key tiles find an SM at once it is the faster one from fewer rows on (2,000 keys: 35 rows 5.6 us
+// here, 6.8 there; 63 rows 7.2, 6.7; 112 rows 10.1, 6.7; 12,000 keys, more than a tile an SM: 112 rows 15.4, 17.6).
 constexpr int kTcRows = 224, kTcRowsFewKeys = 56;
 
 struct WeightParams {
@@ -662,7 +662,7 @@ extern "C" int qe_attention_weights(const qe_attention_weights_args *args, void 
   }
   p.tiles_per_cta = int(per);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool few_keys = all * heads_kv <= int64_t(sm_count()) * (kTile / kKeys);
+  const bool few_keys = std::max<int64_t>(all, batch.batch) * heads_kv <= int64_t(sm_count()) * (kTile / kKeys);
   if (int64_t(batch.max_nodes) * p.group > (few_keys ? kTcRowsFewKeys : kTcRows) && p.group <= kTile) {
     QE_CHECK_ARG(int64_t(heads_kv) * batch.batch <= 65535 && (max_tiles + 7) / 8 < 65535,
                  "qe_attention_weights: too many requests x heads_kv, or keys, for one launch");

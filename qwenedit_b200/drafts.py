@@ -230,6 +230,15 @@ def _check_rows(name: str, t: torch.Tensor, n: int, heads: int, head_dim: int, d
         raise ValueError(f"{name} must be [at least {n} tokens, {heads} heads, {head_dim}] with contiguous head rows")
 
 
+def _check_apart(t: torch.Tensor) -> None:
+    """An output's rows (its last dimension) must not share memory: several of them are written at once."""
+    end = t.shape[-1]
+    for step, n in sorted((t.stride(i), t.shape[i]) for i in range(t.dim() - 1) if t.shape[i] > 1):
+        if step < end:
+            raise ValueError("out must not have rows that overlap")
+        end += step * (n - 1)
+
+
 def _check_pool(cache: PagedBatch, layer: int):
     pool = cache.pool
     if pool.kv.dtype not in DTYPES or pool.head_dim not in HEAD_DIMS:
@@ -299,6 +308,7 @@ class _TreePlan:
             self.draft = (2 * k_draft.stride(0), 2 * k_draft.stride(1))
         if out is not None:
             _check_rows("out", out, total, heads_q, d, kv.dtype, device)
+            _check_apart(out)
         self.device, self.exact, self.head = device, q.shape[0] == total, view.batch
         self.q, self.rows = (2 * q.stride(0), 2 * q.stride(1)), pool.rows
         self.plane, self.to_v = 2 * layer * kv.stride(0), 2 * kv.stride(1)

@@ -19,7 +19,7 @@ import math
 import torch
 
 from qwenedit_b200 import _lib
-from qwenedit_b200.drafts import DTYPES, DraftTree, PagedBatch, _check_pool, _check_rows, _view
+from qwenedit_b200.drafts import DTYPES, DraftTree, PagedBatch, _check_apart, _check_pool, _check_rows, _view
 
 
 def attention_weights(q: torch.Tensor, lse: torch.Tensor, cache: PagedBatch, tree: DraftTree, layer: int = 0,
@@ -91,8 +91,7 @@ class _WeightsPlan:
                 raise ValueError(f"out must be [{cache.batch}, {heads_kv}, at least {width}] float32 on {device} with "
                                  "contiguous rows")
             width = out.shape[2]
-            if (cache.batch > 1 and abs(strides[0]) < width) or (heads_kv > 1 and abs(strides[1]) < width):
-                raise ValueError("out must not have rows that overlap")
+            _check_apart(out)
         self.device, self.head, self.shape, self.lse = device, view.batch, (cache.batch, heads_kv, width), lse.stride(0)
         self.q, self.plane, self.rows = (2 * q.stride(0), 2 * q.stride(1)), 2 * layer * kv.stride(0), pool.rows
         self.tail = (strides[0], strides[1], width, pool._err.data_ptr(), heads_q, heads_kv, d, DTYPES[kv.dtype],

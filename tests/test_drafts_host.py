@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from qwenedit_b200 import _lib
-from qwenedit_b200.drafts import DraftTree, PagedBatch, tree_attention
+from qwenedit_b200.drafts import DraftTree, PagedBatch, _check_apart, tree_attention
 from qwenedit_b200.evict import attention_weights, heaviest
 from qwenedit_b200.paged import PagedKVPool
 
@@ -79,6 +79,17 @@ def test_tree_attention_refuses_before_any_launch():
         tree_attention(*_args(_pool(dtype=torch.float32)))
     with pytest.raises(ValueError, match="bf16 or fp16 heads"):
         tree_attention(*_args(_pool(d=32)))
+
+
+def test_outputs_must_not_overlap_themselves():
+    x = torch.zeros(10_000)
+    for sizes, strides in [((3, 2, 64), (128, 64, 1)), ((3, 2, 64), (64, 192, 1)), ((2, 3, 50), (300, 64, 1)),
+                           ((1, 1, 64), (0, 0, 1)), ((1, 4, 64), (3, 64, 1)), ((0, 4, 64), (0, 64, 1))]:
+        _check_apart(x.as_strided(sizes, strides))
+    for sizes, strides in [((3, 2, 64), (64, 64, 1)), ((3, 2, 64), (0, 64, 1)), ((3, 2, 64), (128, 63, 1)),
+                           ((3, 2, 64), (64, 128, 1)), ((2, 3, 50), (130, 50, 1))]:
+        with pytest.raises(ValueError, match="overlap"):
+            _check_apart(x.as_strided(sizes, strides))
 
 
 def test_weights_refuse_before_any_launch():

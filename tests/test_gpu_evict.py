@@ -92,7 +92,8 @@ def test_weights_of_a_prompt(n, length, d, dtype):
     _run([length], [n], 4, 2, d, dtype, 16, seed=n)
 
 
-@pytest.mark.parametrize("counts,hq,hkv", [([3, 2], 132, 1), ([2], 260, 1), ([3, 40], 100, 1), ([2], 128, 1)])
+@pytest.mark.parametrize("counts,hq,hkv", [([3, 2], 132, 1), ([2], 260, 1), ([3, 40], 100, 1), ([2], 128, 1),
+                                            ([1], 64, 1), ([1, 1], 100, 1), ([1, 0], 256, 2)])
 def test_weights_of_large_groups(counts, hq, hkv):
     _run([300, 17][: len(counts)], counts, hq, hkv, 64, torch.bfloat16, 16, seed=hq)
 
@@ -110,6 +111,18 @@ def test_weights_of_middle_rows_over_few_and_many_keys(kind, n):
     """The border moves with the keys: few of them (every tile finds an SM) and many, at the same rows."""
     _run([900, 0, 129], [n, 3, n - 1], 28, 4, 128, torch.float16, 64, kind, seed=n)
     _run([4100, 0, 129, 1203], [n, 3, n - 1, n], 28, 4, 128, torch.bfloat16, 16, kind, seed=n)
+
+
+def test_outputs_whose_rows_overlap_are_refused():
+    pool, slots, q, kn = _case([20, 9], [1, 1], 4, 2, 64, torch.bfloat16, 16, 0)
+    cache, tree = PagedBatch(pool, slots), DraftTree([1, 1])
+    lse = torch.zeros(4, 2, device=DEV)
+    store = torch.zeros(1000, device=DEV)
+    with pytest.raises(ValueError, match="overlap"):
+        attention_weights(q, lse, cache, tree, 0, kn, out=store.as_strided((2, 2, 21), (24, 24, 1)))
+    same = torch.zeros(1, 4, 64, dtype=torch.bfloat16, device=DEV).expand(2, 4, 64)
+    with pytest.raises(ValueError, match="overlap"):
+        tree_attention(q, cache, tree, 0, kn, kn, out=same)
 
 
 def test_weights_accumulate_into_a_wider_buffer():
