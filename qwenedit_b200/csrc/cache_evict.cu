@@ -15,11 +15,12 @@ namespace {
 // Per row the key (an order-preserving integer) of the last position kept, by radix selection from the top bits, then
 // one ordered pass that writes the kept positions. A CTA per row, each warp a run of neighbouring positions. The keys
 // of a row of up to 73,728 positions stay on the SM, in registers (to 32,768) and shared memory, read once with the
-// loads in flight together; a longer row is read again in each pass (from L2), eight loads at a time. Digits are 11, 11
+// loads in flight together; longer rows are shared by the CTAs of a cluster, which past 8 x 73,728 positions read them
+// again in each pass (from L2), eight loads at a time. Digits are 11, 11
 // and 10 bits: the first holds the sign, the exponent and two mantissa bits, so that weights spread over some octaves
 // meet in one counter a few at a time; a pass whose digit is kept whole ends the search. What bounds it is instructions
 // over all the passes and, with one row an SM, the waits of its start and barriers (1,792 rows of 3,001 to 32,749: 144
-// us, 0.17 of the copy rate).
+// us, 0.17 of the copy rate). Few long rows: a cluster per row, counters added up over distributed shared memory.
 
 struct HeaviestParams {
   const float *weights;
@@ -27,7 +28,7 @@ struct HeaviestParams {
   const int32_t *lengths;
   int32_t *keep;
   float *kept;
-  int width, budget, sinks, recent;
+  int width, budget, sinks, recent, parts;
 };
 
 // Order-preserving map of fp32 to uint32: NaN as -inf, -0 as +0, so that equal weights are equal keys. Never 0, which
@@ -45,7 +46,8 @@ __device__ __forceinline__ bool weight_of(uint32_t key, float *x) {
 }
 
 // kItems > 0: up to kItems positions a thread in registers, kStored more in shared memory; 0: any number.
-template <int kThreads, int kItems, int kStored>
+// kSplit: a cluster's CTAs share a row, a part of the positions each, and read each other's counters.
+template <int kThreads, int kItems, int kStored, bool kSplit>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(const HeaviestParams p) {
   constexpr int kWarps = kThreads / 32, kBins = 2048, kPer = kBins / kThreads;  // counters per thread
   // positions a lane handles without a branch between: one 187 us, two and four 156, eight 171 (1,792 rows)
@@ -54,17 +56,18 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
   // 26). Of few, all lanes add, the others nothing, without a branch (112 rows of 4,096: 7.4 us, 7.7 with it).
   constexpr bool kSkip = kItems == 0 || kItems > 16;
   extern __shared__ uint32_t stored[];  // [kStored][kThreads]
-  __shared__ int hists[3][kBins];
+  __shared__ __align__(16) int hists[3][kBins];
   __shared__ int warp_sum[kWarps], warp_at[kWarps];
   __shared__ int found[3];  // digit, positions above it, positions at it
-  const int64_t row = blockIdx.x;
+  const int parts = kSplit ? p.parts : 1, part = kSplit ? int(blockIdx.x % unsigned(parts)) : 0;
+  const int64_t row = blockIdx.x / unsigned(parts);
   const float *w = p.weights + row / (p.n1 * p.n2) * p.s0 + row / p.n2 % p.n1 * p.s1 + row % p.n2 * p.s2;
   int32_t *keep = p.keep + row * p.budget;
   float *kept = p.kept ? p.kept + row * p.budget : nullptr;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n = p.lengths ? min(max(p.lengths[row], 0), p.width) : p.width;
   if (n <= p.budget) {  // all of them
-    for (int i = tid; i < p.budget; i += kThreads) {
+    for (int i = part * kThreads + tid; i < p.budget; i += parts * kThreads) {
       keep[i] = i < n ? i : -1;
       if (kept) kept[i] = i < n ? w[i] : 0.0f;
     }
@@ -74,8 +77,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
   const float *mid = w + lo;
   const int count = hi - lo;
   // this warp's run [from, to) of the positions between, `steps` times 32
-  const int run = (count + kThreads - 1) / kThreads * 32;
-  const int from = warp * run, to = min(count, from + run);
+  const int run = (count + kThreads * parts - 1) / (kThreads * parts) * 32;
+  const int from = (part * kWarps + warp) * run, to = min(count, from + run);
   const int steps = to > from ? (to - from + 31) / 32 : 0;
   uint32_t held[kItems > 0 ? kItems : 1];
   if (kItems > 0) {
@@ -143,13 +146,27 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
     int x = lane < kWarps && lane < warp ? sums[lane] : 0;
     return __reduce_add_sync(0xffffffffu, x);
   };
+  auto before_part = [&](const int *sums) {
+    int x = 0;
+    for (int r = 0; r < part; ++r)
+      x += lane < kWarps ? __float_as_int(ld_cluster1(smem_u32(sums + lane), uint32_t(r))) : 0;
+    return __reduce_add_sync(0xffffffffu, x);
+  };
+  auto sync_row = [&] {  // all threads of the row
+    if (kSplit) {
+      __syncwarp();
+      cluster_sync();
+    } else {
+      __syncthreads();
+    }
+  };
 #pragma unroll
   for (int e = 0; e < 3 * kPer; ++e) hists[0][e * kThreads + tid] = 0;
-  for (int i = tid; i < p.sinks; i += kThreads) {
+  for (int i = part * kThreads + tid; i < p.sinks; i += parts * kThreads) {
     keep[i] = i;
     if (kept) kept[i] = w[i];
   }
-  for (int i = tid; i < p.recent; i += kThreads) {
+  for (int i = part * kThreads + tid; i < p.recent; i += parts * kThreads) {
     keep[p.budget - p.recent + i] = hi + i;
     if (kept) kept[p.budget - p.recent + i] = w[hi + i];
   }
@@ -170,11 +187,32 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
       if (!kSkip) atomicAdd(counter, counts ? 1 : 0);
       else if (counts) atomicAdd(counter, 1);
     });
-    __syncthreads();
+    sync_row();
     // the digit at which the count from the top reaches `need`: thread t sums counters kBins - 1 - kPer t and below
     int c[kPer], mine = 0;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) mine += c[e] = hist[kBins - 1 - (tid * kPer + e)];
+    for (int e = 0; e < kPer; ++e) c[e] = hist[kBins - 1 - (tid * kPer + e)];
+    if (kSplit)  // and the other parts'
+      for (int x = 1; x < parts; ++x) {
+        const uint32_t r = uint32_t(part + x) % uint32_t(parts);
+#pragma unroll
+        for (int e = 0; e < kPer; e += kPer < 4 ? 2 : 4) {
+          const uint32_t at = smem_u32(hist + kBins - tid * kPer - e - (kPer < 4 ? 2 : 4));
+          if constexpr (kPer < 4) {
+            const float2 v = ld_cluster2(at, r);
+            c[e] += __float_as_int(v.y);
+            c[e + 1] += __float_as_int(v.x);
+          } else {
+            const float4 v = ld_cluster4(at, r);
+            c[e] += __float_as_int(v.w);
+            c[e + 1] += __float_as_int(v.z);
+            c[e + 2] += __float_as_int(v.y);
+            c[e + 3] += __float_as_int(v.x);
+          }
+        }
+      }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) mine += c[e];
     int upto = mine;
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) {
@@ -220,9 +258,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
     warp_sum[warp] = above;
     warp_at[warp] = at;
   }
-  __syncthreads();
+  sync_row();
   above = before_warp(warp_sum);
   at = before_warp(warp_at);
+  if (kSplit) {
+    above += before_part(warp_sum);
+    at += before_part(warp_at);
+  }
   const uint32_t below = (1u << lane) - 1u;
   auto put = [&](uint32_t k, int place, int i) {
     keep[p.sinks + place] = lo + i;
@@ -254,6 +296,35 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) heaviest_kernel(con
         if (k[u] >= least) put(k[u], place[u], i + u * 32);
     }
   });
+  if (kSplit) sync_row();  // nobody leaves while its counters are read
+}
+
+template <int kThreads, int kItems, int kStored, bool kSplit>
+int run_heaviest(const HeaviestParams &p, int64_t rows, cudaStream_t stream) {
+  auto kernel = heaviest_kernel<kThreads, kItems, kStored, kSplit>;
+  constexpr int kBytes = kStored * kThreads * 4;
+  if (kBytes > 0) {
+    static std::atomic<bool> raised[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (!raised[dev].load(std::memory_order_relaxed)) {
+      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+      if (e != cudaSuccess) return cuda_status(e, "qe_heaviest: smem attribute");
+      raised[dev].store(true, std::memory_order_relaxed);
+    }
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(rows * p.parts));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(p.parts);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = kSplit ? 1 : 0;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p), "qe_heaviest launch");
 }
 
 // ---- retain -----------------------------------------------------------------------------------------------------
@@ -349,36 +420,36 @@ extern "C" int qe_heaviest(const float *weights, int64_t n0, int64_t n1, int64_t
   QE_CHECK_ARG(rows < (int64_t(1) << 31), "qe_heaviest: too many rows");
   if (rows == 0 || budget == 0) return ok();
   QE_CHECK_ARG((weights || width == 0) && keep, "qe_heaviest: null weights or keep");
-  HeaviestParams p{weights, n1, n2, s0, s1, s2, lengths, keep, kept, int(width), int(budget), int(sinks), int(recent)};
-  const unsigned n = unsigned(rows);
+  HeaviestParams p{weights,    n1,         n2,         s0,          s1, s2, lengths, keep, kept,
+                   int(width), int(budget), int(sinks), int(recent), 1};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t mid = width - sinks - recent;  // at most
-  if (mid <= 1024) {
-    heaviest_kernel<256, 4, 0><<<n, 256, 0, st>>>(p);
-  } else if (mid <= 4096) {
-    heaviest_kernel<256, 16, 0><<<n, 256, 0, st>>>(p);
-  } else if (mid <= 8192) {
-    heaviest_kernel<512, 16, 0><<<n, 512, 0, st>>>(p);
-  } else if (mid <= 16384) {
-    heaviest_kernel<512, 32, 0><<<n, 512, 0, st>>>(p);
-  } else if (mid <= 32768) {
-    heaviest_kernel<1024, 32, 0><<<n, 1024, 0, st>>>(p);
-  } else if (mid <= 73728) {
-    constexpr int kStored = 48, kBytes = kStored * 1024 * 4;
-    auto kernel = heaviest_kernel<1024, 24, kStored>;
-    static std::atomic<bool> raised[64];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
-    if (!raised[dev].load(std::memory_order_relaxed)) {
-      cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-      if (e != cudaSuccess) return cuda_status(e, "qe_heaviest: smem attribute");
-      raised[dev].store(true, std::memory_order_relaxed);
-    }
-    kernel<<<n, 1024, kBytes, st>>>(p);
+  int64_t mid = std::max<int64_t>(1, width - sinks - recent);  // at most
+  // Few long rows are split over clusters, in parts of more than 4,096 positions (28 rows of 16,000: one part 11.9 us,
+  // two 11.3, four 14.4; of 37,655: 18.7 / 15.2 / 14.1 / eight 20.4; of 65,000: 24.5 / 17.2 / 15.2 / 19.8), over eight
+  // only where four would not hold a row's keys in registers. Many are not (112 rows of 37,655: 19.9 us whole, 28.6 in
+  // halves), but where a row's keys do not fit on one SM (28 rows of 200,000: 134 us whole, 28 split; 112: 163, 111; 896
+  // of 100,000: 472, 342).
+  while (p.parts < 8 && ((rows * p.parts * 2 <= sm_count() &&
+                          mid > int64_t(p.parts) * (p.parts < 4 ? 8192 : 32768)) ||
+                         (rows < (1 << 27) && mid > int64_t(p.parts) * 73728)))
+    p.parts *= 2;
+  mid = (mid + p.parts - 1) / p.parts;
+  int s;
+  if (p.parts > 1) {
+    s = mid <= 8192    ? run_heaviest<512, 16, 0, true>(p, rows, st)
+        : mid <= 16384 ? run_heaviest<512, 32, 0, true>(p, rows, st)
+        : mid <= 32768 ? run_heaviest<1024, 32, 0, true>(p, rows, st)
+        : mid <= 73728 ? run_heaviest<1024, 24, 48, true>(p, rows, st)
+                       : run_heaviest<1024, 0, 0, true>(p, rows, st);
   } else {
-    heaviest_kernel<1024, 0, 0><<<n, 1024, 0, st>>>(p);
+    s = mid <= 1024    ? run_heaviest<256, 4, 0, false>(p, rows, st)
+        : mid <= 4096  ? run_heaviest<256, 16, 0, false>(p, rows, st)
+        : mid <= 8192  ? run_heaviest<512, 16, 0, false>(p, rows, st)
+        : mid <= 16384 ? run_heaviest<512, 32, 0, false>(p, rows, st)
+        : mid <= 32768 ? run_heaviest<1024, 32, 0, false>(p, rows, st)
+        : mid <= 73728 ? run_heaviest<1024, 24, 48, false>(p, rows, st)
+                       : run_heaviest<1024, 0, 0, false>(p, rows, st);
   }
-  const int s = cuda_status(cudaGetLastError(), "qe_heaviest launch");
   return s ? s : ok();
 }
 

@@ -169,6 +169,14 @@ __device__ __forceinline__ float ld_cluster1(uint32_t local, uint32_t rank) {
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_at(local, rank)) : "memory");
   return v;
 }
+__device__ __forceinline__ float2 ld_cluster2(uint32_t local, uint32_t rank) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(cluster_at(local, rank))
+               : "memory");
+  return v;
+}
 __device__ __forceinline__ float4 ld_cluster4(uint32_t local, uint32_t rank) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"

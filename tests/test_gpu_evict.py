@@ -256,6 +256,20 @@ def test_heaviest_lengths_and_strides():
     assert bool((keep[1] == -1).all()) and not kept[1].any()
 
 
+@pytest.mark.parametrize("rows,width", [(7, 8193), (70, 16385), (74, 140003), (18, 140003), (3, 300001), (75, 40000),
+                                        (80, 90001),                                        (2, 600011)])
+def test_heaviest_rows_shared_by_several_blocks(rows, width):
+    g = torch.Generator(device=DEV).manual_seed(width)
+    w = torch.rand(rows, width, generator=g, device=DEV)
+    w[0] = (w[0] * 5).floor()  # ties past every part's border
+    lengths = torch.randint(0, width + 1, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    lengths[0], lengths[1] = width, 300
+    _check_heaviest(w, 1000, lengths, 4, 31)
+    _check_heaviest(w[:2], width // 3, lengths[:2], 0, 5)
+    keep, _ = heaviest(w, 700, lengths, 400, 300)  # nothing left to choose
+    assert keep[0].tolist() == list(range(400)) + list(range(width - 300, width))
+
+
 def test_heaviest_many_rows_and_none():
     g = torch.Generator(device=DEV).manual_seed(3)
     _check_heaviest(torch.rand(300, 257, generator=g, device=DEV), 100, sinks=4, recent=16)
