@@ -15,12 +15,12 @@ namespace {
 // Per row the key (an order-preserving integer) of the last position kept, by radix selection from the top bits, then
 // one ordered pass that writes the kept positions. A CTA per row, each warp a run of neighbouring positions. The keys
 // of a row of up to 73,728 positions stay on the SM, in registers (to 32,768) and shared memory, read once with the
-// loads in flight together; longer rows are shared by the CTAs of a cluster, which past 8 x 73,728 positions read them
-// again in each pass (from L2), eight loads at a time. Digits are 11, 11
-// and 10 bits: the first holds the sign, the exponent and two mantissa bits, so that weights spread over some octaves
-// meet in one counter a few at a time; a pass whose digit is kept whole ends the search. What bounds it is instructions
-// over all the passes and, with one row an SM, the waits of its start and barriers (1,792 rows of 3,001 to 32,749: 144
-// us, 0.17 of the copy rate). Few long rows: a cluster per row, counters added up over distributed shared memory.
+// loads in flight together; longer rows, and a few long ones, are shared by the CTAs of a cluster, which add up their
+// counters over distributed shared memory and past 8 x 73,728 positions read the row again in each pass (from L2),
+// eight loads at a time. Digits are 11, 11 and 10 bits: the first holds the sign, the exponent and two mantissa bits,
+// so that weights spread over some octaves meet in one counter a few at a time; a pass whose digit is kept whole ends
+// the search. What bounds it is instructions over all the passes and, with one row an SM, the waits of its start and
+// barriers (1,792 rows of 3,001 to 32,749: 144 us, 0.17 of the copy rate).
 
 struct HeaviestParams {
   const float *weights;
@@ -424,15 +424,16 @@ extern "C" int qe_heaviest(const float *weights, int64_t n0, int64_t n1, int64_t
                    int(width), int(budget), int(sinks), int(recent), 1};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int64_t mid = std::max<int64_t>(1, width - sinks - recent);  // at most
-  // Few long rows are split over clusters, in parts of more than 4,096 positions (28 rows of 16,000: one part 11.9 us,
-  // two 11.3, four 14.4; of 37,655: 18.7 / 15.2 / 14.1 / eight 20.4; of 65,000: 24.5 / 17.2 / 15.2 / 19.8), over eight
-  // only where four would not hold a row's keys in registers. Many are not (112 rows of 37,655: 19.9 us whole, 28.6 in
-  // halves), but where a row's keys do not fit on one SM (28 rows of 200,000: 134 us whole, 28 split; 112: 163, 111; 896
-  // of 100,000: 472, 342).
+  // Few long rows are split over clusters, in parts of more than 4,096 positions (28 rows of 16,000: one part 11.9
+  // us, two 11.3, four 14.4; of 37,655: 18.7 / 15.2 / 14.1 / eight 20.4; of 65,000: 24.5 / 17.2 / 15.2 / 19.8), over
+  // eight only where four would not hold a row's keys in registers. Many are not (112 rows of 37,655: 19.9 us whole,
+  // 28.6 in halves), but where a row's keys do not fit on one SM (28 rows of 200,000: 134 us whole, 28 split; 112:
+  // 163, 111; 896 of 100,000: 472, 342).
   while (p.parts < 8 && ((rows * p.parts * 2 <= sm_count() &&
                           mid > int64_t(p.parts) * (p.parts < 4 ? 8192 : 32768)) ||
-                         (rows < (1 << 27) && mid > int64_t(p.parts) * 73728)))
+                         mid > int64_t(p.parts) * 73728))
     p.parts *= 2;
+  QE_CHECK_ARG(rows * p.parts < (int64_t(1) << 31), "qe_heaviest: too many rows");
   mid = (mid + p.parts - 1) / p.parts;
   int s;
   if (p.parts > 1) {
@@ -447,8 +448,7 @@ extern "C" int qe_heaviest(const float *weights, int64_t n0, int64_t n1, int64_t
         : mid <= 8192  ? run_heaviest<512, 16, 0, false>(p, rows, st)
         : mid <= 16384 ? run_heaviest<512, 32, 0, false>(p, rows, st)
         : mid <= 32768 ? run_heaviest<1024, 32, 0, false>(p, rows, st)
-        : mid <= 73728 ? run_heaviest<1024, 24, 48, false>(p, rows, st)
-                       : run_heaviest<1024, 0, 0, false>(p, rows, st);
+                       : run_heaviest<1024, 24, 48, false>(p, rows, st);
   }
   return s ? s : ok();
 }

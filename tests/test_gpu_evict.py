@@ -257,7 +257,7 @@ def test_heaviest_lengths_and_strides():
 
 
 @pytest.mark.parametrize("rows,width", [(7, 8193), (70, 16385), (74, 140003), (18, 140003), (3, 300001), (75, 40000),
-                                        (80, 90001),                                        (2, 600011)])
+                                        (80, 90001), (2, 600011)])
 def test_heaviest_rows_shared_by_several_blocks(rows, width):
     g = torch.Generator(device=DEV).manual_seed(width)
     w = torch.rand(rows, width, generator=g, device=DEV)
