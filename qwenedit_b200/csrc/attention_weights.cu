@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(kWarps * 32) attention_weights_kernel(const We
     const int j = (t - cached_tiles) * kKeys + lane;
     return t < last && lane < kKeys && j < drafted ? rq.lo + j : -1;
   };
-  for (int q0 = 0; q0 < rows || q0 == 0; q0 += q_rows) {
+  int q0 = 0;
+  do {  // once without query rows too: the keys get zeros
     int t_load = first + warp;
     int page = fetch(t_load);
     auto copy_next = [&](int stage) {
@@ -203,7 +204,8 @@ __global__ void __launch_bounds__(kWarps * 32) attention_weights_kernel(const We
     }
     cp_async_wait<0>();
     __syncwarp();
-  }
+    q0 += q_rows;
+  } while (q0 < rows);
 }
 
 // ---- many rows: S = Q K^T on the fifth-generation tensor cores ----------------------------------------------------
@@ -640,7 +642,8 @@ extern "C" int qe_attention_weights(const qe_attention_weights_args *args, void 
   const int max_tiles = std::max(1, (batch.max_length + kKeys - 1) / kKeys + (nodes + kKeys - 1) / kKeys);
   // tiles a CTA: the count that ends first by waves x (tiles + a start's 12), half a CTA more per request
   const int64_t all = (batch.sum_length + kKeys - 1) / kKeys + int64_t(batch.batch) * ((nodes + kKeys - 1) / kKeys);
-  p.q_rows = int(std::min<int64_t>((int64_t(batch.max_nodes) * p.group + 7) / 8 * 8, kQRows));
+  // at least one block, in a batch without new tokens too
+  p.q_rows = int(std::clamp<int64_t>((int64_t(batch.max_nodes) * p.group + 7) / 8 * 8, 8, kQRows));
   // (kept for the sizes asked for last on this thread: a model's layers ask for the same ones)
   thread_local std::array<int64_t, 6> last{-1};
   thread_local int64_t per = 0;

@@ -125,6 +125,25 @@ def test_outputs_whose_rows_overlap_are_refused():
         tree_attention(q, cache, tree, 0, kn, kn, out=same)
 
 
+@pytest.mark.parametrize("lens,hq,hkv,d,dtype", [([70], 28, 4, 128, torch.bfloat16), ([0, 700], 6, 2, 64, torch.float16),
+                                                 ([2000, 1, 130], 256, 1, 128, torch.bfloat16)])
+@pytest.mark.parametrize("draft", [False, True])
+def test_weights_of_a_batch_without_new_tokens(lens, hq, hkv, d, dtype, draft):
+    """Every request has finished: all weights are zero, and an accumulating call leaves them as they were."""
+    pool, slots, q, kn = _case(lens, [0] * len(lens), hq, hkv, d, dtype, 16, 0)
+    cache, tree = PagedBatch(pool, slots), DraftTree([0] * len(lens))
+    out, lse = tree_attention(q, cache, tree, 0, kn, kn, return_lse=True)
+    assert out.shape == (0, hq, d) and lse.shape == (hq, 0)
+    w = attention_weights(q, lse, cache, tree, 0, kn if draft else None)
+    assert w.shape == (len(lens), hkv, max(lens)) and not w.any()
+    base = torch.rand(len(lens), hkv, max(lens) + 5, device=DEV)
+    acc = base.clone()
+    attention_weights(q, lse, cache, tree, 0, kn if draft else None, out=acc, accumulate=True)
+    assert torch.equal(acc, base)
+    attention_weights(q, lse, cache, tree, 0, kn if draft else None, out=acc)
+    assert not acc.any()
+
+
 def test_weights_accumulate_into_a_wider_buffer():
     lens, counts, rooms = [130, 40], [2, 1], [200, 64]
     pool, slots, q, kn = _case(lens, counts, 28, 4, 128, torch.bfloat16, 64, 3, rooms=rooms)
