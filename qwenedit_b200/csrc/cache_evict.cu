@@ -360,6 +360,7 @@ __global__ void __launch_bounds__(256) retain_kernel(const RetainParams p) {
   const int chunks = kChunks > 0 ? kChunks : int(p.head_bytes / 16);
   constexpr int kUnroll = 8;
   const int total = kRows * chunks;
+  const int turns = (total + 31) / 32 * 32;  // whole warps: every lane takes the same turns, all of them shuffle
   for (int64_t item = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); item < p.items; item += warps) {
     const int64_t lh = item / p.blocks, i0 = (item - lh * p.blocks) * kRows;
     const int64_t layer = lh / p.heads, head = lh - layer * p.heads;
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(256) retain_kernel(const RetainParams p) {
     }
     const int f = int(from), t = int(to);  // pool_rows < 2^31; f < 0: nothing to move
     char *plane = p.base + layer * p.outer + head * p.head_bytes;
-    for (int c0 = lane; c0 < total; c0 += 32 * kUnroll) {
+    for (int c0 = lane; c0 < turns; c0 += 32 * kUnroll) {
       uint4 v[2][kUnroll];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {

@@ -323,6 +323,27 @@ def test_retain(layers, heads, d, dtype, page, length, n):
     assert pool.device_errors() == 0
 
 
+@pytest.mark.parametrize("d,dtype", [(8, torch.bfloat16), (4, torch.float32), (136, torch.bfloat16), (68, torch.float32),
+                                     (264, torch.float16), (16, torch.bfloat16), (40, torch.float16)])
+@pytest.mark.parametrize("layers,heads,length,n", [(1, 3, 60, 37), (4, 2, 2500, 1201), (28, 16, 1500, 700)])
+def test_retain_of_heads_of_odd_sizes(d, dtype, layers, heads, length, n):
+    """Heads of 1, 17 and 33 sixteen-byte chunks among them: a warp's last turn has chunks for half its lanes."""
+    pool, (src, dst) = R.make_pool(layers, heads, d, 1, [length, n], dtype, 3)
+    pool.kv.normal_()
+    g = torch.Generator(device=DEV).manual_seed(4)
+    keep = torch.rand(layers, heads, length, generator=g, device=DEV).topk(n).indices.sort().values.int()
+    keep[:, 1, ::3] = -1
+    want = pool.kv.clone()
+    for layer in range(layers):
+        for h in range(heads):
+            k = keep[layer, h].long()
+            there = k >= 0
+            want[layer, :, dst[there], h] = pool.kv[layer, :, src[k[there]], h]
+    pool.retain(src, keep, dst)
+    assert torch.equal(pool.kv, want)
+    assert pool.device_errors() == 0
+
+
 def test_retain_skips_and_reports_positions_past_the_sequence():
     pool, (src, dst) = R.make_pool(1, 2, 64, 1, [10, 4], torch.bfloat16, 3)
     pool.kv.normal_()
