@@ -461,6 +461,10 @@ int qe_index_evict(qe_index *ix, int64_t num_tokens, int64_t *out_evicted);
 int qe_index_alloc(qe_index *ix, int64_t n, int64_t *out_slots, int32_t *out_ok);
 /* allocator.free(slots) (paged.py:102). */
 int qe_index_free(qe_index *ix, const int64_t *slots, int64_t n);
+/* Gives allocated slots back that the tree does not hold (an addition; qe_index_free takes the caller's word for it,
+ * as insert's callers need). Each slot once; with pages, all the slots of each page that its allocation handed out.
+ * QE_ERR_STATE, with nothing freed, for slots that are free, twice in the call, in the tree, or part of a page. */
+int qe_index_give_back(qe_index *ix, const int64_t *slots, int64_t n);
 /* Permute the free list (seeded) so later allocations come from scattered pages. No counterpart in the
  * reference, whose allocator starts sorted: it builds a fragmented pool for tests and benchmarks. */
 int qe_index_shuffle_free(qe_index *ix, uint64_t seed);

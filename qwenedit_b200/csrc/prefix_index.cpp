@@ -78,6 +78,8 @@ struct Index {
   size_t free_head = 0;
   std::vector<int64_t> release_units;
   std::vector<uint8_t> unit_free;  // 1 when the unit is in free_units or release_units
+  std::vector<int32_t> unit_given;   // tokens of the unit that its last allocation handed out (page mode)
+  std::vector<int64_t> unit_cached;  // tokens of the unit that tree nodes hold
 
   uint64_t tick() { return ++clock; }
 
@@ -148,6 +150,8 @@ struct Index {
     release_units.clear();
     unit_free.assign(size_t(num_pages + 1), 1);
     unit_free[0] = 0;
+    unit_given.assign(page == 1 ? 0 : size_t(num_pages + 1), 0);
+    unit_cached.assign(size_t(num_pages + 1), 0);
   }
 
   // ---- keys ------------------------------------------------------------------------------
@@ -235,6 +239,20 @@ struct Index {
     *out_node = len ? handle(node) : 0;
   }
 
+  void count_cached(const std::vector<int64_t> &slots, int64_t sign) {
+    const size_t n = slots.size();
+    if (page == 1) {
+      for (int64_t slot : slots) unit_cached[size_t(slot)] += sign;
+      return;
+    }
+    for (size_t i = 0; i < n;) {  // a division per run of slots in a page
+      const int64_t unit = slots[i] / page, lo = unit * page;
+      const size_t from = i;
+      while (i < n && slots[i] >= lo && slots[i] < lo + page) ++i;
+      unit_cached[size_t(unit)] += sign * int64_t(i - from);
+    }
+  }
+
   int64_t insert(const int64_t *key, const int64_t *value, int64_t n) {
     n = aligned(n);
     uint64_t access = tick();
@@ -258,6 +276,7 @@ struct Index {
       l.parent = node;
       l.key.assign(key + pos, key + n);
       l.value.assign(value + pos, value + n);
+      count_cached(l.value, 1);
       nodes[node].children.push_back(leaf);
       evictable += n - pos;
     }
@@ -373,6 +392,7 @@ struct Index {
       int32_t x = it.node;
       if (x == root) break;
       if (nodes[x].lock_ref > 0) continue;
+      count_cached(nodes[x].value, -1);
       free_slots(nodes[x].value.data(), int64_t(nodes[x].value.size()), /*check=*/false);
       evicted += int64_t(nodes[x].value.size());
       int32_t parent = nodes[x].parent;
@@ -414,6 +434,8 @@ struct Index {
       }
     }
     for (int64_t i = 0; i < units; ++i) unit_free[size_t(u[i])] = 0;
+    if (page > 1)
+      for (int64_t i = 0; i < units; ++i) unit_given[size_t(u[i])] = int32_t(std::min<int64_t>(page, n - i * page));
     free_head += size_t(units);
     if (free_head == free_units.size()) {
       free_units.clear();
@@ -426,12 +448,16 @@ struct Index {
   bool free_slots(const int64_t *s, int64_t n, bool check) {
     if (n <= 0) return true;
     if (page == 1) {
-      if (check) {
-        for (int64_t i = 0; i < n; ++i)
-          if (s[i] < 1 || s[i] > num_pages || unit_free[size_t(s[i])]) return false;
-      }
-      for (int64_t i = 0; i < n; ++i) unit_free[size_t(s[i])] = 1;
+      const size_t before = release_units.size();
       release_units.insert(release_units.end(), s, s + n);
+      for (int64_t i = 0; i < n; ++i) {
+        if (check && (s[i] < 1 || s[i] > num_pages || unit_free[size_t(s[i])])) {  // twice in this call, too
+          for (int64_t j = 0; j < i; ++j) unit_free[size_t(s[j])] = 0;
+          release_units.resize(before);
+          return false;
+        }
+        unit_free[size_t(s[i])] = 1;
+      }
       return true;
     }
     // unique pages, ascending (torch.unique(free_index // page_size)); the slots of a page come as runs, so
@@ -448,9 +474,29 @@ struct Index {
       for (int64_t p : pages)
         if (p < 1 || p > num_pages || unit_free[size_t(p)]) return false;
     }
-    for (int64_t p : pages) unit_free[size_t(p)] = 1;
     release_units.insert(release_units.end(), pages.begin(), pages.end());
+    for (int64_t p : pages) unit_free[size_t(p)] = 1;
     return true;
+  }
+
+  // Frees allocated slots that no tree node holds: each once, in page mode with all the slots of their page that its
+  // allocation handed out. Returns what is wrong with them (nothing is freed then), or null.
+  const char *give_back(const int64_t *s, int64_t n) {
+    std::vector<int64_t> slots(s, s + n);
+    if (!std::is_sorted(slots.begin(), slots.end())) std::sort(slots.begin(), slots.end());
+    if (std::adjacent_find(slots.begin(), slots.end()) != slots.end()) return "a slot twice";
+    for (int64_t i = 0; i < n;) {
+      const int64_t unit = slots[size_t(i)] < page ? 0 : slots[size_t(i)] / page;
+      if (unit < 1 || unit > num_pages || unit_free[size_t(unit)]) return "slot out of range or already free";
+      if (unit_cached[size_t(unit)]) return "a slot that the tree holds (its own eviction frees it)";
+      const int64_t given = page == 1 ? 1 : unit_given[size_t(unit)];
+      int64_t here = 0;  // slots of this unit: its first ones, without a gap
+      while (here < given && i + here < n && slots[size_t(i + here)] == unit * page + here) ++here;
+      i += here;
+      if (here != given || (i < n && slots[size_t(i)] / page == unit)) return "a part of an allocated page";
+    }
+    free_slots(s, n, /*check=*/false);
+    return nullptr;
   }
 };
 
@@ -579,6 +625,17 @@ int qe_index_free(qe_index *ix, const int64_t *slots, int64_t n) {
       return fail(QE_ERR_STATE, "qe_index_free: slot out of range or already free");
   } catch (const std::bad_alloc &) {
     return fail(QE_ERR_NOMEM, "qe_index_free: out of host memory");
+  }
+  return qe::ok();
+}
+
+int qe_index_give_back(qe_index *ix, const int64_t *slots, int64_t n) {
+  QE_CHECK_ARG(ix, "qe_index_give_back: null index");
+  QE_CHECK_ARG(n >= 0 && (n == 0 || slots), "qe_index_give_back: bad slots");
+  try {
+    if (const char *wrong = ix->ix.give_back(slots, n)) return fail(QE_ERR_STATE, "qe_index_give_back: %s", wrong);
+  } catch (const std::bad_alloc &) {
+    return fail(QE_ERR_NOMEM, "qe_index_give_back: out of host memory");
   }
   return qe::ok();
 }

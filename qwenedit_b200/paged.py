@@ -111,6 +111,10 @@ class PrefixIndex:
         slots = np.ascontiguousarray(slots, dtype=np.int64)
         _lib.call("qe_index_free", self._h, _lib.ptr64(slots), len(slots))
 
+    def give_back(self, slots: np.ndarray) -> None:
+        slots = np.ascontiguousarray(slots, dtype=np.int64)
+        _lib.call("qe_index_give_back", self._h, _lib.ptr64(slots), len(slots))
+
     def usage(self) -> dict:
         out = np.zeros(4, np.int64)
         _lib.call("qe_index_usage", self._h, _lib.ptr64(out))
@@ -431,10 +435,12 @@ class PagedKVPool:
                       self._err.data_ptr(), self._stream())
 
     def free(self, indices: torch.Tensor) -> None:
-        """Gives slots from ``alloc`` that were never given to ``insert`` back to the allocator (an addition: e.g. a
-        request's own cache after ``retain``). In page mode whole pages: all the slots of an ``alloc``."""
+        """Gives slots from ``alloc`` back to the allocator (an addition: e.g. a request's own cache after ``retain``).
+        Refused, with nothing freed: slots that the tree holds (``insert``ed, or from ``match``: eviction frees those),
+        slots that are free already or stand twice, and, in page mode, a part of the slots that ``alloc`` handed out of
+        a page."""
         with self.lock:
-            self.index.free(self._host_slots(indices))
+            self.index.give_back(self._host_slots(indices))
 
     def gather_extra(self, indices: torch.Tensor) -> torch.Tensor:
         """``extra.index_select(0, indices)`` (encoder.py:114) as one gather launch."""

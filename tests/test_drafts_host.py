@@ -121,6 +121,99 @@ def test_retain_and_free():
         pool.free(slots)
 
 
+def _owners(pool):
+    """(free, evictable) tokens."""
+    return pool.usage()["free"], pool.usage()["evictable"]
+
+
+@pytest.mark.parametrize("page", [1, 4])
+def test_free_refuses_slots_of_the_tree(page):
+    pool = _pool(page=page)
+    a, b = pool.alloc(8), pool.alloc(8)
+    pool.insert(np.arange(100, 108), a, 0)
+    before = _owners(pool)
+    hit = pool.match(np.arange(100, 108))
+    mixed = torch.cat([hit.indices, b])
+    for bad in (a, a[:4], hit.indices, mixed):
+        with pytest.raises(_lib.QEError, match="tree"):
+            pool.free(bad)
+    assert _owners(pool) == (before[0], 0)  # locked by the match, none of b's freed
+    hit.release()
+    pool.free(b)
+    assert _owners(pool) == (before[0] + 8, before[1])
+    rest = pool.alloc(pool.usage()["free"])  # all that is free: nothing of the tree among it
+    assert not set(rest.tolist()) & set(a.tolist())
+    # what eviction gave back is free once, and can be handed out and given back again
+    assert pool.index.evict(8) == 8
+    with pytest.raises(_lib.QEError, match="already free"):
+        pool.free(a)
+    again = pool.alloc(8)
+    assert sorted(again.tolist()) == sorted(a.tolist())
+    pool.free(again)
+    pool.free(rest)
+    assert _owners(pool) == (32, 0)
+
+
+def test_free_after_a_split_and_a_partial_eviction():
+    pool = _pool(page=4)
+    a = pool.alloc(12)
+    pool.insert(np.arange(12), a, 0)
+    c = pool.alloc(4)
+    pool.insert(np.r_[np.arange(8), 50, 51, 52, 53], torch.cat([a[:8], c]), 8)  # splits a's node
+    assert pool.index.evict(4) == 4  # one of the two tails
+    with pytest.raises(_lib.QEError, match="tree"):
+        pool.free(a[:8])
+    assert pool.index.evict(100) == 12
+    with pytest.raises(_lib.QEError, match="already free"):
+        pool.free(a[:8])
+    assert len(set(pool.alloc(32).tolist())) == 32
+    pool.clear()
+    pool.free(pool.alloc(32))
+
+
+@pytest.mark.parametrize("page", [1, 4])
+def test_free_refuses_a_slot_twice(page):
+    pool = _pool(page=page)
+    a = pool.alloc(8)
+    for bad in (torch.cat([a, a]), torch.cat([a, a[:1]]), torch.cat([a[4:], a[:4], a[4:]])):
+        with pytest.raises(_lib.QEError, match="twice"):
+            pool.free(bad)
+    assert pool.usage()["free"] == 24
+    pool.free(a.flip(0))  # any order
+    assert len(set(pool.alloc(32).tolist())) == 32
+
+
+def test_free_of_the_c_index_marks_as_it_checks():
+    pool = _pool(page=1)
+    a = pool.alloc(8).numpy()
+    with pytest.raises(_lib.QEError, match="already free"):
+        pool.index.free(np.r_[a, a[:1]])
+    assert pool.usage()["free"] == 24
+    pool.index.free(a)
+    assert len(set(pool.alloc(32).tolist())) == 32
+
+
+def test_free_takes_whole_pages_as_they_were_handed_out():
+    pool = _pool(page=4)
+    a, b = pool.alloc(6), pool.alloc(4)  # pages 1, 2 (two slots of it), 3
+    for bad in (a[:5], a[4:5], a[5:], a[1:4], torch.cat([a[:4], b[:3]]), torch.tensor([*a[:4].tolist(), 8, 9, 10])):
+        with pytest.raises(_lib.QEError, match="part of an allocated page"):
+            pool.free(bad)
+    for bad in (torch.tensor([0, 1, 2, 3]), torch.tensor([-4, -3]), torch.arange(36, 40)):
+        with pytest.raises(_lib.QEError, match="out of range"):
+            pool.free(bad)
+    assert pool.usage()["free"] == 20
+    pool.free(a[4:])  # its second page
+    assert pool.alloc(25) is None and pool.usage()["free"] == 24
+    d = pool.alloc(24)  # that page anew, whole now
+    assert set(range(8, 12)) <= set(d.tolist())
+    with pytest.raises(_lib.QEError, match="part of an allocated page"):
+        pool.free(torch.tensor([8, 9]))
+    pool.free(torch.cat([d, a[:4], b]))
+    assert pool.usage()["free"] == 32
+    pool.free(torch.empty(0, dtype=torch.int64))
+
+
 def _batch(**over):
     base = dict(starts=16, lengths=16, tables=16, masks=0, batch=1, table_width=2, page_size=4, mask_words=0, mode=0,
                 total=3, max_nodes=3, max_length=8, sum_length=8)
