@@ -139,16 +139,37 @@ class Match:
             self.node = None
 
 
+def _mirror(t: torch.Tensor) -> np.ndarray | None:
+    """The host copy that a slot tensor carries, while the tensor holds what it did when the copy was attached."""
+    host = getattr(t, "_qe_host", None)
+    if host is None or t.is_inference():  # tensors made in inference mode do not count their changes
+        return host
+    version = t._version
+    if getattr(t, "_qe_version", version) != version:
+        del t._qe_host, t._qe_version
+        t._qe_pages = None
+        return None
+    t._qe_version = version
+    return host
+
+
+def _attach(t: torch.Tensor, host: np.ndarray) -> torch.Tensor:
+    t._qe_host, t._qe_pages = host, None
+    if not t.is_inference():
+        t._qe_version = t._version
+    return t
+
+
 def _slots_tensor(host: np.ndarray, pool: "PagedKVPool") -> torch.Tensor:
     """Device int64 slot tensor with its host mirror attached (no sync needed to inspect it later)."""
-    cpu = torch.from_numpy(host)
-    if pool.device.type == "cuda":
-        t = cpu.pin_memory().to(pool.device, non_blocking=True)
-        pool.h2d_bytes += host.nbytes
-    else:
-        t = cpu.to(pool.device)
-    t._qe_host = host
-    return t
+    with torch.inference_mode(False):  # a tensor that counts its changes
+        cpu = torch.from_numpy(host)
+        if pool.device.type == "cuda":
+            t = cpu.pin_memory().to(pool.device, non_blocking=True)
+            pool.h2d_bytes += host.nbytes
+        else:
+            t = cpu.to(pool.device)
+        return _attach(t, host)
 
 
 COPY_MODES = {"auto": 0, "warp": 1, "bulk": 2, "warp_row": 3, "warp16": 4}
@@ -163,11 +184,10 @@ def set_copy_mode(mode: str) -> None:
 
 def cat_slots(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     """``torch.cat([a, b])`` of slot tensors, keeping the host mirror when both carry one."""
-    out = torch.cat([a, b])
-    ha, hb = getattr(a, "_qe_host", None), getattr(b, "_qe_host", None)
-    if ha is not None and hb is not None:
-        out._qe_host = np.concatenate([ha, hb])
-    return out
+    ha, hb = _mirror(a), _mirror(b)
+    with torch.inference_mode(False):
+        out = torch.cat([a, b])
+        return out if ha is None or hb is None else _attach(out, np.concatenate([ha, hb]))
 
 
 def pool_geometry(layers, heads, head_dim, budget_bytes, dtype, extra_dim=0, page_size=1) -> tuple[int, int, int]:
@@ -268,10 +288,13 @@ class PagedKVPool:
 
     # ---- data movement -----------------------------------------------------------------------
     def _host_slots(self, indices: torch.Tensor) -> np.ndarray:
-        host = getattr(indices, "_qe_host", None)
+        """The slots on the host: the copy that the tensor carries, or, where it has none or was written in place since
+        (by torch: a kernel's or a replayed graph's own writes do not show), read from it."""
+        host = _mirror(indices)
         if host is None:
             host = indices.detach().to("cpu", torch.int64).numpy().reshape(-1)
-            indices._qe_host = host
+            if not indices.is_inference():
+                _attach(indices, host)
         return host
 
     def _row_bytes(self, t: torch.Tensor) -> int:
@@ -296,7 +319,8 @@ class PagedKVPool:
         bt = torch.from_numpy(pages.astype(np.int32))
         bt = bt.pin_memory().to(self.device, non_blocking=True)
         self.h2d_bytes += bt.numel() * 4
-        indices._qe_pages = bt
+        if getattr(indices, "_qe_host", None) is not None:  # kept as long as the host copy
+            indices._qe_pages = bt
         return bt
 
     def _require_cuda(self, *tensors: torch.Tensor) -> None:
@@ -368,7 +392,7 @@ class PagedKVPool:
         self._require_cuda(indices, kv)
         if kv.stride(4) != 1 or kv.stride(3) != self.head_dim or kv.stride(2) != self.heads * self.head_dim:
             kv = kv.contiguous()
-        host = getattr(indices, "_qe_host", None)
+        host = _mirror(indices)
         self._copy("append", self.kv, kv, indices, host, n_planes=2 * self.layers)
 
     def write_layers(self, indices: torch.Tensor, keys: list[torch.Tensor], values: list[torch.Tensor]) -> None:
@@ -463,7 +487,7 @@ class PagedKVPool:
             raise ValueError(f"extra rows must be [{n}, {self.extra_dim}]")
         if n:
             self._require_cuda(indices, rows)
-            self._copy_extra("append", rows, indices, getattr(indices, "_qe_host", None))
+            self._copy_extra("append", rows, indices, _mirror(indices))
 
     def _check_kv_shape(self, t: torch.Tensor, n: int) -> None:
         want = (self.layers, 2, n, self.heads, self.head_dim)

@@ -10,7 +10,7 @@ import torch
 from qwenedit_b200 import _lib
 from qwenedit_b200.drafts import DraftTree, PagedBatch, _check_apart, tree_attention
 from qwenedit_b200.evict import attention_weights, heaviest
-from qwenedit_b200.paged import PagedKVPool
+from qwenedit_b200.paged import PagedKVPool, cat_slots
 
 
 def _pool(page=4, dtype=torch.bfloat16, d=64, heads=2):
@@ -33,6 +33,48 @@ def test_batch_needs_whole_pages_in_the_pool():
         with pytest.raises(ValueError, match="lengths"):
             PagedBatch(pool, [run, None, None], lengths)
     assert PagedBatch(_pool(page=1), [torch.tensor([5, 3, 9])]).tables.tolist() == [[5, 3, 9]]
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_slots_written_in_place_are_read_again(dtype):
+    pool = _pool(page=1)
+    slots = torch.tensor([5, 3, 9], dtype=dtype)
+    assert PagedBatch(pool, [slots]).tables.tolist() == [[5, 3, 9]]
+    slots[1] = 7
+    assert PagedBatch(pool, [slots]).tables.tolist() == [[5, 7, 9]]
+    with torch.inference_mode():
+        slots.add_(1)
+        assert PagedBatch(pool, [slots]).tables.tolist() == [[6, 8, 10]]
+    tail = slots[1:]
+    assert PagedBatch(pool, [tail]).tables.tolist() == [[8, 10]]
+    slots[2] = 1  # through the tensor that it is a view of
+    assert PagedBatch(pool, [tail]).tables.tolist() == [[8, 1]]
+    slots[0] = pool.rows
+    with pytest.raises(ValueError, match="outside the pool"):
+        PagedBatch(pool, [slots])
+    with torch.inference_mode():  # tensors that do not count their changes
+        own = torch.tensor([5, 3], dtype=dtype)
+        assert PagedBatch(pool, [own]).tables.tolist() == [[5, 3]]
+        own[0] = 4
+        assert PagedBatch(pool, [own]).tables.tolist() == [[4, 3]]
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_allocated_slots_written_in_place_are_read_again(inference):
+    pool = _pool(page=4)
+    with torch.inference_mode(inference):
+        a = pool.alloc(8)
+        both = cat_slots(a, pool.alloc(4))
+        assert PagedBatch(pool, [both]).tables.tolist() == [[1, 2, 3]]
+        a.copy_(a.flip(0).reshape(2, 4).flip(1).reshape(-1))  # its pages the other way round
+        both[:8] = a
+        assert PagedBatch(pool, [a, both, cat_slots(both, a)]).tables.tolist() == [
+            [2, 1, -1, -1, -1], [2, 1, 3, -1, -1], [2, 1, 3, 2, 1]]
+        pool.insert(np.arange(12), both, 0)
+        hit = pool.match(np.arange(12))
+        assert hit.indices.tolist() == both.tolist()
+        hit.indices[:4] = 0
+        assert pool.match(np.arange(12)).indices.tolist() == both.tolist()
 
 
 def test_tree_counts_parents_and_masks():

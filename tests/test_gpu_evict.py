@@ -366,6 +366,29 @@ def test_retain_past_32_bit_offsets():
     assert torch.equal(kv[:, :, dst], kv[:, :, src[::4]])
 
 
+def test_slots_written_in_place_are_seen():
+    """The host's copy of a slot tensor is read anew after a write: by retain's checks, batches, copies."""
+    pool = PagedKVPool("written", 1, 2, 64, 16 * 16 * 2 * 2 * 64 * 2, torch.bfloat16, DEV, page_size=16)
+    pool.kv.normal_()
+    src, dst = pool.alloc(64), pool.alloc(32)
+    keep = torch.arange(32, dtype=torch.int32, device=DEV).broadcast_to(1, 2, 32)
+    pool.gather(src)
+    pool.retain(src, keep, dst)
+    dst[5] = src[40]
+    with pytest.raises(ValueError, match="twice, or among"):
+        pool.retain(src, keep, dst)
+    dst[5] = dst[6]
+    with pytest.raises(ValueError, match="twice, or among"):
+        pool.retain(src, keep, dst)
+    src.copy_(src.reshape(4, 16).flip(0).reshape(-1))
+    assert torch.equal(pool.gather(src), pool.kv[:, :, src])
+    assert PagedBatch(pool, [src]).tables.tolist() == [[4, 3, 2, 1]]
+    new = torch.randn(1, 2, 64, 2, 64, device=DEV).bfloat16()
+    src.copy_(src.roll(16))
+    pool.write(src, new)
+    assert torch.equal(pool.kv[:, :, src], new)
+
+
 # ---- together ------------------------------------------------------------------------------------------------------
 
 def test_decode_evict_decode():
