@@ -78,6 +78,7 @@ class PrefixIndex:
             self._h = None
 
     def match(self, key: np.ndarray) -> tuple[int, np.ndarray, int]:
+        key = np.ascontiguousarray(key, dtype=np.int64)
         n = len(key)
         out = np.empty(max(n, 1), np.int64)
         length, node = ctypes.c_int64(), ctypes.c_uint64()
@@ -92,6 +93,7 @@ class PrefixIndex:
         _lib.call("qe_index_unlock", self._h, node)
 
     def insert(self, key: np.ndarray, slots: np.ndarray) -> int:
+        key, slots = np.ascontiguousarray(key, dtype=np.int64), np.ascontiguousarray(slots, dtype=np.int64)
         present = ctypes.c_int64()
         _lib.call("qe_index_insert", self._h, _lib.ptr64(key), _lib.ptr64(slots), len(key), ctypes.byref(present))
         return present.value
@@ -448,7 +450,7 @@ class PagedKVPool:
         if n == 0:
             return
         self._require_cuda(indices, keep, slots)
-        src, dst = self._host_slots(indices), self._host_slots(slots)
+        src, dst = (np.ascontiguousarray(self._host_slots(t), dtype=np.int64) for t in (indices, slots))
         keep = keep.contiguous()
         src_t = (indices if indices.dtype == torch.int64 else indices.to(torch.int64)).contiguous()
         dst_t = (slots if slots.dtype == torch.int64 else slots.to(torch.int64)).contiguous()

@@ -217,6 +217,17 @@ def test_misuse_raises():
     assert ours.usage() == before and ours.match(np.arange(100, 104)).length == 0
 
 
+def test_slots_with_gaps_in_memory():
+    """Slot tensors on the CPU that are views with a step are taken by value, like contiguous ones."""
+    ours, _ = pools(32)
+    a = torch.from_numpy(ours.alloc(16)._qe_host.copy())
+    ours.insert(np.arange(8), a[::2], 0)
+    assert ours.match(np.arange(8)).indices._qe_host.tolist() == a[::2].tolist()
+    key = np.arange(100, 116)
+    assert ours.index.insert(key[::2], a[1::2].numpy()) == 0
+    assert ours.index.match(key[::2])[1].tolist() == a[1::2].tolist()
+
+
 def test_clear_resets_everything():
     ours, ref = pools(64)
     for pool in (ours, ref):
