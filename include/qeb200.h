@@ -327,9 +327,9 @@ int qe_latent_crop(const void *src, void *out, int64_t h, int64_t w, int64_t row
  * its row of `masks` ([total][mask_words] 32-bit words, bit j % 32 of word j / 32 = node j of the same request),
  * 2 all. starts, lengths, tables and masks are device memory and are read when the kernel runs, so a captured graph
  * replays with their current values; `total` and max_nodes bound the nodes of the batch and of one request,
- * max_length and sum_length the cached tokens of one request and of all (they size the grid and the split, nothing
- * past tables' room is read whatever they say: cached tokens past max_length are not attended to). A page outside
- * the pool reads as zeros and sets bit 1 of *err_flag. */
+ * max_length and sum_length the cached tokens of one request and of all (max_nodes and max_length at most 2^30; they
+ * size the grid and the split, nothing past tables' room is read whatever they say: cached tokens past max_length are
+ * not attended to). A page outside the pool reads as zeros and sets bit 1 of *err_flag. */
 typedef struct qe_draft_batch {
   const int32_t *starts;   /* [batch + 1] */
   const int32_t *lengths;  /* [batch] */

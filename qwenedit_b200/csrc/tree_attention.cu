@@ -18,11 +18,15 @@
 
 namespace qe {
 
+// the counts of key tiles and their sums stay within 32 bits
+static bool bounded(const qe_draft_batch &in) { return in.max_length <= 1 << 30 && in.max_nodes <= 1 << 30; }
+
 int decode_batch(const char *who, const qe_draft_batch &in, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
                  int32_t dtype, int64_t pool_rows, bool has_pool, int32_t *err, DecodeBatch *out) {
   QE_CHECK_ARG(in.batch >= 0 && in.batch <= 65535 && in.total >= 0 && in.max_nodes >= 0 && in.max_length >= 0 &&
                    in.sum_length >= 0 && in.table_width >= 0,
                "%s: negative size, or more than 65535 requests", who);
+  QE_CHECK_ARG(bounded(in), "%s: max_length or max_nodes passes 2^30", who);
   QE_CHECK_ARG(heads_q >= 1 && heads_kv >= 1 && heads_q % heads_kv == 0 && heads_q <= 65535,
                "%s: heads_q must be a positive multiple of heads_kv (at most 65535)", who);
   QE_CHECK_ARG(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128", who);
@@ -1386,6 +1390,7 @@ extern "C" int qe_tree_attention_workspace(const qe_tree_attention_args *args, i
                    batch.sum_length >= 0 && args->heads_q >= 1 && args->heads_kv >= 1 &&
                    args->heads_q % args->heads_kv == 0 && (args->head_dim == 64 || args->head_dim == 128),
                "qe_tree_attention_workspace: bad size");
+  QE_CHECK_ARG(bounded(batch), "qe_tree_attention_workspace: max_length or max_nodes passes 2^30");
   *bytes = tree_plan(batch, args->heads_q, args->heads_kv, args->head_dim).workspace;
   return ok();
 }

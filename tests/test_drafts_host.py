@@ -291,6 +291,21 @@ def test_c_tree_attention_rejects(kw, match):
         _attend(**kw)
 
 
+@pytest.mark.parametrize("over", [dict(max_length=2**31 - 1), dict(max_nodes=2**31 - 1), dict(max_length=2**30 + 1)])
+def test_c_bounds_whose_tiles_would_pass_32_bits_are_refused(over):
+    """Loose bounds on the sizes of a batch are welcome, but not such that the counts of key tiles wrap round (a
+    workspace of no bytes, and splits without room for their parts)."""
+    batch, size = _batch(**over), ctypes.c_int64(-1)
+    with pytest.raises(ValueError, match="2\\^30"):
+        _lib.call("qe_tree_attention_workspace", _tree_args(batch), ctypes.byref(size))
+    with pytest.raises(ValueError, match="2\\^30"):
+        _attend(batch)
+    with pytest.raises(ValueError, match="2\\^30"):
+        _lib.call("qe_attention_weights", batch + _weights_args(width=2**33)[len(batch):], None)
+    _lib.call("qe_tree_attention_workspace", _tree_args(_batch(max_length=2**30, sum_length=2**30)), ctypes.byref(size))
+    assert size.value > 0
+
+
 def test_c_entry_points_reject_and_accept_nothing():
     size = ctypes.c_int64(-1)
     long = _batch(max_length=1 << 20, sum_length=1 << 20)
