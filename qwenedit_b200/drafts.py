@@ -217,8 +217,8 @@ def _view(cache: PagedBatch, tree: DraftTree) -> _View:
                                   0 if tree.masks is None else tree.masks.data_ptr(), cache.batch, cache.table_width,
                                   cache.pool.page_size, tree.words, tree.mode, tree.total, tree.max_nodes,
                                   cache.max_length, cache.sum_length)
-    tree._view = _View(cache, batch)
-    return tree._view
+    view = tree._view = _View(cache, batch)
+    return view  # (the tree's may be another thread's by now)
 
 
 def _check_rows(name: str, t: torch.Tensor, n: int, heads: int, head_dim: int, dtype, device) -> None:

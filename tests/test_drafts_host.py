@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from qwenedit_b200 import _lib
-from qwenedit_b200.drafts import DraftTree, PagedBatch, _check_apart, tree_attention
+from qwenedit_b200.drafts import DraftTree, PagedBatch, _check_apart, _view, tree_attention
 from qwenedit_b200.evict import attention_weights, heaviest
 from qwenedit_b200.paged import PagedKVPool, cat_slots
 
@@ -107,6 +107,26 @@ def _args(pool=None, n=3, hq=4, dtype=torch.bfloat16):
     pool = _pool() if pool is None else pool
     rand = lambda h: torch.zeros(n, h, pool.head_dim, dtype=dtype)  # noqa: E731
     return rand(hq), PagedBatch(pool, [torch.arange(4, 8)]), DraftTree([n], device="cpu"), 0, rand(pool.heads), rand(pool.heads)
+
+
+def test_a_tree_shared_by_threads_with_their_own_caches():
+    """Between one thread's storing of its view with the tree and its next line another thread stores its own."""
+    pool = _pool()
+    ours, theirs = PagedBatch(pool, [torch.arange(4, 8)]), PagedBatch(pool, [torch.arange(8, 20)])
+
+    class Shared(DraftTree):
+        @property
+        def _view(self):
+            return self.stored
+
+        @_view.setter
+        def _view(self, view):
+            self.stored = view if view is None else _view(theirs, DraftTree([3], device="cpu"))
+
+    tree = Shared([3], device="cpu")
+    view = _view(ours, tree)
+    assert view.cache is ours and view.batch == _view(ours, tree).batch
+    assert tree.stored.cache is theirs
 
 
 def test_tree_attention_refuses_before_any_launch():
