@@ -2,6 +2,8 @@
 ``PagedKVPool.retain`` / ``free`` against plain indexing, and the operators together, as a decoding program calls
 them."""
 
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
@@ -439,4 +441,43 @@ def test_decode_evict_decode():
             assert bool(((lse[:, :1].double() - ref_lse).abs() <= lse_tol).all())
             assert keep[layer, h].tolist()[:2] == [0, 1] and keep[layer, h, -1].item() == length - 1
     assert cat_slots(small, slots[1]).numel() == budget + lens[1] + steps
+    assert pool.device_errors() == 0
+
+
+@pytest.mark.parametrize("page,dtype", [(16, torch.bfloat16), (1, torch.float16)])
+def test_attention_over_a_cut_cache_is_that_over_the_kept_tokens(page, dtype):
+    """The reference takes each head's keys from a copy of the pool made before ``retain``, by ``keep``; and ``keep``
+    is what the accumulated weights call for."""
+    layers, hq, hkv, d, length, budget, sinks, recent = 3, 12, 3, 64, 210, 70, 2, 8
+    pool, (slots, small) = R.make_pool(layers, hkv, d, page, [length, budget], dtype, 7)
+    R.fill(pool, [slots], [length], 1)
+    cache, tree, scale = PagedBatch(pool, [slots]), DraftTree([5]), R.default_scale(d)
+    g = torch.Generator(device=DEV).manual_seed(2)
+    rand = lambda n, h: torch.randn(n, h, d, generator=g, device=DEV).to(dtype)  # noqa: E731
+    acc = torch.zeros(layers, 1, hkv, length, device=DEV)
+    for layer in range(layers):
+        q = rand(5, hq) * 2
+        _, lse = tree_attention(q, cache, tree, layer, return_lse=True)
+        attention_weights(q, lse, cache, tree, layer, out=acc[layer])
+    keep, kept = heaviest(acc[:, 0], budget, sinks=sinks, recent=recent)
+    rows = acc[:, 0].cpu().numpy()
+    for layer in range(layers):
+        for h in range(hkv):
+            want = _heaviest_ref(rows[layer, h], length, budget, sinks, recent)
+            assert keep[layer, h].tolist() == want
+            np.testing.assert_array_equal(kept[layer, h].cpu().numpy(), rows[layer, h][want])
+    before = pool.kv.clone()
+    pool.retain(slots, keep, small)
+    after, one = PagedBatch(pool, [small]), DraftTree([1])
+    group = hq // hkv
+    for layer in range(layers):
+        q, kn, vn = rand(1, hq) * 2, rand(1, hkv), rand(1, hkv)
+        out, lse = tree_attention(q, after, one, layer, kn, vn, return_lse=True)
+        for h in range(hkv):
+            mine = slice(h * group, (h + 1) * group)
+            head = SimpleNamespace(kv=before[:, :, :, h : h + 1], heads=1)
+            ref, ref_lse, tol, lse_tol = R.attention64(head, layer, slots[keep[layer, h].long()], budget, q[:, mine],
+                                                       kn[:, h : h + 1], vn[:, h : h + 1], R.chain(1), scale)
+            assert bool(((out[:, mine].double() - ref).abs() <= tol).all())
+            assert bool(((lse[mine].double() - ref_lse).abs() <= lse_tol).all())
     assert pool.device_errors() == 0
