@@ -129,7 +129,8 @@ class DraftTree:
 
     @property
     def starts(self) -> torch.Tensor:
-        """[batch + 1] int32: the first node of each request, on the device (in place only)."""
+        """[batch + 1] int32: the first node of each request, on the device (for kernels to read: the counts are fixed, and
+        a call's outputs have their rows)."""
         return self._starts
 
     @property
