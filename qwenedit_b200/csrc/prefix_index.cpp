@@ -79,7 +79,7 @@ struct Index {
   std::vector<int64_t> release_units;
   std::vector<uint8_t> unit_free;  // 1 when the unit is in free_units or release_units
   std::vector<int32_t> unit_given;   // tokens of the unit that its last allocation handed out (page mode)
-  std::vector<int64_t> unit_cached;  // tokens of the unit that tree nodes hold
+  std::vector<int32_t> unit_cached;  // tokens of the unit that tree nodes hold
 
   uint64_t tick() { return ++clock; }
 
@@ -239,17 +239,22 @@ struct Index {
     *out_node = len ? handle(node) : 0;
   }
 
-  void count_cached(const std::vector<int64_t> &slots, int64_t sign) {
-    const size_t n = slots.size();
+  void count_cached(const std::vector<int64_t> &slots, int32_t sign) {
+    const int64_t n = int64_t(slots.size()), *s = slots.data();
     if (page == 1) {
-      for (int64_t slot : slots) unit_cached[size_t(slot)] += sign;
+      for (int64_t i = 0; i < n; ++i) unit_cached[size_t(s[i])] += sign;
       return;
     }
-    for (size_t i = 0; i < n;) {  // a division per run of slots in a page
-      const int64_t unit = slots[i] / page, lo = unit * page;
-      const size_t from = i;
-      while (i < n && slots[i] >= lo && slots[i] < lo + page) ++i;
-      unit_cached[size_t(unit)] += sign * int64_t(i - from);
+    for (int64_t i = 0; i < n;) {  // a division and a scan without a branch per whole page, the usual run
+      const int64_t unit = s[i] / page;
+      int64_t run = 1;
+      if (i + page <= n && s[i] == unit * page) {
+        int64_t differ = 0;
+        for (int64_t o = 1; o < page; ++o) differ |= s[i + o] ^ (s[i] + o);
+        if (!differ) run = page;
+      }
+      unit_cached[size_t(unit)] += sign * int32_t(run);
+      i += run;
     }
   }
 

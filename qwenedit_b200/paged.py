@@ -59,6 +59,11 @@ def _as_key(vids) -> np.ndarray:
     return np.ascontiguousarray(vids, dtype=np.int64).reshape(-1)
 
 
+def _flat64(a) -> np.ndarray:
+    """`a` as int64 values without gaps (itself where it is that already)."""
+    return a if a.dtype == np.int64 and a.flags.c_contiguous else np.ascontiguousarray(a, dtype=np.int64)
+
+
 class PrefixIndex:
     """Owning wrapper of a native ``qe_index`` (radix tree + allocator + LRU)."""
 
@@ -78,7 +83,7 @@ class PrefixIndex:
             self._h = None
 
     def match(self, key: np.ndarray) -> tuple[int, np.ndarray, int]:
-        key = np.ascontiguousarray(key, dtype=np.int64)
+        key = _flat64(key)
         n = len(key)
         out = np.empty(max(n, 1), np.int64)
         length, node = ctypes.c_int64(), ctypes.c_uint64()
@@ -93,7 +98,7 @@ class PrefixIndex:
         _lib.call("qe_index_unlock", self._h, node)
 
     def insert(self, key: np.ndarray, slots: np.ndarray) -> int:
-        key, slots = np.ascontiguousarray(key, dtype=np.int64), np.ascontiguousarray(slots, dtype=np.int64)
+        key, slots = _flat64(key), _flat64(slots)
         present = ctypes.c_int64()
         _lib.call("qe_index_insert", self._h, _lib.ptr64(key), _lib.ptr64(slots), len(key), ctypes.byref(present))
         return present.value
@@ -114,7 +119,7 @@ class PrefixIndex:
         _lib.call("qe_index_free", self._h, _lib.ptr64(slots), len(slots))
 
     def give_back(self, slots: np.ndarray) -> None:
-        slots = np.ascontiguousarray(slots, dtype=np.int64)
+        slots = _flat64(slots)
         _lib.call("qe_index_give_back", self._h, _lib.ptr64(slots), len(slots))
 
     def usage(self) -> dict:
@@ -143,35 +148,38 @@ class Match:
 
 def _mirror(t: torch.Tensor) -> np.ndarray | None:
     """The host copy that a slot tensor carries, while the tensor holds what it did when the copy was attached."""
-    host = getattr(t, "_qe_host", None)
+    held = t.__dict__
+    host = held.get("_qe_host")
     if host is None or t.is_inference():  # tensors made in inference mode do not count their changes
         return host
     version = t._version
-    if getattr(t, "_qe_version", version) != version:
-        del t._qe_host, t._qe_version
-        t._qe_pages = None
-        return None
-    t._qe_version = version
-    return host
+    if held.setdefault("_qe_version", version) == version:
+        return host
+    del t._qe_host, t._qe_version
+    t._qe_pages = None
+    return None
 
 
 def _attach(t: torch.Tensor, host: np.ndarray) -> torch.Tensor:
-    t._qe_host, t._qe_pages = host, None
+    held = t.__dict__
+    held["_qe_host"], held["_qe_pages"] = host, None
     if not t.is_inference():
-        t._qe_version = t._version
+        held["_qe_version"] = t._version
     return t
 
 
 def _slots_tensor(host: np.ndarray, pool: "PagedKVPool") -> torch.Tensor:
     """Device int64 slot tensor with its host mirror attached (no sync needed to inspect it later)."""
-    with torch.inference_mode(False):  # a tensor that counts its changes
-        cpu = torch.from_numpy(host)
-        if pool.device.type == "cuda":
-            t = cpu.pin_memory().to(pool.device, non_blocking=True)
-            pool.h2d_bytes += host.nbytes
-        else:
-            t = cpu.to(pool.device)
-        return _attach(t, host)
+    if torch.is_inference_mode_enabled():  # a tensor that counts its changes there too
+        with torch.inference_mode(False):
+            return _slots_tensor(host, pool)
+    cpu = torch.from_numpy(host)
+    if pool.device.type == "cuda":
+        t = cpu.pin_memory().to(pool.device, non_blocking=True)
+        pool.h2d_bytes += host.nbytes
+    else:
+        t = cpu.to(pool.device)
+    return _attach(t, host)
 
 
 COPY_MODES = {"auto": 0, "warp": 1, "bulk": 2, "warp_row": 3, "warp16": 4}
@@ -450,7 +458,7 @@ class PagedKVPool:
         if n == 0:
             return
         self._require_cuda(indices, keep, slots)
-        src, dst = (np.ascontiguousarray(self._host_slots(t), dtype=np.int64) for t in (indices, slots))
+        src, dst = (_flat64(self._host_slots(t)) for t in (indices, slots))
         keep = keep.contiguous()
         src_t = (indices if indices.dtype == torch.int64 else indices.to(torch.int64)).contiguous()
         dst_t = (slots if slots.dtype == torch.int64 else slots.to(torch.int64)).contiguous()
