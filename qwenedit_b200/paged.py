@@ -155,8 +155,8 @@ def _mirror(t: torch.Tensor) -> np.ndarray | None:
     version = t._version
     if held.setdefault("_qe_version", version) == version:
         return host
-    del t._qe_host, t._qe_version
-    t._qe_pages = None
+    for name in ("_qe_host", "_qe_pages", "_qe_version"):  # (another thread may have found the same)
+        held.pop(name, None)
     return None
 
 
